@@ -19,7 +19,7 @@ import torch  # noqa: F401  (must precede the library load, see module docstring
 LIB_PATH = Path(os.environ.get("FFTSPARSE_AMD_LIB") or Path(__file__).resolve().with_name("libfftsparse_amd.so"))
 
 FS_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 
 class PoolArgs(ctypes.Structure):
@@ -117,12 +117,58 @@ class AttnArgs(ctypes.Structure):
                 ("blk_cnt", c_void_p), ("blk_bits", c_void_p), ("work", c_void_p)]
 
 
-STRUCTS = [PoolArgs, CorrArgs, StatsArgs, SelectArgs, AttnArgs, ScoresArgs, RopePoolArgs, XattnArgs, FlexArgs]
+class PlanArgs(ctypes.Structure):
+    _fields_ = [("block_table", c_void_p), ("t_sb", c_int64), ("seq_lens", c_void_p), ("new_lens", c_void_p),
+                ("free_pages", c_void_p), ("free_count", c_void_p),
+                ("B", c_int), ("P", c_int), ("F", c_int), ("page_size", c_int), ("T", c_int),
+                ("cu_lens", c_void_p), ("seq_lens_out", c_void_p), ("positions", c_void_p), ("slots", c_void_p),
+                ("free_count_out", c_void_p), ("lacking", c_void_p)]
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_st", c_int64), ("q_sh", c_int64),
+                ("k", c_void_p), ("k_st", c_int64), ("k_sh", c_int64),
+                ("v", c_void_p), ("v_st", c_int64), ("v_sh", c_int64),
+                ("positions", c_void_p), ("inv_freq", c_void_p), ("attention_factor", c_float),
+                ("pos_bytes", c_int), ("half", c_int), ("interleaved", c_int),
+                ("dtype", c_int), ("T", c_int), ("Hq", c_int), ("Hk", c_int), ("D", c_int),
+                ("q_out", c_void_p), ("qo_st", c_int64), ("qo_sh", c_int64),
+                ("k_out", c_void_p), ("ko_st", c_int64), ("ko_sh", c_int64),
+                ("slots", c_void_p),
+                ("k_cache", c_void_p), ("kc_sp", c_int64), ("kc_ss", c_int64), ("kc_sh", c_int64),
+                ("v_cache", c_void_p), ("vc_sp", c_int64), ("vc_ss", c_int64), ("vc_sh", c_int64),
+                ("num_pages", c_int64), ("page_size", c_int)]
+
+
+class PagedAttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_st", c_int64), ("q_sh", c_int64),
+                ("out", c_void_p), ("o_st", c_int64), ("o_sh", c_int64),
+                ("k_cache", c_void_p), ("k_sp", c_int64), ("k_ss", c_int64), ("k_sh", c_int64),
+                ("v_cache", c_void_p), ("v_sp", c_int64), ("v_ss", c_int64), ("v_sh", c_int64),
+                ("block_table", c_void_p), ("t_sb", c_int64), ("cu_lens", c_void_p), ("seq_lens", c_void_p),
+                ("dtype", c_int), ("B", c_int), ("T", c_int), ("Hq", c_int), ("Hk", c_int), ("D", c_int),
+                ("P", c_int), ("page_size", c_int), ("num_pages", c_int64),
+                ("max_new", c_int), ("window", c_int), ("sinks", c_int), ("softmax_scale", c_float),
+                ("work", c_void_p)]
+
+
+class WindowAttnArgs(ctypes.Structure):
+    _fields_ = [("q", c_void_p), ("q_sb", c_int64), ("q_sh", c_int64), ("q_sl", c_int64),
+                ("k", c_void_p), ("k_sb", c_int64), ("k_sh", c_int64), ("k_sl", c_int64),
+                ("v", c_void_p), ("v_sb", c_int64), ("v_sh", c_int64), ("v_sl", c_int64),
+                ("out", c_void_p), ("o_sb", c_int64), ("o_sh", c_int64), ("o_sl", c_int64),
+                ("dtype", c_int), ("B", c_int), ("Hq", c_int), ("Hk", c_int), ("Lq", c_int), ("Lk", c_int),
+                ("D", c_int), ("window", c_int), ("sinks", c_int), ("softmax_scale", c_float), ("work", c_void_p)]
+
+
+STRUCTS = [PoolArgs, CorrArgs, StatsArgs, SelectArgs, AttnArgs, ScoresArgs, RopePoolArgs, XattnArgs, FlexArgs,
+           PlanArgs, RopeArgs, PagedAttnArgs, WindowAttnArgs]
 
 ENTRY_POINTS = ["fs_pool", "fs_rope_pool", "fs_corr_work_bytes", "fs_corr", "fs_stats", "fs_scores_work_bytes",
                 "fs_scores", "fs_scores_noalloc", "fs_select", "fs_bsattn_work_bytes",
                 "fs_bsattn", "fs_bsattn_prepare", "fs_bsattn_run", "fs_xattn_work_bytes", "fs_xattn",
-                "fs_flex_work_bytes", "fs_flex",
+                "fs_flex_work_bytes", "fs_flex", "fs_plan", "fs_rope", "fs_paged_attn_work_bytes", "fs_paged_attn",
+                "fs_window_attn_work_bytes", "fs_window_attn",
                 "fs_last_error", "fs_abi_version", "fs_sizeof_args"]
 
 _lib = None
@@ -152,11 +198,16 @@ def load() -> ctypes.CDLL:
     lib.fs_xattn_work_bytes.argtypes = [ctypes.POINTER(XattnArgs)]
     lib.fs_bsattn_work_bytes.restype = c_size_t
     lib.fs_bsattn_work_bytes.argtypes = [POINTER(AttnArgs)]
+    lib.fs_paged_attn_work_bytes.restype = c_size_t
+    lib.fs_paged_attn_work_bytes.argtypes = [POINTER(PagedAttnArgs)]
+    lib.fs_window_attn_work_bytes.restype = c_size_t
+    lib.fs_window_attn_work_bytes.argtypes = [POINTER(WindowAttnArgs)]
     for name, st in [("fs_pool", PoolArgs), ("fs_rope_pool", RopePoolArgs), ("fs_corr", CorrArgs),
                      ("fs_stats", StatsArgs), ("fs_scores", ScoresArgs), ("fs_scores_noalloc", ScoresArgs),
                      ("fs_select", SelectArgs), ("fs_bsattn", AttnArgs), ("fs_bsattn_prepare", AttnArgs),
                      ("fs_bsattn_run", AttnArgs), ("fs_xattn", XattnArgs),
-                     ("fs_flex", FlexArgs)]:
+                     ("fs_flex", FlexArgs), ("fs_plan", PlanArgs), ("fs_rope", RopeArgs),
+                     ("fs_paged_attn", PagedAttnArgs), ("fs_window_attn", WindowAttnArgs)]:
         fn = getattr(lib, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(st), c_void_p]

@@ -27,7 +27,7 @@ int launch_status(const char* what) {
 }  // namespace fs_host
 
 extern "C" const char* fs_last_error(void) { return fs_host::g_err; }
-extern "C" int fs_abi_version(void) { return 12; }
+extern "C" int fs_abi_version(void) { return 13; }
 
 extern "C" size_t fs_sizeof_args(int which) {
   switch (which) {
@@ -40,6 +40,10 @@ extern "C" size_t fs_sizeof_args(int which) {
     case 6: return sizeof(fs_rope_pool_args);
     case 7: return sizeof(fs_xattn_args);
     case 8: return sizeof(fs_flex_args);
+    case 9: return sizeof(fs_plan_args);
+    case 10: return sizeof(fs_rope_args);
+    case 11: return sizeof(fs_paged_attn_args);
+    case 12: return sizeof(fs_window_attn_args);
     default: return 0;
   }
 }

@@ -29,6 +29,7 @@
  *                                            Xattention_prefill (:306-406) hands to block_sparse_attn_func
  *   fs_flex      FlexPrefill's selector       attn_src/Flexprefill.py:946-1061 (get_active_blocks), the
  *                                            block index sets its Flexprefill_prefill (:1063-1098) attends
+ *   fs_plan, fs_rope, fs_paged_attn, fs_window_attn: no counterpart (serving over a paged cache after the prefill)
  *   fs_bsattn    block_sparse_attn_func call  my_attn_v7.py:775-786, fix_mask_attn/my_attn.py:196-207
  *                flash_attn_func(causal=True) my_attn_v7.py:509-519 (blk_cnt == NULL: dense causal)
  */
@@ -386,10 +387,133 @@ FS_API int fs_bsattn(const fs_attn_args* a, void* stream);
 FS_API int fs_bsattn_prepare(const fs_attn_args* a, void* stream);
 FS_API int fs_bsattn_run(const fs_attn_args* a, void* stream);
 
+/* ---- block tables and slot maps of one serving step ----------------------
+ * Request b holds seq_lens[b] tokens, token t in slot t % ps of page
+ * block_table[b * t_sb + t / ps] (ps = page_size), and is given new_lens[b]
+ * more (negative: its last -new_lens[b] are dropped; never below 0 tokens).
+ * With p0 and p1 the pages it holds before and after (ceil(tokens / ps), at
+ * most P): the pages p1 .. p0 - 1 of every request that shrinks are pushed on
+ * the stack free_pages[0 .. free_count[0]) in order of request and position,
+ * then the pages p0 .. p1 - 1 of every request that grows are popped from its
+ * top in that order and written to its row.  Outputs:
+ *   cu_lens [B + 1]     exclusive prefix sum of max(new_lens, 0): request b's
+ *                       new tokens are rows cu_lens[b] .. cu_lens[b + 1] - 1;
+ *   seq_lens_out [B]    tokens held after the step;
+ *   positions [T]       position of each new token, -1 for rows past cu_lens[B];
+ *   slots [T]           page * ps + position % ps, -1 where there is none;
+ *   free_count_out [1]  free pages after the step;
+ *   lacking [1]         new tokens left without a page because the stack or the
+ *                       row ended (their table entries within the row are -1).
+ * seq_lens and free_count are not written and must not be outputs; what is
+ * written to block_table and free_pages does not change what the call reads, so
+ * the same call repeated gives the same result, and a step with lacking != 0 is
+ * undone by not using its outputs.  free_pages has room for every page (F).
+ * Lengths outside 0 .. P ps and counts outside 0 .. F are taken at the border.
+ * B <= 4096, P * page_size < 2^31. */
+typedef struct {
+  int32_t* block_table; int64_t t_sb;    /* [B][P], row stride in elements */
+  const int32_t* seq_lens;               /* [B] */
+  const int32_t* new_lens;               /* [B] */
+  int32_t* free_pages;                   /* [F] */
+  const int32_t* free_count;             /* [1] */
+  int B, P, F, page_size, T;
+  int32_t* cu_lens;
+  int32_t* seq_lens_out;
+  int32_t* positions;
+  int64_t* slots;
+  int32_t* free_count_out;
+  int32_t* lacking;
+} fs_plan_args;
+FS_API int fs_plan(const fs_plan_args* a, void* stream);
+
+/* ---- rotary positions, and keys and values into a paged cache ------------
+ * q [T][Hq][D], k [T][Hk][D] (element strides; d contiguous).  The first 2 half
+ * dims of a head are rotated in pairs (i, i + half), or (2 i, 2 i + 1) if
+ * interleaved: (x1, x2) -> (x1 c - x2 s, x2 c + x1 s) with c, s =
+ * attention_factor * cos, sin of positions[t] * inv_freq[i], the angle in 64
+ * bits, the rotation in 32, rounded once to dtype; the other dims are copied.
+ * slots == NULL: writes q_out and k_out (either may be its input itself).
+ * slots != NULL: writes q_out, and the rotated k and the v rows into slot
+ * slots[t] % page_size of page slots[t] / page_size of k_cache / v_cache (page,
+ * slot and head strides kc_sp, kc_ss, kc_sh, ...).  The slots of one call are
+ * distinct.  A row with a negative position is left as it was (in the cache
+ * too); a slot outside 0 .. num_pages * page_size - 1 is not written.
+ * positions: int32 or int64 (pos_bytes 4 or 8).  dtype f32, bf16 or f16; D a
+ * multiple of 8 up to 512, half <= 128; 16-byte pieces where D and the rotated
+ * part allow them (single elements otherwise). */
+typedef struct {
+  const void* q; int64_t q_st, q_sh;
+  const void* k; int64_t k_st, k_sh;
+  const void* v; int64_t v_st, v_sh;     /* with slots, else NULL */
+  const void* positions;
+  const double* inv_freq;                /* [half] */
+  float attention_factor;
+  int pos_bytes, half, interleaved;
+  int dtype, T, Hq, Hk, D;
+  void* q_out; int64_t qo_st, qo_sh;
+  void* k_out; int64_t ko_st, ko_sh;     /* without slots */
+  const int64_t* slots;                  /* [T] or NULL */
+  void* k_cache; int64_t kc_sp, kc_ss, kc_sh;
+  void* v_cache; int64_t vc_sp, vc_ss, vc_sh;
+  int64_t num_pages;
+  int page_size;
+} fs_rope_args;
+FS_API int fs_rope(const fs_rope_args* a, void* stream);
+
+/* ---- attention of new tokens over a paged cache ---------------------------
+ * Request b's keys and values are tokens 0 .. seq_lens[b] - 1 of the cache
+ * (token s: slot s % page_size of page block_table[b * t_sb + s / page_size];
+ * page, slot and head strides), the last n = cu_lens[b + 1] - cu_lens[b] of them
+ * its new tokens, whose queries are rows cu_lens[b] .. of q [T][Hq][D].  The row
+ * at position p:
+ *   out = softmax(q . k_s * scale) v over the tokens s <= p with s > p - window
+ *         or s < sinks (window == 0: every s <= p),
+ * for query head h on KV head h / (Hq / Hk).  A row that sees no token is 0;
+ * rows past cu_lens[B] are left as they were.  A page outside 0 .. num_pages - 1
+ * holds no token.  The lengths stay on the device: nothing but B, T and P bounds
+ * the work, and max_new (the most new tokens that a request may have, 0: T) only
+ * chooses between forms of the kernel.  bf16 / f16, D 64 or 128, page_size a
+ * multiple of 16 up to 4096, P * page_size <= 2^26.
+ * work: fs_paged_attn_work_bytes(a) bytes of device scratch (it does not depend
+ * on B, T or P).  Calls that overlap on one workspace race. */
+typedef struct {
+  const void* q; int64_t q_st, q_sh;
+  void* out; int64_t o_st, o_sh;
+  const void* k_cache; int64_t k_sp, k_ss, k_sh;
+  const void* v_cache; int64_t v_sp, v_ss, v_sh;
+  const int32_t* block_table; int64_t t_sb;   /* [B][P] */
+  const int32_t* cu_lens;                     /* [B + 1] */
+  const int32_t* seq_lens;                    /* [B] */
+  int dtype, B, T, Hq, Hk, D, P, page_size;
+  int64_t num_pages;
+  int max_new, window, sinks;
+  float softmax_scale;
+  void* work;
+} fs_paged_attn_args;
+FS_API size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a);
+FS_API int fs_paged_attn(const fs_paged_attn_args* a, void* stream);
+
+/* ---- sliding-window attention with sinks ----------------------------------
+ * fs_paged_attn's rule on contiguous tensors: q [B][Hq][Lq][D], k and v
+ * [B][Hk][Lk][D] views, query t at position t + Lk - Lq.  Rows that see no
+ * token (Lq > Lk) are 0. */
+typedef struct {
+  const void* q; int64_t q_sb, q_sh, q_sl;
+  const void* k; int64_t k_sb, k_sh, k_sl;
+  const void* v; int64_t v_sb, v_sh, v_sl;
+  void* out; int64_t o_sb, o_sh, o_sl;
+  int dtype, B, Hq, Hk, Lq, Lk, D;
+  int window, sinks;
+  float softmax_scale;
+  void* work;
+} fs_window_attn_args;
+FS_API size_t fs_window_attn_work_bytes(const fs_window_attn_args* a);
+FS_API int fs_window_attn(const fs_window_attn_args* a, void* stream);
+
 /* Description of the last failure on this thread ("" if none). */
 FS_API const char* fs_last_error(void);
 /* sizeof the argument struct: 0 pool, 1 corr, 2 stats, 3 select, 4 attn, 5 scores, 6 rope_pool, 7 xattn,
- * 8 flex
+ * 8 flex, 9 plan, 10 rope, 11 paged_attn, 12 window_attn
  * (lets a foreign-function binding check its struct layout). */
 FS_API size_t fs_sizeof_args(int which);
 /* ABI version of this library (increments on any struct change). */
