@@ -1,11 +1,45 @@
 // Attention of new tokens over a paged cache, and sliding-window attention with
-// sinks on contiguous tensors: one wave per (token, query head), keys 64 at a
-// time with a running maximum and sum.
+// sinks on contiguous tensors, on bf16 / f16 MFMA (gfx950).
+//
+// Rows.  The query heads that read one KV head are put side by side: row r of
+// (request, KV head) is new token r / G, query head hk G + r % G (G = Hq / Hk).
+// So a single token fills a tile with the G heads that read the same keys, and a
+// chunk's tile of 128 rows reads each key once for all of them.  A row tile sees
+// the keys kbeg .. kend - 1 (the union of its rows' windows) and the first
+// `sinks`; tiles of keys in between are not visited.
+//
+// Pieces.  A row tile's keys are taken in pieces of at most `chunk` key tiles by
+// workgroups of their own where that fills the GPU better (plan_pieces_kernel, from the
+// lengths on the device); the pieces' unnormalised sums are then joined by
+// combine_kernel, in the pieces' order.
+//
+// few_kernel (row tiles of at most 32 rows: single tokens) is bound by the cache
+// being read.  Each of its 4 waves streams keys of its own, 32 at a time, through
+// a ring of two LDS tiles that only it uses: no barrier, so 24 to 32 KiB per wave
+// are always on their way (96 KiB and more per CU).  S^T = K Q^T, P in registers, O^T += V^T P
+// on v_mfma_f32_32x32x16; V is read transposed from LDS as it is stored.
+//
+// many_kernel (128 rows) is bound by MFMA: 4 waves of 32 rows share tiles of 64 keys, two
+// tiles deep, as in bsattn_kernel: S of the next tile and P V of the last one are
+// interleaved with the exponentials of the current one.
+//
+// Groups of 16 keys are never split by a page (its size is a multiple of 16): a
+// copy of one is addressed by one entry of the table.  A group that not all rows
+// of the tile may read as a whole (the end of the request, the window's edge, a
+// page that is none) is copied row by row, zeros in place of the rows that no row
+// of the tile sees: nothing stands there that could spoil a sum.
+#include <algorithm>
 #include <climits>
+#include <type_traits>
 
-#include "common.h"
+#include "attn_tile.h"
 
 namespace fs {
+
+constexpr int kSlotsFew = 256, kSlotsMany = 512;    // workgroups that 256 CUs hold (D = 128)
+constexpr int kPartsFew = 2048, kPartsMany = 1024;  // split pieces that the workspace holds
+constexpr int kMaxRequests = 4096;
+constexpr int kPlanThreads = 1024;
 
 struct PagedKArgs {
   const uint16_t* q;
@@ -13,99 +47,879 @@ struct PagedKArgs {
   const uint16_t* v;
   uint16_t* out;
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh;   // request (contiguous tensors), token, head
-  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;   // page (contiguous: batch), slot, head
+  int64_t k_sp, k_sh, v_sp, v_sh;               // page (contiguous: batch), head
+  int k_ss, v_ss;                               // slot
   const int32_t* table;                         // null: contiguous, the page of request b is b
   const int32_t* cu;
   const int32_t* lens;
   int64_t t_sb, num_pages;
-  int B, T, Hq, Hk, Lq, Lk, P, page_size, window, sinks;
+  int B, T, Hq, Hk, G, Lq, Lk, P, page_size, window, sinks;
+  uint32_t page_magic;                          // x / (page_size / 16) = mulhi(x, magic); 0: x
   float scale;
+  // pieces: null = one piece per row tile, the last row tiles of a request first
+  const int4* pieces;                           // [N] request, row tile, first key tile, slot (-1: the only piece)
+  const int4* pairs;                            // [R] request, row tile, pieces, first slot
+  const int32_t* head;                          // N, R, chunk, split pieces (of one KV head)
+  int row_tiles;                                // of a request (no list)
+  float* part_o;                                // [slot][rows / 32][D / 32][4][64 lanes] 4 floats
+  float* part_ml;                               // [slot][rows / 32][2][32]
 };
 
-template <typename T, int D>
-__global__ __launch_bounds__(64) void row_attn_kernel(PagedKArgs a) {
-  __shared__ float qs[D];
-  const int lane = threadIdx.x;
-  const int h = blockIdx.x % a.Hq, t = blockIdx.x / a.Hq;
-  const int hk = h / (a.Hq / a.Hk);
-  int b, i, n, L;
-  if (a.table != nullptr) {
-    if (t >= a.cu[a.B]) return;
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-      const int m = (lo + hi) >> 1;
-      if (a.cu[m] <= t) lo = m;
-      else hi = m;
-    }
-    b = lo;
-    i = t - a.cu[b];
-    n = a.cu[b + 1] - a.cu[b];
-    L = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.P * a.page_size);
-  } else {
-    b = t / a.Lq;
-    i = t - b * a.Lq;
-    n = a.Lq;
-    L = a.Lk;
-  }
-  const int64_t row = a.table != nullptr ? t : i;
-  const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_sb + row * a.q_st + h * a.q_sh;
-  for (int d = lane; d < D; d += 64) qs[d] = to_f32(q[d]);
-  __syncthreads();
-  const int p = L - n + i;
-  float m = -INFINITY, l = 0.f, o[D / 64] = {};
-  for (int k0 = 0; k0 <= p; k0 += 64) {
-    const int s = k0 + lane;
-    bool seen = s <= p && s < L && (a.window == 0 || s > p - a.window || s < a.sinks);
-    const int pg = s / a.page_size;
-    int64_t page = b;
-    if (a.table != nullptr) {
-      page = seen ? a.table[b * a.t_sb + pg] : 0;
-      if (page < 0 || page >= a.num_pages) seen = false;
-    }
-    if (__ballot(seen) == 0) continue;
-    const int slot = a.table != nullptr ? s - pg * a.page_size : s;
-    float x = -INFINITY;
-    if (seen) {
-      const T* kr = reinterpret_cast<const T*>(a.k) + page * a.k_sp + slot * a.k_ss + hk * a.k_sh;
-      float acc = 0.f;
-      for (int c = 0; c < D; c += 8) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(kr + c);
-        T e[8];
-        __builtin_memcpy(e, &raw, 16);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc += qs[c + j] * to_f32(e[j]);
-      }
-      x = acc * a.scale;
-    }
-    const float mn = fmaxf(m, wave_max(x));
-    const float mu = mn == -INFINITY ? 0.f : mn;
-    const float w = seen ? expf(x - mu) : 0.f;
-    const float al = expf(m - mu);
-    m = mn;
-    l = l * al + wave_sum(w);
-#pragma unroll
-    for (int e = 0; e < D / 64; ++e) o[e] *= al;
-    const int64_t vo = page * a.v_sp + slot * a.v_ss + hk * a.v_sh;
-    const uint64_t any = __ballot(seen);
-    for (int j = 0; j < 64; ++j) {
-      if (!((any >> j) & 1)) continue;
-      const float wj = __shfl(w, j, 64);
-      const T* vr = reinterpret_cast<const T*>(a.v) + __shfl(vo, j, 64);
-#pragma unroll
-      for (int e = 0; e < D / 64; ++e) o[e] += wj * to_f32(vr[lane + 64 * e]);
-    }
-  }
-  T* out = reinterpret_cast<T*>(a.out) + b * a.o_sb + row * a.o_st + h * a.o_sh;
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-  for (int e = 0; e < D / 64; ++e) out[lane + 64 * e] = Conv<T>::store(o[e] * inv);
+// A wave-uniform load through the scalar unit: what no kernel of the launch writes.
+template <typename E>
+__device__ __forceinline__ E scalar_load(const E* p, int64_t i) {
+  return ((const __attribute__((address_space(4))) E*)(uintptr_t)p)[i];
 }
 
-static int run(const PagedKArgs& k, int dtype, int D, int64_t rows, hipStream_t s, const char* fn) {
-  auto f = D == 64 ? (dtype == FS_DTYPE_BF16 ? row_attn_kernel<bf16_t, 64> : row_attn_kernel<f16_t, 64>)
-                   : (dtype == FS_DTYPE_BF16 ? row_attn_kernel<bf16_t, 128> : row_attn_kernel<f16_t, 128>);
-  f<<<(unsigned)(rows * k.Hq), 64, 0, s>>>(k);
-  return fs_host::launch_status(fn);
+// A row tile's place and the keys it sees; everything wave-uniform.
+struct RowTile {
+  int row0, n, L;            // first row of q, new tokens, tokens
+  int r0, nrows;             // rows r0 .. r0 + nrows - 1 of the request
+  int p_lo, p_hi;            // positions of its first and last row
+  int kbeg, kend;            // keys kbeg .. kend - 1 (and the first `sinks`) are seen by some row
+  int ns, t0, nt;            // key tiles: 0 .. ns - 1, then t0 ..; nt in all
+};
+template <int M, int TK>
+__device__ __forceinline__ RowTile row_tile(const PagedKArgs& a, int b, int rt) {
+  RowTile u;
+  if (a.table != nullptr) {
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    u.row0 = c0;
+    u.n = min(max(c1 - c0, 0), a.T);
+    u.L = min(max(a.lens[b], 0), a.P * a.page_size);
+  } else {
+    u.row0 = 0;
+    u.n = a.Lq;
+    u.L = a.Lk;
+  }
+  u.r0 = rt * M;
+  u.nrows = min(M, u.n * a.G - u.r0);
+  u.p_lo = u.L - u.n + u.r0 / a.G;
+  u.p_hi = u.L - u.n + (u.r0 + max(u.nrows, 1) - 1) / a.G;
+  u.kend = u.nrows > 0 ? max(u.p_hi + 1, 0) : 0;
+  u.kbeg = a.window ? max(u.p_lo - a.window + 1, 0) : 0;
+  u.ns = (min(a.sinks, u.kbeg) + TK - 1) / TK;
+  u.t0 = u.kbeg / TK;
+  if (u.ns >= u.t0) u.ns = u.t0 = 0;
+  u.nt = u.kend > 0 ? u.ns + (u.kend + TK - 1) / TK - u.t0 : 0;
+  return u;
+}
+
+// Copies of 16-key groups into an LDS tile of rows of D elements: group g of it at byte
+// 16 g * 2 D, swizzled as the operand reads expect.
+template <int D, bool PAGED>
+struct GroupCopy {
+  static constexpr int ROWB = D * 2, CPR = D / 8, SWM = CPR - 1, LCPR = D == 128 ? 4 : 3;
+  static constexpr int RPR = 1024 / ROWB;          // rows of a 1 KiB copy
+  static constexpr int NI = 16 / RPR;              // copies of a group
+  uint32_t koff[NI], voff[NI];
+  const uint16_t *kp, *vp;
+  __device__ __forceinline__ GroupCopy(const PagedKArgs& a, int hk, int lane) {
+    kp = a.k + hk * a.k_sh;
+    vp = a.v + hk * a.v_sh;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = RPR * i + (lane >> LCPR);
+      koff[i] = (uint32_t)(r * a.k_ss + kchunk(r, lane) * 8) * 2u;
+      voff[i] = (uint32_t)(r * a.v_ss + vchunk(r, lane) * 8) * 2u;
+    }
+  }
+  static __device__ __forceinline__ int kchunk(int r, int lane) { return (lane & SWM) ^ ((D == 128 ? r : r >> 1) & SWM); }
+  static __device__ __forceinline__ int vchunk(int r, int lane) { return (lane & SWM) ^ v_swz<D>(r); }
+  // the table's entry for the group of key k0 (a multiple of 16), -1 where the tile sees no key of it
+  static __device__ __forceinline__ int entry(const PagedKArgs& a, const RowTile& u, int b, int k0) {
+    const int last = k0 + 15;
+    if (k0 >= u.kend || (last < u.kbeg && k0 >= a.sinks)) return -1;
+    if constexpr (!PAGED) return b;
+    const uint32_t x = (uint32_t)k0 >> 4;
+    const uint32_t pg = a.page_magic ? __umulhi(x, a.page_magic) : x;
+    const int e = scalar_load(a.table, (int64_t)b * a.t_sb + pg);
+    return e >= 0 && e < a.num_pages ? e : -1;
+  }
+  static __device__ __forceinline__ int slot_of(const PagedKArgs& a, int k0) {
+    if constexpr (!PAGED) return k0;
+    const uint32_t x = (uint32_t)k0 >> 4;
+    const uint32_t pg = a.page_magic ? __umulhi(x, a.page_magic) : x;
+    return k0 - (int)pg * a.page_size;
+  }
+  // every key of the group is seen by some row of the tile
+  static __device__ __forceinline__ bool whole(const PagedKArgs& a, const RowTile& u, int e, int k0) {
+    return e >= 0 && k0 + 16 <= u.kend && (k0 >= u.kbeg || k0 + 16 <= a.sinks);
+  }
+  template <bool V>
+  __device__ __forceinline__ void issue(const PagedKArgs& a, const RowTile& u, uint32_t lds, int e, int k0) const {
+    const int64_t st = V ? a.v_ss : a.k_ss;
+    const uint16_t* base = (V ? vp : kp) + max(e, 0) * (V ? a.v_sp : a.k_sp) + slot_of(a, k0) * st;
+    if (whole(a, u, e, k0)) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma16s(lds + i * 1024, base, V ? voff[i] : koff[i]);
+    } else {
+      int ln = (int)__lane_id();
+      asm volatile("" : "+v"(ln));                 // keep this rare path's addresses out of the loop's preheader
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = RPR * i + (ln >> LCPR), key = k0 + r;
+        const bool ok = e >= 0 && key < u.kend && (key >= u.kbeg || key < a.sinks);
+        const uint16_t* row = ok ? base + (int64_t)r * st : reinterpret_cast<const uint16_t*>(kZeroRow);
+        dma16(lds + i * 1024, row + (V ? vchunk(r, ln) : kchunk(r, ln)) * 8);
+      }
+    }
+  }
+};
+
+// v and the value of the lane 32 apart (the same row's other keys)
+__device__ __forceinline__ void lane_halves(float v, float& lo, float& hi) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  lo = __uint_as_float(r[0]);
+  hi = __uint_as_float(r[1]);
+}
+
+// This lane's row of a 32-row part of a row tile.
+struct LaneRow {
+  int tok, g, p;             // token of the request, head of the group, position
+  bool on;
+};
+template <typename A>
+__device__ __forceinline__ LaneRow lane_row(const A& a, const RowTile& u, int r) {
+  LaneRow w;
+  const int rr = u.r0 + min(r, max(u.nrows, 1) - 1);  // rows past the tile's follow its last one
+  w.tok = rr / a.G;
+  w.g = rr - w.tok * a.G;
+  w.p = u.L - u.n + w.tok;
+  const int t = u.row0 + w.tok;
+  w.on = r < u.nrows && t >= 0 && t < a.T;
+  return w;
+}
+
+// Q^T fragments of a row (B operand of S^T = K Q^T): dims st*16 + hi*8 .. +7; zeros without a row
+template <typename V8, int D>
+__device__ __forceinline__ void load_q(const PagedKArgs& a, const RowTile& u, const LaneRow& w, int b, int hk, int hi,
+                                       V8* qf) {
+  const uint16_t* qp = a.q + b * a.q_sb + (int64_t)(u.row0 + w.tok) * a.q_st + (int64_t)(hk * a.G + w.g) * a.q_sh;
+#pragma unroll
+  for (int st = 0; st < D / 16; ++st) {
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (w.on) raw = *reinterpret_cast<const uint4*>(qp + st * 16 + hi * 8);
+    qf[st] = __builtin_bit_cast(V8, raw);
+  }
+}
+
+// -inf for the scores of 32 keys from key0 (register r: key (r >> 2) * 8 + (r & 3) + hi * 4) that the row at p
+// does not see; v0, v1: whether the two groups of 16 are there
+__device__ __forceinline__ void mask_keys(const PagedKArgs& a, const RowTile& u, f32x16_t& s, int p, int key0, int hi,
+                                          bool v0, bool v1) {
+  const int k = key0 + hi * 4;
+  const int last = p - k;                          // c <= last
+  const int first = a.window ? p - a.window - k : INT_MIN;   // c > first, or c < sink
+  const int sink = a.window ? a.sinks - k : INT_MIN;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int c = (r >> 2) * 8 + (r & 3);
+    const bool ok = c <= last && (c > first || c < sink) && (r < 8 ? v0 : v1);
+    if (!ok) s[r] = -INFINITY;
+  }
+}
+// whether some row of positions p_lo .. p_hi does not see some key of key0 .. key0 + n - 1
+__device__ __forceinline__ bool needs_mask(const PagedKArgs& a, int p_lo, int p_hi, int key0, int n) {
+  return key0 + n - 1 > p_lo || (a.window && key0 <= p_hi - a.window && key0 + n > a.sinks);
+}
+
+// O^T of one row (this lane's dims dt * 32 + g4 * 8 + hi * 4 .. + 3) to the output
+template <typename T>
+__device__ __forceinline__ void store_out(uint16_t* op, int d0, float x0, float x1, float x2, float x3) {
+  using Ops = MfmaOps<T>;
+  uint2 w;
+  w.x = (uint32_t)Ops::bits(x0) | ((uint32_t)Ops::bits(x1) << 16);
+  w.y = (uint32_t)Ops::bits(x2) | ((uint32_t)Ops::bits(x3) << 16);
+  *reinterpret_cast<uint2*>(op + d0) = w;
+}
+__device__ __forceinline__ uint16_t* out_row(const PagedKArgs& a, const RowTile& u, const LaneRow& w, int b, int hk) {
+  return a.out + b * a.o_sb + (int64_t)(u.row0 + w.tok) * a.o_st + (int64_t)(hk * a.G + w.g) * a.o_sh;
+}
+
+// The piece of workgroup p: KV head, request, row tile, first key tile, key tiles, slot (-1: no other piece).
+struct Piece {
+  int hk, b, rt, begin, count, slot;
+};
+__device__ __forceinline__ bool find_piece(const PagedKArgs& a, int p, Piece& w) {
+  if (a.pieces != nullptr) {
+    const int N = scalar_load(a.head, 0);
+    if (p >= N * a.Hk) return false;
+    w.hk = p / N;
+    const int32_t* e = reinterpret_cast<const int32_t*>(a.pieces + (p - w.hk * N));
+    w.b = scalar_load(e, 0);
+    w.rt = scalar_load(e, 1);
+    w.begin = scalar_load(e, 2);
+    w.slot = scalar_load(e, 3);
+    w.count = scalar_load(a.head, 2);
+    if (w.slot >= 0) w.slot += w.hk * scalar_load(a.head, 3);
+  } else {
+    const int R = a.B * a.row_tiles;
+    if (p >= R * a.Hk) return false;
+    w.hk = p / R;
+    const int i = p - w.hk * R;
+    w.b = i / a.row_tiles;
+    w.rt = a.row_tiles - 1 - (i - w.b * a.row_tiles);
+    w.begin = 0;
+    w.slot = -1;
+    w.count = INT_MAX;
+  }
+  return true;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kSlack = 8.0f;                     // a row's running max is raised past 2^8 only: few rescales of O
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
+  using Ops = MfmaOps<T>;
+  using V8 = typename Ops::V8;
+  using Copy = GroupCopy<D, PAGED>;
+  constexpr int TILE = 32 * D * 2;                 // bytes of 32 keys
+  constexpr int RING = 4 * TILE;                   // of a wave: two K tiles, two V tiles
+  constexpr int NI = 2 * Copy::NI;                 // copies of 32 keys
+  __shared__ __attribute__((aligned(1024))) char lds[4 * RING];
+  Piece pc;
+  if (!find_piece(a, blockIdx.x, pc)) return;
+  const RowTile u = row_tile<32, 128>(a, pc.b, pc.rt);
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneRow me = lane_row(a, u, l32);
+  char* ring = lds + wave * RING;
+  const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
+  const Copy cp(a, pc.hk, lane);
+  V8 qf[D / 16];
+  load_q<V8, D>(a, u, me, pc.b, pc.hk, hi, qf);
+
+  // this wave's 32 keys of each of the piece's tiles of 128
+  auto key_of = [&](int i) {
+    const int o = pc.begin + i;
+    return (o < u.ns ? o : u.t0 + o - u.ns) * 128 + 32 * wave;
+  };
+  int cnt = min(pc.count, u.nt - pc.begin);
+  if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
+  struct Ent {
+    int e[2];
+  };
+  auto load_ent = [&](int i) {
+    Ent x{{-1, -1}};
+    if (i < cnt) {
+      const int k = key_of(i);
+      x.e[0] = Copy::entry(a, u, pc.b, k);
+      x.e[1] = Copy::entry(a, u, pc.b, k + 16);
+    }
+    return x;
+  };
+  auto issue_k = [&](int i, const Ent& x) {
+    const uint32_t at = ring0 + (i & 1) * TILE;
+    cp.template issue<false>(a, u, at, x.e[0], key_of(i));
+    cp.template issue<false>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+  };
+  auto issue_v = [&](int i, const Ent& x) {
+    const uint32_t at = ring0 + (2 + (i & 1)) * TILE;
+    cp.template issue<true>(a, u, at, x.e[0], key_of(i));
+    cp.template issue<true>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+  };
+  constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
+  const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
+  const int vrow = hi * 4 + ((lane & 15) >> 2);
+  const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
+                                     (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
+  const float sc = a.scale * kLog2e;
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+
+  // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this
+  // order; K(i+2) and V(i+2) are requested as soon as their place is read.
+  Ent x0 = load_ent(0), x1 = load_ent(1), x2 = load_ent(2);
+  if (cnt > 0) {
+    issue_k(0, x0);
+    issue_v(0, x0);
+  }
+  if (cnt > 1) {
+    issue_k(1, x1);
+    issue_v(1, x1);
+  }
+  __builtin_amdgcn_s_waitcnt(0);                   // Q's loads too: the loop's waits then count copies only
+  for (int i = 0; i < cnt; ++i) {
+    if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+    const char* kt = ring + (i & 1) * TILE;
+    f32x16_t s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) s = Ops::mma(__builtin_bit_cast(V8, lds16(kt, k_lane ^ (uint32_t)(st << 5))), qf[st], s);
+    const Ent x3 = load_ent(i + 3);
+    if (i + 2 < cnt) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      issue_k(i + 2, x2);
+    }
+    const int key0 = key_of(i);
+    if (x0.e[0] < 0 || x0.e[1] < 0 || needs_mask(a, u.p_lo, u.p_hi, key0, 32))
+      mask_keys(a, u, s, me.p, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+    float mx = s[0], h0, h1;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    lane_halves(mx, h0, h1);
+    mx = fmaxf(h0, h1) * sc;
+    const bool up = mx > m_run + kSlack;
+    const float al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
+    m_run = up ? mx : m_run;
+    const float mu = m_run == -INFINITY ? 0.f : m_run;
+    V8 pb[2];
+    float rs = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      float pv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pv[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * kk + j], sc, -mu));
+      pb[kk] = Ops::pack(pv);
+      rs = Ops::sum8(pb[kk], rs);
+    }
+    lane_halves(rs, h0, h1);
+    l_run = l_run * al + (h0 + h1);
+    if (__builtin_amdgcn_ballot_w64(al != 1.0f) != 0) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[dt][r] *= al;
+    }
+    if (i + 2 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
+    else if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const char* vt = ring + (2 + (i & 1)) * TILE;
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const uint32_t lo = (v_lane ^ (uint32_t)(dt << 6)) + kk * 16 * ROWB;
+        o[dt] = Ops::mma(__builtin_bit_cast(V8, join8(lds_tr8(vt, lo), lds_tr8(vt, lo + 8 * ROWB))), pb[kk], o[dt]);
+      }
+    if (i + 2 < cnt) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      issue_v(i + 2, x2);
+    }
+    x0 = x1;
+    x1 = x2;
+    x2 = x3;
+  }
+  // ---- the four waves' sums joined through LDS, wave w taking dims 32 w ..
+  constexpr int NV = D / 32;
+  float* own = reinterpret_cast<float*>(ring);     // [D / 32][4][64 lanes] 4 floats, then m and l
+#pragma unroll
+  for (int dt = 0; dt < NV; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      reinterpret_cast<float4*>(own)[(dt * 4 + g4) * 64 + lane] =
+          make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+  constexpr int ML = NV * 4 * 64 * 4;
+  own[ML + lane] = m_run;
+  own[ML + 64 + lane] = l_run;
+  __syncthreads();
+  if (wave >= NV || !me.on) return;
+  float m = -INFINITY, l = 0.f, f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
+  const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float* x = reinterpret_cast<const float*>(lds + w * RING) + ML;
+    f[w] = __builtin_amdgcn_exp2f(x[lane] - mu);
+    l += x[64 + lane] * f[w];
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  uint16_t* op = out_row(a, u, me, pc.b, pc.hk);
+#pragma unroll
+  for (int g4 = 0; g4 < 4; ++g4) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(wave * 4 + g4) * 64 + lane];
+      acc.x += x.x * f[w];
+      acc.y += x.y * f[w];
+      acc.z += x.z * f[w];
+      acc.w += x.w * f[w];
+    }
+    if (pc.slot < 0) store_out<T>(op, wave * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    else reinterpret_cast<float4*>(a.part_o)[(((int64_t)pc.slot * NV + wave) * 4 + g4) * 64 + lane] = acc;
+  }
+  if (pc.slot >= 0 && wave == 0 && hi == 0) {
+    a.part_ml[(int64_t)pc.slot * 64 + l32] = m;
+    a.part_ml[(int64_t)pc.slot * 64 + 32 + l32] = l;
+  }
+}
+
+// One 32-row part of one row tile per workgroup, wave w taking dims 32 w ..: the pieces' sums joined in their order.
+template <typename T, int D, int M>
+__global__ __launch_bounds__(2 * D) void combine_kernel(PagedKArgs a) {
+  constexpr int NV = D / 32, QW = M / 32;
+  const int R = scalar_load(a.head, 1);
+  const int part = blockIdx.x % QW, pu = blockIdx.x / QW;
+  if (pu >= R * a.Hk) return;
+  const int hk = pu / R;
+  const int4 pr = a.pairs[pu - hk * R];
+  const int np = __builtin_amdgcn_readfirstlane(pr.z);
+  if (np <= 1) return;
+  const int b = __builtin_amdgcn_readfirstlane(pr.x);
+  const RowTile u = row_tile<M, 64>(a, b, __builtin_amdgcn_readfirstlane(pr.y));
+  const int64_t s0 = (int64_t)(__builtin_amdgcn_readfirstlane(pr.w) + hk * a.head[3]) * QW + part;
+  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
+  const LaneRow me = lane_row(a, u, part * 32 + l32);
+  if (!me.on) return;
+  float m = -INFINITY;
+  for (int j = 0; j < np; ++j) m = fmaxf(m, a.part_ml[(s0 + (int64_t)j * QW) * 64 + l32]);
+  const float mu = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc[4] = {};
+  for (int j = 0; j < np; ++j) {
+    const int64_t s = s0 + (int64_t)j * QW;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[s * 64 + l32] - mu);
+    l += a.part_ml[s * 64 + 32 + l32] * f;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const float4 x = reinterpret_cast<const float4*>(a.part_o)[((s * NV + wave) * 4 + g4) * 64 + lane];
+      acc[g4].x += x.x * f;
+      acc[g4].y += x.y * f;
+      acc[g4].z += x.z * f;
+      acc[g4].w += x.w * f;
+    }
+  }
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  uint16_t* op = out_row(a, u, me, b, hk);
+#pragma unroll
+  for (int g4 = 0; g4 < 4; ++g4)
+    store_out<T>(op, wave * 32 + g4 * 8 + hi * 4, acc[g4].x * inv, acc[g4].y * inv, acc[g4].z * inv, acc[g4].w * inv);
+}
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void many_kernel(PagedKArgs a) {
+  using Ops = MfmaOps<T>;
+  using V8 = typename Ops::V8;
+  using Copy = GroupCopy<D, PAGED>;
+  constexpr int TK = 64, TILE = TK * D * 2;        // bytes of a K or V tile
+  constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM, GB = 16 * ROWB;
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][TILE];   // [K, V][buffer]
+  Piece pc;
+  {
+    // XCD x (workgroups x, x + 8, ..) takes a run of consecutive pieces: row tiles of one head, whose keys its L2 then serves
+    const int total = (a.pieces != nullptr ? scalar_load(a.head, 0) : a.B * a.row_tiles) * a.Hk, per = (total + 7) / 8;
+    const int p = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || !find_piece(a, p, pc)) return;
+  }
+  const RowTile u = row_tile<128, TK>(a, pc.b, pc.rt);
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const LaneRow me = lane_row(a, u, wave * 32 + l32);
+  // positions of this wave's first and last row
+  const int w_lo = u.L - u.n + (u.r0 + min(wave * 32, max(u.nrows, 1) - 1)) / a.G;
+  const int w_hi = u.L - u.n + (u.r0 + min(wave * 32 + 31, max(u.nrows, 1) - 1)) / a.G;
+  const Copy cp(a, pc.hk, lane);
+  const int cnt = min(pc.count, u.nt - pc.begin);
+  auto key_of = [&](int i) {
+    const int o = pc.begin + i;
+    return (o < u.ns ? o : u.t0 + o - u.ns) * TK;
+  };
+  // the table's entries of a tile's four groups; wave w copies group w
+  struct Ent {
+    int e[4];
+  };
+  auto load_ent = [&](int i) {
+    Ent x{{-1, -1, -1, -1}};
+    if (i < cnt) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x.e[g] = Copy::entry(a, u, pc.b, key_of(i) + 16 * g);
+    }
+    return x;
+  };
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&lds[0][0][0]) + wave * GB;
+  auto own = [&](const Ent& x) { return wave == 0 ? x.e[0] : wave == 1 ? x.e[1] : wave == 2 ? x.e[2] : x.e[3]; };
+  auto issue_k = [&](int i, const Ent& x) { cp.template issue<false>(a, u, lds0 + (i & 1) * TILE, own(x), key_of(i) + 16 * wave); };
+  auto issue_v = [&](int i, const Ent& x) { cp.template issue<true>(a, u, lds0 + (2 + (i & 1)) * TILE, own(x), key_of(i) + 16 * wave); };
+
+  V8 qf[D / 16];
+  load_q<V8, D>(a, u, me, pc.b, pc.hk, hi, qf);
+  const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
+  const int vrow = hi * 4 + ((lane & 15) >> 2);
+  const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
+                                     (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
+  const float sc = a.scale * kLog2e;
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16_t o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+
+  auto compute_s = [&](int buf, f32x16_t* s) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[kt][r] = 0.f;
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) {
+      const uint32_t lo = k_lane ^ (uint32_t)(st << 5);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+        s[kt] = Ops::mma(__builtin_bit_cast(V8, lds16(lds[0][buf] + kt * 32 * ROWB, lo)), qf[st], s[kt]);
+    }
+  };
+  auto mask = [&](int i, f32x16_t* s, const Ent& x) {
+    const int key0 = key_of(i);
+    const bool gone = x.e[0] < 0 || x.e[1] < 0 || x.e[2] < 0 || x.e[3] < 0;
+    if (gone || needs_mask(a, w_lo, w_hi, key0, TK)) {
+      mask_keys(a, u, s[0], me.p, key0, hi, x.e[0] >= 0, x.e[1] >= 0);
+      mask_keys(a, u, s[1], me.p, key0 + 32, hi, x.e[2] >= 0, x.e[3] >= 0);
+    }
+  };
+  auto exps = [&](const f32x16_t* s, V8* pb, float m_use) {
+    float rs = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      float pv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pv[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kk >> 1][8 * (kk & 1) + j], sc, -m_use));
+      pb[kk] = Ops::pack(pv);
+      rs = Ops::sum8(pb[kk], rs);
+    }
+    return rs;
+  };
+  auto pv_mma = [&](int buf, const V8* pb) {
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        const uint32_t lo = (v_lane ^ (uint32_t)(dt << 6)) + kk * 16 * ROWB;
+        o[dt] = Ops::mma(__builtin_bit_cast(V8, join8(lds_tr8(lds[1][buf], lo), lds_tr8(lds[1][buf], lo + 8 * ROWB))),
+                         pb[kk], o[dt]);
+      }
+  };
+  // Step t: wait for K(t+1) and V(t-1), one barrier, copy K(t+2) over K(t) and V(t) over V(t-2); then S(t+1) and
+  // P V(t-1) on MFMA between the exponentials of tile t; then O's rescale (rare) and the masks of tile t+1.
+  f32x16_t sa[2], sb[2];
+  V8 pa[4], pb[4];
+  Ent x0{}, x1{}, x2{}, x3{};                      // of tiles t .. t+3
+  typedef std::integral_constant<bool, true> yes;
+  typedef std::integral_constant<bool, false> no;
+  auto iter = [&](int t, f32x16_t* s_next, f32x16_t* s_cur, V8* p_prev, V8* p_cur, auto hasS, auto hasPV, auto hasE) {
+    __builtin_amdgcn_s_setprio(0);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (t + 2 < cnt) issue_k(t + 2, x2);
+    if (t < cnt) issue_v(t, x0);
+    x3 = load_ent(t + 3);
+    __builtin_amdgcn_s_setprio(2);
+    float rs = 0.f, al = 1.0f;
+    if constexpr (decltype(hasS)::value) compute_s((t + 1) & 1, s_next);
+    if constexpr (decltype(hasPV)::value) pv_mma((t - 1) & 1, p_prev);
+    if constexpr (decltype(hasE)::value) {
+      float mx = s_cur[0][0], m0, m1;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s_cur[kt][r]);
+      lane_halves(mx, m0, m1);
+      mx = fmaxf(m0, m1) * sc;
+      const bool up = mx > m_run + kSlack;
+      al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
+      m_run = up ? mx : m_run;
+      rs = exps(s_cur, p_cur, m_run == -INFINITY ? 0.f : m_run);
+    }
+    if constexpr (decltype(hasS)::value && decltype(hasPV)::value && decltype(hasE)::value) {
+      // one MFMA, then three VALU instructions, operand reads six MFMAs ahead (as measured for bsattn_kernel)
+      constexpr int NS = 2 * (D / 16), NM = NS + 4 * (D / 32), LA = 6, VPM = 3;
+      __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (i + LA < NS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        else if (i + LA < NM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
+      }
+    }
+    if constexpr (decltype(hasE)::value) {
+      float r0, r1;
+      lane_halves(rs, r0, r1);
+      l_run = l_run * al + (r0 + r1);
+      if (__builtin_amdgcn_ballot_w64(al != 1.0f) != 0) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= al;   // O holds P V up to t-1 now
+      }
+    }
+    if constexpr (decltype(hasS)::value) mask(t + 1, s_next, x1);
+    x0 = x1;
+    x1 = x2;
+    x2 = x3;
+  };
+  if (cnt > 0) {
+    x0 = load_ent(0);
+    x1 = load_ent(1);
+    x2 = load_ent(2);
+    issue_k(0, x0);
+    if (cnt > 1) issue_k(1, x1);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  if (cnt > 0) {
+    __builtin_amdgcn_s_barrier();
+    compute_s(0, sa);
+    mask(0, sa, x0);
+    if (cnt > 1) iter(0, sb, sa, pb, pa, yes(), no(), yes());
+    else iter(0, sb, sa, pb, pa, no(), no(), yes());
+    int t = 1;
+    for (; t + 2 < cnt; t += 2) {
+      iter(t, sa, sb, pa, pb, yes(), yes(), yes());
+      iter(t + 1, sb, sa, pb, pa, yes(), yes(), yes());
+    }
+    if (t + 1 < cnt) {                             // t odd, t + 1 = cnt - 1
+      iter(t, sa, sb, pa, pb, yes(), yes(), yes());
+      iter(t + 1, sb, sa, pb, pa, no(), yes(), yes());
+      iter(t + 2, sa, sb, pa, pb, no(), yes(), no());
+    } else if (t < cnt) {                          // t = cnt - 1, odd
+      iter(t, sa, sb, pa, pb, no(), yes(), yes());
+      iter(t + 1, sb, sa, pb, pa, no(), yes(), no());
+    } else {                                       // cnt == 1: the final P V
+      iter(t, sa, sb, pa, pb, no(), yes(), no());
+    }
+  }
+  if (!me.on) return;
+  if (pc.slot >= 0) {
+    const int64_t s = (int64_t)pc.slot * 4 + wave;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        reinterpret_cast<float4*>(a.part_o)[((s * (D / 32) + dt) * 4 + g4) * 64 + lane] =
+            make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+    if (hi == 0) {
+      a.part_ml[s * 64 + l32] = m_run;
+      a.part_ml[s * 64 + 32 + l32] = l_run;
+    }
+    return;
+  }
+  const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;
+  uint16_t* op = out_row(a, u, me, pc.b, pc.hk);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4)
+      store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, o[dt][4 * g4] * inv, o[dt][4 * g4 + 1] * inv, o[dt][4 * g4 + 2] * inv,
+                   o[dt][4 * g4 + 3] * inv);
+}
+
+// The pieces of one call, for one KV head (all have the same): row tiles of every request, and the
+// number of key tiles per piece that ends soonest.  With W key tiles in all, N pieces of at most c
+// and S workgroups at a time, a call takes about min(ceil(N / S) c, W / S + c) tiles' time, and each round
+// of pieces some tiles' time for its start and, where sums are joined, their writing and reading.
+// One workgroup; its lists are read by the attention and the joining kernel.
+template <int M, int TK>
+__global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a, int4* pieces, int4* pairs, int32_t* head,
+                                                                   int max_pairs, int max_pieces, int max_parts,
+                                                                   int slots) {
+  constexpr int NC = 12;                           // choices of c
+  constexpr int kStart = 2, kJoin = 3;             // of a round, in tiles
+  __shared__ int base[kMaxRequests + 1];
+  __shared__ int wsum[2][kPlanThreads / 64];
+  __shared__ unsigned long long total_tiles;
+  __shared__ int longest, count[NC], split[NC], choice;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) {
+    total_tiles = 0;
+    longest = 0;
+  }
+  if (tid < NC) count[tid] = split[tid] = 0;
+  // inclusive prefix sums over the workgroup of two values, held at 2^30; sums of all in all0, all1
+  auto sum = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, 1u << 30); };
+  auto scan2 = [&](int& x, int& y, int& all0, int& all1) {
+    for (int o = 1; o < 64; o <<= 1) {
+      const int p = __shfl_up(x, o, 64), q = __shfl_up(y, o, 64);
+      if (lane >= o) {
+        x = sum(x, p);
+        y = sum(y, q);
+      }
+    }
+    __syncthreads();
+    if (lane == 63) {
+      wsum[0][wave] = x;
+      wsum[1][wave] = y;
+    }
+    __syncthreads();
+    int b0 = 0, b1 = 0;
+    all0 = all1 = 0;
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+      if (w < wave) {
+        b0 = sum(b0, wsum[0][w]);
+        b1 = sum(b1, wsum[1][w]);
+      }
+      all0 = sum(all0, wsum[0][w]);
+      all1 = sum(all1, wsum[1][w]);
+    }
+    x = sum(x, b0);
+    y = sum(y, b1);
+  };
+  auto tiles_of = [&](int b) {
+    const int n = a.table != nullptr ? min(max(a.cu[b + 1] - a.cu[b], 0), a.T) : a.Lq;
+    return (int)(((int64_t)n * a.G + M - 1) / M);
+  };
+  int R = 0, dummy;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const int b = b0 + tid, n = b < a.B ? min(tiles_of(b), max_pairs) : 0;
+    int x = n, y = 0, all;
+    scan2(x, y, all, dummy);
+    if (b < a.B) base[b] = min(R + x - n, max_pairs);
+    R = min(sum(R, all), max_pairs);               // more only for row numbers that do not rise
+  }
+  if (tid == 0) base[a.B] = R;
+  __syncthreads();
+  for (int i = tid; i < R; i += kPlanThreads) {
+    int lo = 0, hi = a.B;                          // the last request with base <= i
+    while (hi - lo > 1) {
+      const int m = (lo + hi) >> 1;
+      if (base[m] <= i) lo = m;
+      else hi = m;
+    }
+    const int rt = base[lo + 1] - 1 - i;           // the last row tiles, whose keys are the most, first
+    const int nt = row_tile<M, TK>(a, lo, rt).nt;
+    pairs[i] = make_int4(lo, rt, nt, 0);
+    atomicAdd(&total_tiles, (unsigned long long)nt);
+    atomicMax(&longest, nt);
+  }
+  __syncthreads();
+  const int most = max(longest, 1);
+  const int64_t W = (int64_t)total_tiles * a.Hk;
+  auto chunk_of = [&](int i) {
+    const int c = i < 8 ? (most + i) / (i + 1) : (int)min((W + ((int64_t)slots << (i - 8)) - 1) / ((int64_t)slots << (i - 8)), (int64_t)most);
+    return max(c, 1);
+  };
+  int cn[NC] = {}, cs[NC] = {};
+  for (int i = tid; i < R; i += kPlanThreads) {
+    const int nt = pairs[i].z;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int np = max((nt + chunk_of(k) - 1) / chunk_of(k), 1);
+      cn[k] += np;
+      cs[k] += np > 1 ? np : 0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int n = wave_sum_i(cn[k]), s = wave_sum_i(cs[k]);
+    if (lane == 0 && n) {
+      atomicAdd(&count[k], n);
+      atomicAdd(&split[k], s);
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int best = most;
+    int64_t least = INT64_MAX;
+    for (int k = 0; k < NC; ++k) {
+      const int64_t N = (int64_t)count[k] * a.Hk, c = chunk_of(k), rounds = (N + slots - 1) / slots;
+      if (k > 0 && (count[k] > max_pieces || (int64_t)split[k] * a.Hk > max_parts)) continue;
+      const int64_t t = min(rounds * c, W / slots + c) + rounds * kStart + (split[k] ? kJoin * rounds : 0);
+      if (t < least) {
+        least = t;
+        best = (int)c;
+      }
+    }
+    choice = best;
+  }
+  __syncthreads();
+  const int c = choice;
+  int N = 0, S = 0;
+  for (int i0 = 0; i0 < R; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int4 pr = i < R ? pairs[i] : make_int4(0, 0, 0, 0);
+    const int np = i < R ? max((pr.z + c - 1) / c, 1) : 0;
+    int x = np, y = np > 1 ? np : 0, all0, all1;
+    scan2(x, y, all0, all1);
+    if (i < R) {
+      const int n0 = N + x - np, s0 = np > 1 ? S + y - np : -1;
+      pairs[i] = make_int4(pr.x, pr.y, np, s0);
+      for (int j = 0; j < np; ++j) pieces[n0 + j] = make_int4(pr.x, pr.y, j * c, np > 1 ? s0 + j : -1);
+    }
+    N += all0;
+    S += all1;
+  }
+  if (tid == 0) {
+    head[0] = N;
+    head[1] = R;
+    head[2] = c;
+    head[3] = S;
+  }
+}
+
+// ---- host ---------------------------------------------------------------------
+
+// Workspace of a call: head, pairs, pieces, the split pieces' sums.
+struct Work {
+  int max_pairs, max_pieces, max_parts, rows;
+  size_t pairs, pieces, ml, o, bytes;
+};
+static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+// row tiles of at most `rows` rows of B requests with T tokens in all; few: row tiles of 32
+static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
+  Work w;
+  w.rows = few ? 32 : 128;
+  w.max_pairs = (int)(T * G / w.rows + B);
+  w.max_parts = few ? kPartsFew : kPartsMany;
+  w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
+  w.pairs = 256;
+  w.pieces = w.pairs + align256((size_t)w.max_pairs * 16);
+  w.ml = w.pieces + align256((size_t)w.max_pieces * 16);
+  w.o = w.ml + align256((size_t)w.max_parts * w.rows * 8);
+  w.bytes = w.o + (size_t)w.max_parts * w.rows * D * 4;
+  return w;
+}
+// Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.
+static bool few_rows(int64_t max_new, int G) { return max_new * G <= 32; }
+
+template <typename T, int D, bool PAGED>
+static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, int B, int Lq, hipStream_t s, const char* fn) {
+  const int64_t rows = (int64_t)Lq * k.G;
+  k.row_tiles = (int)((rows + w.rows - 1) / w.rows);
+  int64_t grid = (int64_t)B * k.row_tiles * k.Hk;
+  if (plan) {
+    int4* pairs = reinterpret_cast<int4*>(work + w.pairs);
+    int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
+    int32_t* head = reinterpret_cast<int32_t*>(work);
+    if (few) plan_pieces_kernel<32, 128><<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, head, w.max_pairs, w.max_pieces, w.max_parts, D == 128 ? kSlotsFew : 2 * kSlotsFew);
+    else plan_pieces_kernel<128, 64><<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, head, w.max_pairs, w.max_pieces, w.max_parts, kSlotsMany);
+    if (int rc = fs_host::launch_status(fn)) return rc;
+    k.pieces = pieces;
+    k.pairs = pairs;
+    k.head = head;
+    k.part_ml = reinterpret_cast<float*>(work + w.ml);
+    k.part_o = reinterpret_cast<float*>(work + w.o);
+    grid = (int64_t)w.max_pieces * k.Hk;
+  }
+  if (few) few_kernel<T, D, PAGED><<<(unsigned)grid, 256, 0, s>>>(k);
+  else many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
+  if (int rc = fs_host::launch_status(fn)) return rc;
+  if (plan) {
+    const unsigned parts = (unsigned)((int64_t)w.max_pairs * k.Hk * (w.rows / 32));
+    if (few) combine_kernel<T, D, 32><<<parts, 2 * D, 0, s>>>(k);
+    else combine_kernel<T, D, 128><<<parts, 2 * D, 0, s>>>(k);
+    return fs_host::launch_status(fn);
+  }
+  return FS_OK;
+}
+template <bool PAGED>
+static int run(PagedKArgs k, int dtype, int D, bool few, bool plan, const Work& w, char* work, int B, int Lq, hipStream_t s,
+               const char* fn) {
+  k.G = k.Hq / k.Hk;
+  k.window = k.window > (1 << 27) ? 1 << 27 : k.window;   // past the longest sequence: the same rule
+  k.sinks = k.sinks > (1 << 27) ? 1 << 27 : k.sinks;
+  if (dtype == FS_DTYPE_BF16)
+    return D == 128 ? launch<bf16_t, 128, PAGED>(k, few, plan, w, work, B, Lq, s, fn)
+                    : launch<bf16_t, 64, PAGED>(k, few, plan, w, work, B, Lq, s, fn);
+  return D == 128 ? launch<f16_t, 128, PAGED>(k, few, plan, w, work, B, Lq, s, fn)
+                  : launch<f16_t, 64, PAGED>(k, few, plan, w, work, B, Lq, s, fn);
 }
 
 }  // namespace fs
@@ -113,7 +927,7 @@ static int run(const PagedKArgs& k, int dtype, int D, int64_t rows, hipStream_t 
 using namespace fs;
 
 // checks that both entry points share
-static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int window, int sinks, int64_t rows,
+static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int B, int window, int sinks, int64_t rows,
                         const int64_t* strides, int ns, const void* const* ptrs, int np) {
   FS_CHECK_ARG(Hq >= 1 && Hk >= 1 && Hq % Hk == 0, "%s: Hq=%d must be a multiple of Hk=%d", fn, Hq, Hk);
   FS_CHECK_SUPPORTED(D == 128 || D == 64, "%s: head_dim %d unsupported (64 or 128)", fn, D);
@@ -121,6 +935,7 @@ static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int wi
   FS_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window %d and sinks %d must not be negative", fn, window, sinks);
   FS_CHECK_SUPPORTED(rows * Hq < (1ll << 30) && Hk <= 4096, "%s: %lld rows of %d heads unsupported", fn,
                      (long long)rows, Hq);
+  FS_CHECK_SUPPORTED(B <= kMaxRequests, "%s: %d requests > %d", fn, B, kMaxRequests);
   for (int i = 0; i < ns; ++i) FS_CHECK_ARG(strides[i] % 8 == 0, "%s: strides must be multiples of 8 elements", fn);
   for (int i = 0; i < np; ++i) {
     FS_CHECK_ARG(ptrs[i] != nullptr, "%s: null tensor pointer", fn);
@@ -129,8 +944,23 @@ static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int wi
   return FS_OK;
 }
 
-extern "C" size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a) { return a ? 16 : 0; }
-extern "C" size_t fs_window_attn_work_bytes(const fs_window_attn_args* a) { return a ? 16 : 0; }
+// the most new tokens of one request
+static int64_t most_new(const fs_paged_attn_args& a) { return a.max_new > 0 && a.max_new < a.T ? a.max_new : a.T; }
+static Work work_of(const fs_paged_attn_args& a) {
+  return work_of(few_rows(most_new(a), a.Hq / a.Hk), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D);
+}
+static Work work_of(const fs_window_attn_args& a) {
+  return work_of(few_rows(a.Lq, a.Hq / a.Hk), (int64_t)a.B * a.Lq, a.B, a.Hk, a.Hq / a.Hk, a.D);
+}
+
+extern "C" size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a) {
+  if (!a || a->B <= 0 || a->T <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
+  return work_of(*a).bytes;
+}
+extern "C" size_t fs_window_attn_work_bytes(const fs_window_attn_args* a) {
+  if (!a || a->B <= 0 || a->Lq <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
+  return work_of(*a).bytes;
+}
 
 extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   const char* fn = "fs_paged_attn";
@@ -144,22 +974,28 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   if (a->T == 0) return FS_OK;
   const int64_t st[] = {a->q_st, a->q_sh, a->o_st, a->o_sh, a->k_sp, a->k_ss, a->k_sh, a->v_sp, a->v_ss, a->v_sh};
   const void* const ptrs[] = {a->q, a->out, a->k_cache, a->v_cache, a->work};
-  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->window, a->sinks, a->T, st, 10, ptrs, 5)) return rc;
+  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, a->T, st, 10, ptrs, 5)) return rc;
   FS_CHECK_ARG(a->block_table && a->cu_lens && a->seq_lens && a->t_sb >= a->P &&
                    ((uintptr_t)a->block_table | (uintptr_t)a->cu_lens | (uintptr_t)a->seq_lens) % 4 == 0,
                "%s: block_table (row stride %lld of %d), cu_lens and seq_lens must be given, 4-byte aligned", fn,
                (long long)a->t_sb, a->P);
+  // a copy's lane offsets are 32-bit byte offsets over 16 slots
+  FS_CHECK_SUPPORTED(a->k_ss >= 0 && a->k_ss < (1 << 23) && a->v_ss >= 0 && a->v_ss < (1 << 23),
+                     "%s: slot stride unsupported", fn);
   PagedKArgs k{};
   k.q = static_cast<const uint16_t*>(a->q);
   k.k = static_cast<const uint16_t*>(a->k_cache);
   k.v = static_cast<const uint16_t*>(a->v_cache);
   k.out = static_cast<uint16_t*>(a->out);
   k.q_st = a->q_st; k.q_sh = a->q_sh; k.o_st = a->o_st; k.o_sh = a->o_sh;
-  k.k_sp = a->k_sp; k.k_ss = a->k_ss; k.k_sh = a->k_sh; k.v_sp = a->v_sp; k.v_ss = a->v_ss; k.v_sh = a->v_sh;
+  k.k_sp = a->k_sp; k.k_ss = (int)a->k_ss; k.k_sh = a->k_sh; k.v_sp = a->v_sp; k.v_ss = (int)a->v_ss; k.v_sh = a->v_sh;
   k.table = a->block_table; k.cu = a->cu_lens; k.lens = a->seq_lens; k.t_sb = a->t_sb; k.num_pages = a->num_pages;
   k.B = a->B; k.T = a->T; k.Hq = a->Hq; k.Hk = a->Hk; k.P = a->P; k.page_size = a->page_size;
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
-  return run(k, a->dtype, a->D, a->T, (hipStream_t)stream, fn);
+  const uint32_t groups = a->page_size / 16;       // x / groups for x < 2^22, groups <= 256: mulhi is exact
+  k.page_magic = groups > 1 ? (uint32_t)((1ull << 32) / groups + 1) : 0;
+  const bool few = few_rows(most_new(*a), a->Hq / a->Hk);
+  return run<true>(k, a->dtype, a->D, few, true, work_of(*a), static_cast<char*>(a->work), a->B, a->T, (hipStream_t)stream, fn);
 }
 
 extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
@@ -170,17 +1006,26 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   const int64_t st[] = {a->q_sb, a->q_sh, a->q_sl, a->k_sb, a->k_sh, a->k_sl,
                         a->v_sb, a->v_sh, a->v_sl, a->o_sb, a->o_sh, a->o_sl};
   const void* const ptrs[] = {a->q, a->out, a->k, a->v, a->work};
-  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->window, a->sinks, (int64_t)a->B * a->Lq, st, 12,
+  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, (int64_t)a->B * a->Lq, st, 12,
                             ptrs, 5))
     return rc;
+  FS_CHECK_SUPPORTED(a->k_sl >= 0 && a->k_sl < (1 << 23) && a->v_sl >= 0 && a->v_sl < (1 << 23),
+                     "%s: row stride unsupported", fn);
   PagedKArgs k{};
   k.q = static_cast<const uint16_t*>(a->q);
   k.k = static_cast<const uint16_t*>(a->k);
   k.v = static_cast<const uint16_t*>(a->v);
   k.out = static_cast<uint16_t*>(a->out);
   k.q_sb = a->q_sb; k.q_st = a->q_sl; k.q_sh = a->q_sh; k.o_sb = a->o_sb; k.o_st = a->o_sl; k.o_sh = a->o_sh;
-  k.k_sp = a->k_sb; k.k_ss = a->k_sl; k.k_sh = a->k_sh; k.v_sp = a->v_sb; k.v_ss = a->v_sl; k.v_sh = a->v_sh;
+  k.k_sp = a->k_sb; k.k_ss = (int)a->k_sl; k.k_sh = a->k_sh; k.v_sp = a->v_sb; k.v_ss = (int)a->v_sl; k.v_sh = a->v_sh;
   k.num_pages = a->B; k.B = a->B; k.Hq = a->Hq; k.Hk = a->Hk; k.Lq = a->Lq; k.Lk = a->Lk; k.page_size = a->Lk;
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
-  return run(k, a->dtype, a->D, (int64_t)a->B * a->Lq, (hipStream_t)stream, fn);
+  k.T = a->Lq;
+  const bool few = few_rows(a->Lq, a->Hq / a->Hk);
+  const Work w = work_of(*a);
+  // Every sequence is as long here: whether splitting keys can pay is known.
+  const int64_t tiles = ((int64_t)a->Lq * (a->Hq / a->Hk) + w.rows - 1) / w.rows * a->B * a->Hk;
+  const int64_t keys = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
+  const bool plan = tiles < (few ? kSlotsFew : kSlotsMany) && keys >= 1024;
+  return run<false>(k, a->dtype, a->D, few, plan, w, static_cast<char*>(a->work), a->B, a->Lq, (hipStream_t)stream, fn);
 }
