@@ -36,8 +36,13 @@
 
 namespace fs {
 
-constexpr int kSlotsFew = 256, kSlotsMany = 512;    // workgroups that 256 CUs hold (D = 128)
-constexpr int kPartsFew = 2048, kPartsMany = 1024;  // split pieces that the workspace holds
+#ifndef FEW_WAVES
+#define FEW_WAVES 2
+#endif
+constexpr int kFewWaves = FEW_WAVES;                // of a workgroup of few_kernel
+constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
+static int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
+constexpr int kPartsFew = 8192 / FEW_WAVES, kPartsMany = 1024;  // split pieces that the workspace holds
 constexpr int kMaxRequests = 4096;
 constexpr int kPlanThreads = 1024;
 
@@ -58,8 +63,9 @@ struct PagedKArgs {
   float scale;
   // pieces: null = one piece per row tile, the last row tiles of a request first
   const int4* pieces;                           // [N] request, row tile, first key tile, slot (-1: the only piece)
-  const int4* pairs;                            // [R] request, row tile, pieces, first slot
-  const int32_t* head;                          // N, R, chunk, split pieces (of one KV head)
+  const int4* splits;                           // [Q] request, row tile, pieces, first slot
+  const int32_t* head;                          // N, Q, chunk, split pieces (of one KV head)
+  int max_splits;
   int row_tiles;                                // of a request (no list)
   float* part_o;                                // [slot][rows / 32][D / 32][4][64 lanes] 4 floats
   float* part_ml;                               // [slot][rows / 32][2][32]
@@ -268,20 +274,23 @@ __device__ __forceinline__ bool find_piece(const PagedKArgs& a, int p, Piece& w)
 }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+// f16 holds weights down to 2^-24; taken 2^7 times as large they reach from 2^15 (past the slack) to 2^-31 of the
+// running maximum's weight
+template <typename T> constexpr float kBias = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
 constexpr float kSlack = 8.0f;                     // a row's running max is raised past 2^8 only: few rescales of O
 
-template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
+template <typename T, int D, bool PAGED, int NW>
+__global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
   using Ops = MfmaOps<T>;
   using V8 = typename Ops::V8;
   using Copy = GroupCopy<D, PAGED>;
   constexpr int TILE = 32 * D * 2;                 // bytes of 32 keys
   constexpr int RING = 4 * TILE;                   // of a wave: two K tiles, two V tiles
   constexpr int NI = 2 * Copy::NI;                 // copies of 32 keys
-  __shared__ __attribute__((aligned(1024))) char lds[4 * RING];
+  __shared__ __attribute__((aligned(1024))) char lds[NW * RING];
   Piece pc;
   if (!find_piece(a, blockIdx.x, pc)) return;
-  const RowTile u = row_tile<32, 128>(a, pc.b, pc.rt);
+  const RowTile u = row_tile<32, 32 * NW>(a, pc.b, pc.rt);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const LaneRow me = lane_row(a, u, l32);
@@ -291,10 +300,10 @@ __global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
   V8 qf[D / 16];
   load_q<V8, D>(a, u, me, pc.b, pc.hk, hi, qf);
 
-  // this wave's 32 keys of each of the piece's tiles of 128
+  // this wave's 32 keys of each of the piece's tiles
   auto key_of = [&](int i) {
     const int o = pc.begin + i;
-    return (o < u.ns ? o : u.t0 + o - u.ns) * 128 + 32 * wave;
+    return (o < u.ns ? o : u.t0 + o - u.ns) * (32 * NW) + 32 * wave;
   };
   int cnt = min(pc.count, u.nt - pc.begin);
   if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
@@ -370,7 +379,7 @@ __global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
     const bool up = mx > m_run + kSlack;
     const float al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
     m_run = up ? mx : m_run;
-    const float mu = m_run == -INFINITY ? 0.f : m_run;
+    const float mu = (m_run == -INFINITY ? 0.f : m_run) - kBias<T>;
     V8 pb[2];
     float rs = 0.f;
 #pragma unroll
@@ -408,7 +417,7 @@ __global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
     x1 = x2;
     x2 = x3;
   }
-  // ---- the four waves' sums joined through LDS, wave w taking dims 32 w ..
+  // ---- the waves' sums joined through LDS, wave w taking dims 32 w, 32 (w + NW) ..
   constexpr int NV = D / 32;
   float* own = reinterpret_cast<float*>(ring);     // [D / 32][4][64 lanes] 4 floats, then m and l
 #pragma unroll
@@ -421,13 +430,13 @@ __global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
   own[ML + lane] = m_run;
   own[ML + 64 + lane] = l_run;
   __syncthreads();
-  if (wave >= NV || !me.on) return;
-  float m = -INFINITY, l = 0.f, f[4];
+  if (!me.on) return;
+  float m = -INFINITY, l = 0.f, f[NW];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
+  for (int w = 0; w < NW; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
   const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     const float* x = reinterpret_cast<const float*>(lds + w * RING) + ML;
     f[w] = __builtin_amdgcn_exp2f(x[lane] - mu);
     l += x[64 + lane] * f[w];
@@ -435,65 +444,99 @@ __global__ __launch_bounds__(256) void few_kernel(PagedKArgs a) {
   const float inv = l != 0.f ? 1.0f / l : 0.f;
   uint16_t* op = out_row(a, u, me, pc.b, pc.hk);
 #pragma unroll
-  for (int g4 = 0; g4 < 4; ++g4) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int dt = wave; dt < NV; dt += NW)
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(wave * 4 + g4) * 64 + lane];
-      acc.x += x.x * f[w];
-      acc.y += x.y * f[w];
-      acc.z += x.z * f[w];
-      acc.w += x.w * f[w];
+    for (int g4 = 0; g4 < 4; ++g4) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(dt * 4 + g4) * 64 + lane];
+        acc.x += x.x * f[w];
+        acc.y += x.y * f[w];
+        acc.z += x.z * f[w];
+        acc.w += x.w * f[w];
+      }
+      if (pc.slot < 0) store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      else reinterpret_cast<float4*>(a.part_o)[(((int64_t)pc.slot * NV + dt) * 4 + g4) * 64 + lane] = acc;
     }
-    if (pc.slot < 0) store_out<T>(op, wave * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    else reinterpret_cast<float4*>(a.part_o)[(((int64_t)pc.slot * NV + wave) * 4 + g4) * 64 + lane] = acc;
-  }
   if (pc.slot >= 0 && wave == 0 && hi == 0) {
     a.part_ml[(int64_t)pc.slot * 64 + l32] = m;
     a.part_ml[(int64_t)pc.slot * 64 + 32 + l32] = l;
   }
 }
 
-// One 32-row part of one row tile per workgroup, wave w taking dims 32 w ..: the pieces' sums joined in their order.
+// The pieces' sums joined: 32 rows and 32 dims of a split row tile per workgroup.  A thread adds 4 dims of one
+// row over every J-th piece (J as many threads as 256 give an item), then the J sums are added in LDS; always in
+// the same order.
 template <typename T, int D, int M>
-__global__ __launch_bounds__(2 * D) void combine_kernel(PagedKArgs a) {
-  constexpr int NV = D / 32, QW = M / 32;
-  const int R = scalar_load(a.head, 1);
-  const int part = blockIdx.x % QW, pu = blockIdx.x / QW;
-  if (pu >= R * a.Hk) return;
-  const int hk = pu / R;
-  const int4 pr = a.pairs[pu - hk * R];
-  const int np = __builtin_amdgcn_readfirstlane(pr.z);
-  if (np <= 1) return;
-  const int b = __builtin_amdgcn_readfirstlane(pr.x);
-  const RowTile u = row_tile<M, 64>(a, b, __builtin_amdgcn_readfirstlane(pr.y));
-  const int64_t s0 = (int64_t)(__builtin_amdgcn_readfirstlane(pr.w) + hk * a.head[3]) * QW + part;
-  const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5, wave = threadIdx.x >> 6;
-  const LaneRow me = lane_row(a, u, part * 32 + l32);
-  if (!me.on) return;
-  float m = -INFINITY;
-  for (int j = 0; j < np; ++j) m = fmaxf(m, a.part_ml[(s0 + (int64_t)j * QW) * 64 + l32]);
-  const float mu = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  float4 acc[4] = {};
-  for (int j = 0; j < np; ++j) {
-    const int64_t s = s0 + (int64_t)j * QW;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[s * 64 + l32] - mu);
-    l += a.part_ml[s * 64 + 32 + l32] * f;
+__global__ __launch_bounds__(256) void combine_kernel(PagedKArgs a) {
+  constexpr int NV = D / 32, QW = M / 32, AHEAD = 4;
+  __shared__ float4 part[256];
+  __shared__ float2 ml[256];
+  int w = blockIdx.x;
+  const int dt = w % NV;
+  w /= NV;
+  const int qq = w % QW;
+  w /= QW;
+  const int Q = scalar_load(a.head, 1), hk = w / a.max_splits, i = w - hk * a.max_splits;
+  if (i >= Q) return;
+  const int32_t* e = reinterpret_cast<const int32_t*>(a.splits + i);
+  const int b = scalar_load(e, 0), rt = scalar_load(e, 1), np = scalar_load(e, 2);
+  const int64_t s0 = (int64_t)(scalar_load(e, 3) + hk * scalar_load(a.head, 3)) * QW + qq;
+  const RowTile u = row_tile<M, 64>(a, b, rt);
+  const int rows = min(u.nrows - qq * 32, 32);
+  if (rows <= 0) return;
+  const int items = rows * 8, J = 256 / items;     // an item: row, half, quarter of 32 dims
+  const int tid = threadIdx.x, jg = tid / items, it = tid - jg * items;
+  const int r = it % rows, hi = (it / rows) & 1, g4 = it / rows >> 1;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (jg < J)
+    for (int j0 = jg; j0 < np; j0 += AHEAD * J) {
+      float mj[AHEAD], lj[AHEAD];
+      float4 xj[AHEAD];
 #pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {
-      const float4 x = reinterpret_cast<const float4*>(a.part_o)[((s * NV + wave) * 4 + g4) * 64 + lane];
-      acc[g4].x += x.x * f;
-      acc[g4].y += x.y * f;
-      acc[g4].z += x.z * f;
-      acc[g4].w += x.w * f;
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t s = s0 + (int64_t)min(j0 + k * J, np - 1) * QW;
+        mj[k] = a.part_ml[s * 64 + r];
+        lj[k] = a.part_ml[s * 64 + 32 + r];
+        xj[k] = reinterpret_cast<const float4*>(a.part_o)[((s * NV + dt) * 4 + g4) * 64 + hi * 32 + r];
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (j0 + k * J >= np) break;
+        const float mn = fmaxf(m, mj[k]), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(mj[k] - mu);
+        m = mn;
+        l = l * f0 + lj[k] * f1;
+        acc.x = acc.x * f0 + xj[k].x * f1;
+        acc.y = acc.y * f0 + xj[k].y * f1;
+        acc.z = acc.z * f0 + xj[k].z * f1;
+        acc.w = acc.w * f0 + xj[k].w * f1;
+      }
+    }
+  if (J > 1) {
+    part[tid] = acc;
+    ml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (jg > 0) return;
+    for (int k = 1; k < J; ++k) {
+      const float2 o = ml[k * items + it];
+      const float4 x = part[k * items + it];
+      const float mn = fmaxf(m, o.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(o.x - mu);
+      m = mn;
+      l = l * f0 + o.y * f1;
+      acc.x = acc.x * f0 + x.x * f1;
+      acc.y = acc.y * f0 + x.y * f1;
+      acc.z = acc.z * f0 + x.z * f1;
+      acc.w = acc.w * f0 + x.w * f1;
     }
   }
+  const LaneRow me = lane_row(a, u, qq * 32 + r);
+  if (jg > 0 || !me.on) return;
   const float inv = l != 0.f ? 1.0f / l : 0.f;
-  uint16_t* op = out_row(a, u, me, b, hk);
-#pragma unroll
-  for (int g4 = 0; g4 < 4; ++g4)
-    store_out<T>(op, wave * 32 + g4 * 8 + hi * 4, acc[g4].x * inv, acc[g4].y * inv, acc[g4].z * inv, acc[g4].w * inv);
+  store_out<T>(out_row(a, u, me, b, hk), dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 template <typename T, int D, bool PAGED>
@@ -627,7 +670,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       const bool up = mx > m_run + kSlack;
       al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
       m_run = up ? mx : m_run;
-      rs = exps(s_cur, p_cur, m_run == -INFINITY ? 0.f : m_run);
+      rs = exps(s_cur, p_cur, (m_run == -INFINITY ? 0.f : m_run) - kBias<T>);
     }
     if constexpr (decltype(hasS)::value && decltype(hasPV)::value && decltype(hasE)::value) {
       // one MFMA, then three VALU instructions, operand reads six MFMAs ahead (as measured for bsattn_kernel)
@@ -714,68 +757,58 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
 // The pieces of one call, for one KV head (all have the same): row tiles of every request, and the
 // number of key tiles per piece that ends soonest.  With W key tiles in all, N pieces of at most c
-// and S workgroups at a time, a call takes about min(ceil(N / S) c, W / S + c) tiles' time, and each round
-// of pieces some tiles' time for its start and, where sums are joined, their writing and reading.
+// and S workgroups at a time, a call takes about min(ceil(N / S) c, W / S + c) tiles' time, a start per
+// round of pieces and, where sums are joined, the joining.  16 choices of c are tried, one by each wave: the
+// longest row tile's i-th part, and the c that gives about i rounds.
 // One workgroup; its lists are read by the attention and the joining kernel.
 template <int M, int TK>
-__global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a, int4* pieces, int4* pairs, int32_t* head,
-                                                                   int max_pairs, int max_pieces, int max_parts,
-                                                                   int slots) {
-  constexpr int NC = 12;                           // choices of c
-  constexpr int kStart = 2, kJoin = 3;             // of a round, in tiles
-  __shared__ int base[kMaxRequests + 1];
-  __shared__ int wsum[2][kPlanThreads / 64];
-  __shared__ unsigned long long total_tiles;
-  __shared__ int longest, count[NC], split[NC], choice;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (tid == 0) {
-    total_tiles = 0;
-    longest = 0;
-  }
-  if (tid < NC) count[tid] = split[tid] = 0;
-  // inclusive prefix sums over the workgroup of two values, held at 2^30; sums of all in all0, all1
+__global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a, int4* pieces, int4* pairs, int4* splits,
+                                                                   int32_t* head, int max_pairs, int max_pieces,
+                                                                   int max_parts, int slots) {
+  constexpr int NW = kPlanThreads / 64;
+  constexpr int kHeld = 8192;                      // row tiles whose key tiles are kept in LDS
+  constexpr float kStart = 1.5f, kJoin = 2.0f;     // in tiles' time
+  __shared__ int base[kMaxRequests + 1], tiles[kHeld];
+  __shared__ int wsum[3][NW];
+  __shared__ float wtot[NW], cost[NW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // inclusive prefix sums over the workgroup of three values, held at 2^30; sums of all in all[]
   auto sum = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, 1u << 30); };
-  auto scan2 = [&](int& x, int& y, int& all0, int& all1) {
-    for (int o = 1; o < 64; o <<= 1) {
-      const int p = __shfl_up(x, o, 64), q = __shfl_up(y, o, 64);
-      if (lane >= o) {
-        x = sum(x, p);
-        y = sum(y, q);
+  auto scan = [&](int (&x)[3], int (&all)[3], int n) {
+    for (int k = 0; k < n; ++k)
+      for (int o = 1; o < 64; o <<= 1) {
+        const int p = __shfl_up(x[k], o, 64);
+        if (lane >= o) x[k] = sum(x[k], p);
       }
-    }
     __syncthreads();
-    if (lane == 63) {
-      wsum[0][wave] = x;
-      wsum[1][wave] = y;
-    }
+    if (lane == 63)
+      for (int k = 0; k < n; ++k) wsum[k][wave] = x[k];
     __syncthreads();
-    int b0 = 0, b1 = 0;
-    all0 = all1 = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wave) {
-        b0 = sum(b0, wsum[0][w]);
-        b1 = sum(b1, wsum[1][w]);
+    for (int k = 0; k < n; ++k) {
+      int before = 0;
+      all[k] = 0;
+      for (int w = 0; w < NW; ++w) {
+        if (w == wave) before = all[k];
+        all[k] = sum(all[k], wsum[k][w]);
       }
-      all0 = sum(all0, wsum[0][w]);
-      all1 = sum(all1, wsum[1][w]);
+      x[k] = sum(x[k], before);
     }
-    x = sum(x, b0);
-    y = sum(y, b1);
   };
-  auto tiles_of = [&](int b) {
-    const int n = a.table != nullptr ? min(max(a.cu[b + 1] - a.cu[b], 0), a.T) : a.Lq;
-    return (int)(((int64_t)n * a.G + M - 1) / M);
-  };
-  int R = 0, dummy;
+  int R = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
-    const int b = b0 + tid, n = b < a.B ? min(tiles_of(b), max_pairs) : 0;
-    int x = n, y = 0, all;
-    scan2(x, y, all, dummy);
-    if (b < a.B) base[b] = min(R + x - n, max_pairs);
-    R = min(sum(R, all), max_pairs);               // more only for row numbers that do not rise
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < a.B) n = a.table != nullptr ? min(max(a.cu[b + 1] - a.cu[b], 0), a.T) : a.Lq;
+    n = min((int)(((int64_t)n * a.G + M - 1) / M), max_pairs);
+    int x[3] = {n, 0, 0}, all[3];
+    scan(x, all, 1);
+    if (b < a.B) base[b] = min(R + x[0] - n, max_pairs);
+    R = min(sum(R, all[0]), max_pairs);            // more only for row numbers that do not rise
   }
   if (tid == 0) base[a.B] = R;
   __syncthreads();
+  float total = 0.f;                               // an estimate: its rounding does not matter
+  int longest = 1;
   for (int i = tid; i < R; i += kPlanThreads) {
     int lo = 0, hi = a.B;                          // the last request with base <= i
     while (hi - lo > 1) {
@@ -786,69 +819,68 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
     const int rt = base[lo + 1] - 1 - i;           // the last row tiles, whose keys are the most, first
     const int nt = row_tile<M, TK>(a, lo, rt).nt;
     pairs[i] = make_int4(lo, rt, nt, 0);
-    atomicAdd(&total_tiles, (unsigned long long)nt);
-    atomicMax(&longest, nt);
+    if (i < kHeld) tiles[i] = nt;
+    total += (float)nt;
+    longest = max(longest, nt);
+  }
+  total = wave_sum(total);
+  for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
+  if (lane == 0) {
+    wtot[wave] = total;
+    wsum[0][wave] = longest;
   }
   __syncthreads();
-  const int most = max(longest, 1);
-  const int64_t W = (int64_t)total_tiles * a.Hk;
+  total = 0.f;
+  for (int w = 0; w < NW; ++w) {
+    total += wtot[w];
+    longest = max(longest, wsum[0][w]);
+  }
+  const float W = total * (float)a.Hk;
   auto chunk_of = [&](int i) {
-    const int c = i < 8 ? (most + i) / (i + 1) : (int)min((W + ((int64_t)slots << (i - 8)) - 1) / ((int64_t)slots << (i - 8)), (int64_t)most);
-    return max(c, 1);
+    if (i < 8) return (longest + i) / (i + 1);
+    const float s = (float)slots * (float)(i - 7);
+    return max(1, min(longest, (int)ceilf(W / (s - 0.5f * fminf((float)R * (float)a.Hk, s)))));
   };
-  int cn[NC] = {}, cs[NC] = {};
-  for (int i = tid; i < R; i += kPlanThreads) {
-    const int nt = pairs[i].z;
-#pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      const int np = max((nt + chunk_of(k) - 1) / chunk_of(k), 1);
-      cn[k] += np;
-      cs[k] += np > 1 ? np : 0;
+  auto parts = [](int nt, int c) { return max((int)((float)(nt + c - 1) / (float)c), 1); };   // exact below 2^22
+  {
+    const int c = chunk_of(wave);
+    int n = 0, sp = 0;
+    for (int i = lane; i < R; i += 64) {
+      const int np = parts(i < kHeld ? tiles[i] : pairs[i].z, c);
+      n += np;
+      sp += np > 1 ? np : 0;
     }
-  }
-#pragma unroll
-  for (int k = 0; k < NC; ++k) {
-    const int n = wave_sum_i(cn[k]), s = wave_sum_i(cs[k]);
-    if (lane == 0 && n) {
-      atomicAdd(&count[k], n);
-      atomicAdd(&split[k], s);
-    }
+    n = wave_sum_i(n);
+    sp = wave_sum_i(sp);
+    const float rounds = ceilf((float)n * (float)a.Hk / (float)slots);
+    float t = fminf(rounds * (float)c, W / (float)slots + (float)c) + rounds * kStart + (sp ? kJoin : 0.f);
+    if (wave > 0 && (n > max_pieces || (int64_t)sp * a.Hk > max_parts)) t = INFINITY;
+    if (lane == 0) cost[wave] = t;
   }
   __syncthreads();
-  if (tid == 0) {
-    int best = most;
-    int64_t least = INT64_MAX;
-    for (int k = 0; k < NC; ++k) {
-      const int64_t N = (int64_t)count[k] * a.Hk, c = chunk_of(k), rounds = (N + slots - 1) / slots;
-      if (k > 0 && (count[k] > max_pieces || (int64_t)split[k] * a.Hk > max_parts)) continue;
-      const int64_t t = min(rounds * c, W / slots + c) + rounds * kStart + (split[k] ? kJoin * rounds : 0);
-      if (t < least) {
-        least = t;
-        best = (int)c;
-      }
-    }
-    choice = best;
-  }
-  __syncthreads();
-  const int c = choice;
-  int N = 0, S = 0;
+  int best = 0;
+  for (int w = 1; w < NW; ++w)
+    if (cost[w] < cost[best]) best = w;
+  const int c = chunk_of(best);
+  int N = 0, S = 0, Q = 0;
   for (int i0 = 0; i0 < R; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int4 pr = i < R ? pairs[i] : make_int4(0, 0, 0, 0);
-    const int np = i < R ? max((pr.z + c - 1) / c, 1) : 0;
-    int x = np, y = np > 1 ? np : 0, all0, all1;
-    scan2(x, y, all0, all1);
+    const int4 pr = i < R ? pairs[i] : make_int4(0, 0, 0, 0);
+    const int np = i < R ? parts(pr.z, c) : 0, sp = np > 1 ? np : 0;
+    int x[3] = {np, sp, sp > 0}, all[3];
+    scan(x, all, 3);
     if (i < R) {
-      const int n0 = N + x - np, s0 = np > 1 ? S + y - np : -1;
-      pairs[i] = make_int4(pr.x, pr.y, np, s0);
-      for (int j = 0; j < np; ++j) pieces[n0 + j] = make_int4(pr.x, pr.y, j * c, np > 1 ? s0 + j : -1);
+      const int n0 = N + x[0] - np, s0 = S + x[1] - sp;
+      if (sp) splits[Q + x[2] - 1] = make_int4(pr.x, pr.y, np, s0);
+      for (int j = 0; j < np; ++j) pieces[n0 + j] = make_int4(pr.x, pr.y, j * c, sp ? s0 + j : -1);
     }
-    N += all0;
-    S += all1;
+    N += all[0];
+    S += all[1];
+    Q += all[2];
   }
   if (tid == 0) {
     head[0] = N;
-    head[1] = R;
+    head[1] = Q;
     head[2] = c;
     head[3] = S;
   }
@@ -858,8 +890,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
 
 // Workspace of a call: head, pairs, pieces, the split pieces' sums.
 struct Work {
-  int max_pairs, max_pieces, max_parts, rows;
-  size_t pairs, pieces, ml, o, bytes;
+  int max_pairs, max_pieces, max_parts, max_splits, rows;
+  size_t pairs, pieces, splits, ml, o, bytes;
 };
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // row tiles of at most `rows` rows of B requests with T tokens in all; few: row tiles of 32
@@ -869,9 +901,11 @@ static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
   w.max_pairs = (int)(T * G / w.rows + B);
   w.max_parts = few ? kPartsFew : kPartsMany;
   w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
+  w.max_splits = std::min(w.max_pairs, std::max(w.max_parts / (2 * Hk), 1));
   w.pairs = 256;
   w.pieces = w.pairs + align256((size_t)w.max_pairs * 16);
-  w.ml = w.pieces + align256((size_t)w.max_pieces * 16);
+  w.splits = w.pieces + align256((size_t)w.max_pieces * 16);
+  w.ml = w.splits + align256((size_t)w.max_splits * 16);
   w.o = w.ml + align256((size_t)w.max_parts * w.rows * 8);
   w.bytes = w.o + (size_t)w.max_parts * w.rows * D * 4;
   return w;
@@ -887,24 +921,27 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
   if (plan) {
     int4* pairs = reinterpret_cast<int4*>(work + w.pairs);
     int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
+    int4* splits = reinterpret_cast<int4*>(work + w.splits);
     int32_t* head = reinterpret_cast<int32_t*>(work);
-    if (few) plan_pieces_kernel<32, 128><<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, head, w.max_pairs, w.max_pieces, w.max_parts, D == 128 ? kSlotsFew : 2 * kSlotsFew);
-    else plan_pieces_kernel<128, 64><<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, head, w.max_pairs, w.max_pieces, w.max_parts, kSlotsMany);
+    auto plan_pieces = few ? plan_pieces_kernel<32, 32 * kFewWaves> : plan_pieces_kernel<128, 64>;
+    plan_pieces<<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, splits, head, w.max_pairs, w.max_pieces, w.max_parts,
+                                           few ? few_slots(D) : kSlotsMany);
     if (int rc = fs_host::launch_status(fn)) return rc;
     k.pieces = pieces;
-    k.pairs = pairs;
+    k.splits = splits;
+    k.max_splits = w.max_splits;
     k.head = head;
     k.part_ml = reinterpret_cast<float*>(work + w.ml);
     k.part_o = reinterpret_cast<float*>(work + w.o);
     grid = (int64_t)w.max_pieces * k.Hk;
   }
-  if (few) few_kernel<T, D, PAGED><<<(unsigned)grid, 256, 0, s>>>(k);
+  if (few) few_kernel<T, D, PAGED, kFewWaves><<<(unsigned)grid, 64 * kFewWaves, 0, s>>>(k);
   else many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    const unsigned parts = (unsigned)((int64_t)w.max_pairs * k.Hk * (w.rows / 32));
-    if (few) combine_kernel<T, D, 32><<<parts, 2 * D, 0, s>>>(k);
-    else combine_kernel<T, D, 128><<<parts, 2 * D, 0, s>>>(k);
+    const unsigned parts = (unsigned)((int64_t)w.max_splits * k.Hk * (w.rows / 32) * (D / 32));
+    if (few) combine_kernel<T, D, 32><<<parts, 256, 0, s>>>(k);
+    else combine_kernel<T, D, 128><<<parts, 256, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;
@@ -1026,6 +1063,6 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   // Every sequence is as long here: whether splitting keys can pay is known.
   const int64_t tiles = ((int64_t)a->Lq * (a->Hq / a->Hk) + w.rows - 1) / w.rows * a->B * a->Hk;
   const int64_t keys = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
-  const bool plan = tiles < (few ? kSlotsFew : kSlotsMany) && keys >= 1024;
+  const bool plan = tiles < (few ? few_slots(a->D) : kSlotsMany) && keys >= 1024;
   return run<false>(k, a->dtype, a->D, few, plan, w, static_cast<char*>(a->work), a->B, a->Lq, (hipStream_t)stream, fn);
 }
