@@ -9,9 +9,9 @@
 // `sinks`; tiles of keys in between are not visited.
 //
 // Pieces.  A row tile's keys are taken in pieces of at most `chunk` key tiles by
-// workgroups of their own where that fills the GPU better (plan_pieces_kernel, from the
+// workgroups of their own where that fills the GPU better (plan_in_wave, from the
 // lengths on the device); the pieces' unnormalised sums are then joined by
-// combine_kernel, in the pieces' order.
+// combine_kernel, in an order of their own.
 //
 // few_kernel (row tiles of at most 32 rows: single tokens) is bound by the cache
 // being read.  Each of its 4 waves streams keys of its own, 32 at a time, through
@@ -41,8 +41,9 @@ namespace fs {
 #endif
 constexpr int kFewWaves = FEW_WAVES;                // of a workgroup of few_kernel
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
-static int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
-constexpr int kPartsFew = 8192 / FEW_WAVES, kPartsMany = 1024;  // split pieces that the workspace holds
+constexpr int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
+constexpr int kLeastTiles = 2;                      // of a workgroup of few_kernel
+constexpr int kPartsMany = 1024;                    // split pieces that the workspace holds
 constexpr int kMaxRequests = 4096;
 constexpr int kPlanThreads = 1024;
 
@@ -61,11 +62,12 @@ struct PagedKArgs {
   int B, T, Hq, Hk, G, Lq, Lk, P, page_size, window, sinks;
   uint32_t page_magic;                          // x / (page_size / 16) = mulhi(x, magic); 0: x
   float scale;
-  // pieces: null = one piece per row tile, the last row tiles of a request first
+  // pieces, the last row tiles of a request first
   const int4* pieces;                           // [N] request, row tile, first key tile, slot (-1: the only piece)
-  const int4* splits;                           // [Q] request, row tile, pieces, first slot
-  const int32_t* head;                          // N, Q, chunk, split pieces (of one KV head)
+  int4* splits;                                 // [Q] request, row tile, pieces, first slot
+  int32_t* head;                                // N, Q, chunk, split pieces (of one KV head); null: nothing is split
   int max_splits;
+  int slots;                                    // workgroups of few_kernel
   int row_tiles;                                // of a request (no list)
   float* part_o;                                // [slot][rows / 32][D / 32][4][64 lanes] 4 floats
   float* part_ml;                               // [slot][rows / 32][2][32]
@@ -85,19 +87,20 @@ struct RowTile {
   int kbeg, kend;            // keys kbeg .. kend - 1 (and the first `sinks`) are seen by some row
   int ns, t0, nt;            // key tiles: 0 .. ns - 1, then t0 ..; nt in all
 };
+struct Lengths {
+  int row0, n, L;
+};
+__device__ __forceinline__ Lengths lengths_of(const PagedKArgs& a, int b) {
+  if (a.table == nullptr) return {0, a.Lq, a.Lk};
+  const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], 0), a.T);
+  return {c0, c1 - c0, min(max(a.lens[b], 0), a.P * a.page_size)};   // c1 < c0: no row (row numbers that fall)
+}
 template <int M, int TK>
-__device__ __forceinline__ RowTile row_tile(const PagedKArgs& a, int b, int rt) {
+__device__ __forceinline__ RowTile row_tile(const PagedKArgs& a, const Lengths& x, int rt) {
   RowTile u;
-  if (a.table != nullptr) {
-    const int c0 = a.cu[b], c1 = a.cu[b + 1];
-    u.row0 = c0;
-    u.n = min(max(c1 - c0, 0), a.T);
-    u.L = min(max(a.lens[b], 0), a.P * a.page_size);
-  } else {
-    u.row0 = 0;
-    u.n = a.Lq;
-    u.L = a.Lk;
-  }
+  u.row0 = x.row0;
+  u.n = x.n;
+  u.L = x.L;
   u.r0 = rt * M;
   u.nrows = min(M, u.n * a.G - u.r0);
   u.p_lo = u.L - u.n + u.r0 / a.G;
@@ -247,9 +250,132 @@ __device__ __forceinline__ uint16_t* out_row(const PagedKArgs& a, const RowTile&
 struct Piece {
   int hk, b, rt, begin, count, slot;
 };
-__device__ __forceinline__ bool find_piece(const PagedKArgs& a, int p, Piece& w) {
-  if (a.pieces != nullptr) {
-    const int N = scalar_load(a.head, 0);
+
+// How long a call takes, in key tiles' time: N pieces of at most c tiles of the W in all, `slots` at a time; a start
+// per round of pieces and, where sums are joined, the joining.
+__device__ __forceinline__ float call_time(float N, float c, float W, float slots, bool joined) {
+  constexpr float kStart = 1.5f, kJoin = 2.0f;
+  const float rounds = ceilf(N / slots);
+  return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined ? kJoin : 0.f);
+}
+// The 16 numbers of key tiles per piece that are tried: an i-th part of the longest row tile's, and what gives about i
+// rounds of pieces (U row tiles, of which each may leave a shorter piece).
+__device__ __forceinline__ int chunk_choice(int i, int longest, float W, float U, float slots) {
+  if (i < 8) return (longest + i) / (i + 1);
+  const float s = slots * (float)(i - 7);
+  return max(1, min(longest, (int)ceilf(W / (s - 0.5f * fminf(U, s)))));
+}
+// ceil(nt / c), at least 1; the division is exact below 2^22
+__device__ __forceinline__ int parts_of(int nt, int c) { return max((int)((float)(nt + c - 1) / (float)c), 1); }
+
+// The piece of this workgroup among n: XCD x, that is workgroups x, x + 8, .., takes a run of consecutive ones,
+// row tiles of one head, whose keys its L2 then serves.  Past the last one: n.
+__device__ __forceinline__ int piece_of(int n) {
+  const int per = (n + 7) / 8, x = blockIdx.x & 7, i = blockIdx.x >> 3;
+  return i < per ? x * per + i : n;
+}
+
+// Inclusive prefix sum over the wave (DPP: no LDS round trips).
+__device__ __forceinline__ int wave_prefix(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // row_shr 1, 2, 4, 8: rows of 16 lanes
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row_bcast 15, 31: the rows below
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+// n / d for n < 2^30 with a quotient below 2^22 (one rounding of the reciprocal and one of the product: off by one at most)
+__device__ __forceinline__ int small_quotient(int n, int d) {
+  int q = (int)((float)n * __builtin_amdgcn_rcpf((float)d));
+  const int r = n - q * d;
+  return r < 0 ? q - 1 : r >= d ? q + 1 : q;
+}
+
+// few_kernel's work: the key tiles of all (KV head, request, row tile), one after another, are W (below 2^30, checked on the
+// host); workgroup w takes the `per` tiles from w per on, so all end together whatever the lengths are, and a row
+// tile's keys are cut where a range ends.  Every wave finds its place by itself, from the lengths: in a first step
+// lane l adds the tiles of a group of requests, in a second one the lanes take one request each of the group that is
+// looked for (one request per lane up to 64: the second step is the first).  It is kept short: a wave takes 4 cycles per
+// instruction and its first copies wait for it.
+template <int M, int TK>
+struct Ranges {
+  struct Request {
+    Lengths x;
+    int rts, nt;                                   // row tiles, and the key tiles that each is given (the most that any has)
+  };
+  const PagedKArgs& a;
+  int lane, group;                                 // requests of a lane
+  Request own;                                     // the lane's (last) one
+  int before;                                      // tiles of the lanes below, for one KV head
+  int W1, W, per;                                  // tiles of a KV head, of all, of a workgroup
+  __device__ __forceinline__ Request request(int b) const {
+    Request r{{0, 0, 0}, 0, 0};
+    if (b >= a.B) return r;
+    r.x = lengths_of(a, b);
+    r.rts = r.x.n > 0 ? (r.x.n * a.G + M - 1) / M : r.x.n;
+    const int all = (max(r.x.L, 1) + TK - 1) / TK;
+    r.nt = all;                                    // its last row's keys; a row tile that sees none is written too
+    if (a.window) {
+      if (r.rts <= 1) r.nt = max(row_tile<M, TK>(a, r.x, 0).nt, 1);
+      else r.nt = min(all, (a.sinks + TK - 1) / TK + (a.window + (M + a.G - 2) / a.G + TK - 2) / TK + 1);
+    }
+    return r;
+  }
+  // groups: a power of two
+  __device__ __forceinline__ Ranges(const PagedKArgs& args, int groups) : a(args) {
+    lane = lane_id();
+    group = (a.B + 63) >> 6;
+    int tiles = 0;
+    bool falls = false;
+    for (int k = 0; k < group; ++k) {
+      own = request(lane * group + k);
+      falls |= own.rts < 0;
+      tiles += own.rts * own.nt;
+    }
+    if (__ballot(falls) != 0) tiles = 0;           // row numbers that fall: no row is written
+    const int upto = wave_prefix(tiles);
+    before = upto - tiles;
+    W1 = __builtin_amdgcn_readlane(upto, 63);
+    W = W1 * a.Hk;
+    const int sh = 31 - __builtin_clz(groups);
+    per = max((W + groups - 1) >> sh, kLeastTiles);
+  }
+  // The row tile that tile `pos` (< W) of all belongs to: its first tile's place `start`, its key tiles nt.
+  struct Place {
+    Lengths x;
+    int hk, b, rt, nt, start;
+  };
+  __device__ __forceinline__ Place find(int pos) const {
+    Place w;
+    w.hk = __builtin_amdgcn_readfirstlane(small_quotient(pos, W1));
+    const int i = pos - w.hk * W1;
+    Request r = own;
+    int l = __popcll(__ballot(before <= i)) - 1, at = before;   // the last lane of those at the same place: it holds tiles
+    w.b = l * group;
+    if (group > 1) {                               // group <= 64
+      const int base = __builtin_amdgcn_readlane(before, l);
+      r = request(lane < group ? w.b + lane : a.B);
+      const int tiles = r.rts * r.nt;
+      at = base + wave_prefix(tiles) - tiles;
+      l = (int)__builtin_ctzll(__ballot(at <= i && at + tiles > i));
+      w.b += l;
+    }
+    w.nt = __builtin_amdgcn_readlane(r.nt, l);
+    w.x.row0 = __builtin_amdgcn_readlane(r.x.row0, l);
+    w.x.n = __builtin_amdgcn_readlane(r.x.n, l);
+    w.x.L = __builtin_amdgcn_readlane(r.x.L, l);
+    const int rts = __builtin_amdgcn_readlane(r.rts, l), from = w.hk * W1 + __builtin_amdgcn_readlane(at, l);
+    const int x = rts > 1 ? (pos - from) / w.nt : 0;
+    w.rt = rts - 1 - x;
+    w.start = from + x * w.nt;
+    return w;
+  }
+};
+
+__device__ __forceinline__ bool find_piece(const PagedKArgs& a, Piece& w) {
+  if (a.pieces != nullptr) {                       // plan_pieces_kernel's list
+    const int N = scalar_load(a.head, 0), p = piece_of(N * a.Hk);
     if (p >= N * a.Hk) return false;
     w.hk = p / N;
     const int32_t* e = reinterpret_cast<const int32_t*>(a.pieces + (p - w.hk * N));
@@ -259,17 +385,17 @@ __device__ __forceinline__ bool find_piece(const PagedKArgs& a, int p, Piece& w)
     w.slot = scalar_load(e, 3);
     w.count = scalar_load(a.head, 2);
     if (w.slot >= 0) w.slot += w.hk * scalar_load(a.head, 3);
-  } else {
-    const int R = a.B * a.row_tiles;
-    if (p >= R * a.Hk) return false;
-    w.hk = p / R;
-    const int i = p - w.hk * R;
-    w.b = i / a.row_tiles;
-    w.rt = a.row_tiles - 1 - (i - w.b * a.row_tiles);
-    w.begin = 0;
-    w.slot = -1;
-    w.count = INT_MAX;
+    return true;
   }
+  const int R = a.B * a.row_tiles, p = piece_of(R * a.Hk);   // one piece per row tile
+  if (p >= R * a.Hk) return false;
+  w.hk = p / R;
+  const int i = p - w.hk * R;
+  w.b = i / a.row_tiles;
+  w.rt = a.row_tiles - 1 - (i - w.b * a.row_tiles);
+  w.begin = 0;
+  w.slot = -1;
+  w.count = INT_MAX;
   return true;
 }
 
@@ -288,255 +414,312 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
   constexpr int RING = 4 * TILE;                   // of a wave: two K tiles, two V tiles
   constexpr int NI = 2 * Copy::NI;                 // copies of 32 keys
   __shared__ __attribute__((aligned(1024))) char lds[NW * RING];
-  Piece pc;
-  if (!find_piece(a, blockIdx.x, pc)) return;
-  const RowTile u = row_tile<32, 32 * NW>(a, pc.b, pc.rt);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const LaneRow me = lane_row(a, u, l32);
   char* ring = lds + wave * RING;
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
-  const Copy cp(a, pc.hk, lane);
-  V8 qf[D / 16];
-  load_q<V8, D>(a, u, me, pc.b, pc.hk, hi, qf);
+  const Ranges<32, 32 * NW> ranges(a, gridDim.x);
+  const int first = blockIdx.x * ranges.per, end = min(first + ranges.per, ranges.W);
+  for (int pos = first; pos < end;) {
+    const auto at = ranges.find(pos);
+    const int begin = pos - at.start, count = min(at.start + at.nt, end) - pos;
+    // where the sums of a part go: a range's first piece or, not starting with it, its last
+    const int slot = count == at.nt ? -1 : 2 * blockIdx.x + (pos != first);
+    pos += count;
+    const RowTile u = row_tile<32, 32 * NW>(a, at.x, at.rt);
+    const LaneRow me = lane_row(a, u, l32);
+    const Copy cp(a, at.hk, lane);
+    V8 qf[D / 16];
+    load_q<V8, D>(a, u, me, at.b, at.hk, hi, qf);
 
-  // this wave's 32 keys of each of the piece's tiles
-  auto key_of = [&](int i) {
-    const int o = pc.begin + i;
-    return (o < u.ns ? o : u.t0 + o - u.ns) * (32 * NW) + 32 * wave;
-  };
-  int cnt = min(pc.count, u.nt - pc.begin);
-  if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
-  struct Ent {
-    int e[2];
-  };
-  auto load_ent = [&](int i) {
-    Ent x{{-1, -1}};
-    if (i < cnt) {
-      const int k = key_of(i);
-      x.e[0] = Copy::entry(a, u, pc.b, k);
-      x.e[1] = Copy::entry(a, u, pc.b, k + 16);
-    }
-    return x;
-  };
-  auto issue_k = [&](int i, const Ent& x) {
-    const uint32_t at = ring0 + (i & 1) * TILE;
-    cp.template issue<false>(a, u, at, x.e[0], key_of(i));
-    cp.template issue<false>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
-  };
-  auto issue_v = [&](int i, const Ent& x) {
-    const uint32_t at = ring0 + (2 + (i & 1)) * TILE;
-    cp.template issue<true>(a, u, at, x.e[0], key_of(i));
-    cp.template issue<true>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
-  };
-  constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
-  const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
-  const int vrow = hi * 4 + ((lane & 15) >> 2);
-  const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
-                                     (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
-  const float sc = a.scale * kLog2e;
-  float m_run = -INFINITY, l_run = 0.f;
-  f32x16_t o[D / 32];
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-
-  // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this
-  // order; K(i+2) and V(i+2) are requested as soon as their place is read.
-  Ent x0 = load_ent(0), x1 = load_ent(1), x2 = load_ent(2);
-  if (cnt > 0) {
-    issue_k(0, x0);
-    issue_v(0, x0);
-  }
-  if (cnt > 1) {
-    issue_k(1, x1);
-    issue_v(1, x1);
-  }
-  __builtin_amdgcn_s_waitcnt(0);                   // Q's loads too: the loop's waits then count copies only
-  for (int i = 0; i < cnt; ++i) {
-    if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
-    const char* kt = ring + (i & 1) * TILE;
-    f32x16_t s;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-#pragma unroll
-    for (int st = 0; st < D / 16; ++st) s = Ops::mma(__builtin_bit_cast(V8, lds16(kt, k_lane ^ (uint32_t)(st << 5))), qf[st], s);
-    const Ent x3 = load_ent(i + 3);
-    if (i + 2 < cnt) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue_k(i + 2, x2);
-    }
-    const int key0 = key_of(i);
-    if (x0.e[0] < 0 || x0.e[1] < 0 || needs_mask(a, u.p_lo, u.p_hi, key0, 32))
-      mask_keys(a, u, s, me.p, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
-    float mx = s[0], h0, h1;
-#pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    lane_halves(mx, h0, h1);
-    mx = fmaxf(h0, h1) * sc;
-    const bool up = mx > m_run + kSlack;
-    const float al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
-    m_run = up ? mx : m_run;
-    const float mu = (m_run == -INFINITY ? 0.f : m_run) - kBias<T>;
-    V8 pb[2];
-    float rs = 0.f;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      float pv[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) pv[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * kk + j], sc, -mu));
-      pb[kk] = Ops::pack(pv);
-      rs = Ops::sum8(pb[kk], rs);
-    }
-    lane_halves(rs, h0, h1);
-    l_run = l_run * al + (h0 + h1);
-    if (__builtin_amdgcn_ballot_w64(al != 1.0f) != 0) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= al;
-    }
-    if (i + 2 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
-    else if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const char* vt = ring + (2 + (i & 1)) * TILE;
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt) {
-        const uint32_t lo = (v_lane ^ (uint32_t)(dt << 6)) + kk * 16 * ROWB;
-        o[dt] = Ops::mma(__builtin_bit_cast(V8, join8(lds_tr8(vt, lo), lds_tr8(vt, lo + 8 * ROWB))), pb[kk], o[dt]);
+    // this wave's 32 keys of each of the piece's tiles
+    auto key_of = [&](int i) {
+      const int o = begin + i;
+      return (o < u.ns ? o : u.t0 + o - u.ns) * (32 * NW) + 32 * wave;
+    };
+    int cnt = min(count, u.nt - begin);
+    if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
+    struct Ent {
+      int e[2];
+    };
+    auto load_ent = [&](int i) {
+      Ent x{{-1, -1}};
+      if (i < cnt) {
+        const int k = key_of(i);
+        x.e[0] = Copy::entry(a, u, at.b, k);
+        x.e[1] = Copy::entry(a, u, at.b, k + 16);
       }
-    if (i + 2 < cnt) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      issue_v(i + 2, x2);
+      return x;
+    };
+    auto issue_k = [&](int i, const Ent& x) {
+      const uint32_t at = ring0 + (i & 1) * TILE;
+      cp.template issue<false>(a, u, at, x.e[0], key_of(i));
+      cp.template issue<false>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+    };
+    auto issue_v = [&](int i, const Ent& x) {
+      const uint32_t at = ring0 + (2 + (i & 1)) * TILE;
+      cp.template issue<true>(a, u, at, x.e[0], key_of(i));
+      cp.template issue<true>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+    };
+    constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
+    const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
+    const int vrow = hi * 4 + ((lane & 15) >> 2);
+    const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
+                                       (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
+    const float sc = a.scale * kLog2e;
+    float m_run = -INFINITY, l_run = 0.f;
+    f32x16_t o[D / 32];
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+
+    // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this
+    // order; K(i+2) and V(i+2) are requested as soon as their place is read.
+    Ent x0 = load_ent(0), x1 = load_ent(1), x2 = load_ent(2);
+    if (cnt > 0) {
+      issue_k(0, x0);
+      issue_v(0, x0);
     }
-    x0 = x1;
-    x1 = x2;
-    x2 = x3;
-  }
-  // ---- the waves' sums joined through LDS, wave w taking dims 32 w, 32 (w + NW) ..
-  constexpr int NV = D / 32;
-  float* own = reinterpret_cast<float*>(ring);     // [D / 32][4][64 lanes] 4 floats, then m and l
+    if (cnt > 1) {
+      issue_k(1, x1);
+      issue_v(1, x1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);                   // Q's loads too: the loop's waits then count copies only
+    for (int i = 0; i < cnt; ++i) {
+      if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+      const char* kt = ring + (i & 1) * TILE;
+      f32x16_t s;
 #pragma unroll
-  for (int dt = 0; dt < NV; ++dt)
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4)
-      reinterpret_cast<float4*>(own)[(dt * 4 + g4) * 64 + lane] =
-          make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
-  constexpr int ML = NV * 4 * 64 * 4;
-  own[ML + lane] = m_run;
-  own[ML + 64 + lane] = l_run;
-  __syncthreads();
-  if (!me.on) return;
-  float m = -INFINITY, l = 0.f, f[NW];
+      for (int st = 0; st < D / 16; ++st) s = Ops::mma(__builtin_bit_cast(V8, lds16(kt, k_lane ^ (uint32_t)(st << 5))), qf[st], s);
+      const Ent x3 = load_ent(i + 3);
+      if (i + 2 < cnt) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue_k(i + 2, x2);
+      }
+      const int key0 = key_of(i);
+      if (x0.e[0] < 0 || x0.e[1] < 0 || needs_mask(a, u.p_lo, u.p_hi, key0, 32))
+        mask_keys(a, u, s, me.p, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+      float mx = s[0], h0, h1;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
-  const float mu = m == -INFINITY ? 0.f : m;
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      lane_halves(mx, h0, h1);
+      mx = fmaxf(h0, h1) * sc;
+      const bool up = mx > m_run + kSlack;
+      const float al = up ? __builtin_amdgcn_exp2f(m_run - mx) : 1.0f;
+      m_run = up ? mx : m_run;
+      const float mu = (m_run == -INFINITY ? 0.f : m_run) - kBias<T>;
+      V8 pb[2];
+      float rs = 0.f;
 #pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const float* x = reinterpret_cast<const float*>(lds + w * RING) + ML;
-    f[w] = __builtin_amdgcn_exp2f(x[lane] - mu);
-    l += x[64 + lane] * f[w];
-  }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
-  uint16_t* op = out_row(a, u, me, pc.b, pc.hk);
+      for (int kk = 0; kk < 2; ++kk) {
+        float pv[8];
 #pragma unroll
-  for (int dt = wave; dt < NV; dt += NW)
+        for (int j = 0; j < 8; ++j) pv[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * kk + j], sc, -mu));
+        pb[kk] = Ops::pack(pv);
+        rs = Ops::sum8(pb[kk], rs);
+      }
+      lane_halves(rs, h0, h1);
+      l_run = l_run * al + (h0 + h1);
+      if (__builtin_amdgcn_ballot_w64(al != 1.0f) != 0) {
 #pragma unroll
-    for (int g4 = 0; g4 < 4; ++g4) {
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[dt][r] *= al;
+      }
+      if (i + 2 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
+      else if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const char* vt = ring + (2 + (i & 1)) * TILE;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+          const uint32_t lo = (v_lane ^ (uint32_t)(dt << 6)) + kk * 16 * ROWB;
+          o[dt] = Ops::mma(__builtin_bit_cast(V8, join8(lds_tr8(vt, lo), lds_tr8(vt, lo + 8 * ROWB))), pb[kk], o[dt]);
+        }
+      if (i + 2 < cnt) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        issue_v(i + 2, x2);
+      }
+      x0 = x1;
+      x1 = x2;
+      x2 = x3;
+    }
+    // ---- the waves' sums joined through LDS, wave w taking dims 32 w, 32 (w + NW) ..
+    constexpr int NV = D / 32;
+    float* own = reinterpret_cast<float*>(ring);     // [D / 32][4][64 lanes] 4 floats, then m and l
+#pragma unroll
+    for (int dt = 0; dt < NV; ++dt)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4)
+        reinterpret_cast<float4*>(own)[(dt * 4 + g4) * 64 + lane] =
+            make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+    constexpr int ML = NV * 4 * 64 * 4;
+    own[ML + lane] = m_run;
+    own[ML + 64 + lane] = l_run;
+    __syncthreads();
+    if (me.on) {
+      float m = -INFINITY, l = 0.f, f[NW];
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
+      const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(dt * 4 + g4) * 64 + lane];
-        acc.x += x.x * f[w];
-        acc.y += x.y * f[w];
-        acc.z += x.z * f[w];
-        acc.w += x.w * f[w];
+        const float* x = reinterpret_cast<const float*>(lds + w * RING) + ML;
+        f[w] = __builtin_amdgcn_exp2f(x[lane] - mu);
+        l += x[64 + lane] * f[w];
       }
-      if (pc.slot < 0) store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      else reinterpret_cast<float4*>(a.part_o)[(((int64_t)pc.slot * NV + dt) * 4 + g4) * 64 + lane] = acc;
+      const float inv = l != 0.f ? 1.0f / l : 0.f;
+      uint16_t* op = out_row(a, u, me, at.b, at.hk);
+#pragma unroll
+      for (int dt = wave; dt < NV; dt += NW)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(dt * 4 + g4) * 64 + lane];
+            acc.x += x.x * f[w];
+            acc.y += x.y * f[w];
+            acc.z += x.z * f[w];
+            acc.w += x.w * f[w];
+          }
+          if (slot < 0) store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+          else reinterpret_cast<float4*>(a.part_o)[(((int64_t)slot * NV + dt) * 4 + g4) * 64 + lane] = acc;
+        }
+      if (slot >= 0 && wave == 0 && hi == 0) {
+        a.part_ml[(int64_t)slot * 64 + l32] = m;
+        a.part_ml[(int64_t)slot * 64 + 32 + l32] = l;
+      }
     }
-  if (pc.slot >= 0 && wave == 0 && hi == 0) {
-    a.part_ml[(int64_t)pc.slot * 64 + l32] = m;
-    a.part_ml[(int64_t)pc.slot * 64 + 32 + l32] = l;
+    __syncthreads();                               // the rings are read: the next row tile's copies may come
   }
 }
 
-// The pieces' sums joined: 32 rows and 32 dims of a split row tile per workgroup.  A thread adds 4 dims of one
-// row over every J-th piece (J as many threads as 256 give an item), then the J sums are added in LDS; always in
-// the same order.
+// The pieces' sums joined: 32 rows of a split row tile per workgroup.  A thread adds 4 dims of one row over every J-th
+// piece (J as many threads as there are for an item), then the J sums are added in LDS; always in the same
+// order.  Wave 0 looks up what the workgroup joins (mostly nothing).
+constexpr int kJoinThreads = 512;
 template <typename T, int D, int M>
-__global__ __launch_bounds__(256) void combine_kernel(PagedKArgs a) {
-  constexpr int NV = D / 32, QW = M / 32, AHEAD = 4;
-  __shared__ float4 part[256];
-  __shared__ float2 ml[256];
-  int w = blockIdx.x;
-  const int dt = w % NV;
-  w /= NV;
-  const int qq = w % QW;
-  w /= QW;
-  const int Q = scalar_load(a.head, 1), hk = w / a.max_splits, i = w - hk * a.max_splits;
-  if (i >= Q) return;
-  const int32_t* e = reinterpret_cast<const int32_t*>(a.splits + i);
-  const int b = scalar_load(e, 0), rt = scalar_load(e, 1), np = scalar_load(e, 2);
-  const int64_t s0 = (int64_t)(scalar_load(e, 3) + hk * scalar_load(a.head, 3)) * QW + qq;
-  const RowTile u = row_tile<M, 64>(a, b, rt);
+__global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
+  constexpr int QW = M / 32, AHEAD = 8;
+  constexpr bool FEW = M == 32;
+  __shared__ float4 part[kJoinThreads];
+  __shared__ float2 ml[kJoinThreads];
+  __shared__ int job[10];                          // pieces, first slot, second slot, KV head, request, row tile, lengths
+  const int tid = threadIdx.x, qq = blockIdx.x % QW, w = blockIdx.x / QW;
+  if (tid < 64) {
+    int np = 0;
+    if constexpr (FEW) {
+      // the row tile that the end of range w cuts, if it is the first that does
+      const Ranges<M, 32 * kFewWaves> ranges(a, a.slots);
+      const int cut = (w + 1) * ranges.per;
+      if (cut < ranges.W) {
+        const auto at = ranges.find(cut);
+        if (at.start < cut && at.start >= w * ranges.per) {
+          np = small_quotient(at.start + at.nt - 1, ranges.per) - w + 1;
+          if (tid == 0) {
+            job[1] = 2 * w + (at.start != w * ranges.per);
+            job[2] = 2 * (w + 1);                  // the others are their ranges' first pieces
+            job[3] = at.hk;
+            job[4] = at.b;
+            job[5] = at.rt;
+            job[6] = at.x.row0;
+            job[7] = at.x.n;
+            job[8] = at.x.L;
+          }
+        }
+      }
+    } else {
+      const int Q = scalar_load(a.head, 1), hk = w / a.max_splits, i = w - hk * a.max_splits;
+      if (i < Q) {
+        const int32_t* e = reinterpret_cast<const int32_t*>(a.splits + i);
+        const int b = scalar_load(e, 0);
+        const Lengths x = lengths_of(a, b);
+        np = scalar_load(e, 2);
+        if (tid == 0) {
+          job[1] = (scalar_load(e, 3) + hk * scalar_load(a.head, 3)) * QW + qq;
+          job[2] = job[1] + QW;
+          job[3] = hk;
+          job[4] = b;
+          job[5] = scalar_load(e, 1);
+          job[6] = x.row0;
+          job[7] = x.n;
+          job[8] = x.L;
+        }
+      }
+    }
+    if (tid == 0) job[0] = np;
+  }
+  __syncthreads();
+  const int np = __builtin_amdgcn_readfirstlane(job[0]);
+  if (np == 0) return;
+  const int s0 = __builtin_amdgcn_readfirstlane(job[1]), s1 = __builtin_amdgcn_readfirstlane(job[2]);
+  const int hk = __builtin_amdgcn_readfirstlane(job[3]), b = __builtin_amdgcn_readfirstlane(job[4]);
+  const Lengths x = {__builtin_amdgcn_readfirstlane(job[6]), __builtin_amdgcn_readfirstlane(job[7]),
+                     __builtin_amdgcn_readfirstlane(job[8])};
+  const RowTile u = row_tile<M, 64>(a, x, __builtin_amdgcn_readfirstlane(job[5]));
   const int rows = min(u.nrows - qq * 32, 32);
   if (rows <= 0) return;
-  const int items = rows * 8, J = 256 / items;     // an item: row, half, quarter of 32 dims
-  const int tid = threadIdx.x, jg = tid / items, it = tid - jg * items;
-  const int r = it % rows, hi = (it / rows) & 1, g4 = it / rows >> 1;
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (jg < J)
-    for (int j0 = jg; j0 < np; j0 += AHEAD * J) {
-      float mj[AHEAD], lj[AHEAD];
-      float4 xj[AHEAD];
+  const int items = rows * (D / 4);                // an item: row, and 4 dims: 32 dt + 8 g4 + 4 hi ..
+  const int J = max(kJoinThreads / items, 1);
+  auto slot_of = [&](int j) { return (int64_t)(j == 0 ? s0 : s1 + (j - 1) * (FEW ? 2 : QW)); };
+  for (int i0 = 0; i0 < items; i0 += kJoinThreads) {
+    const int jg = items < kJoinThreads ? tid / items : 0, it = items < kJoinThreads ? tid - jg * items : i0 + tid;
+    const int c = it / rows, r = it - c * rows;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (jg < J && it < items)
+      for (int j0 = jg; j0 < np; j0 += AHEAD * J) {
+        float mj[AHEAD], lj[AHEAD];
+        float4 xj[AHEAD];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int64_t s = s0 + (int64_t)min(j0 + k * J, np - 1) * QW;
-        mj[k] = a.part_ml[s * 64 + r];
-        lj[k] = a.part_ml[s * 64 + 32 + r];
-        xj[k] = reinterpret_cast<const float4*>(a.part_o)[((s * NV + dt) * 4 + g4) * 64 + hi * 32 + r];
+        for (int k = 0; k < AHEAD; ++k) {
+          const int64_t s = slot_of(min(j0 + k * J, np - 1));
+          mj[k] = a.part_ml[s * 64 + r];
+          lj[k] = a.part_ml[s * 64 + 32 + r];
+          xj[k] = reinterpret_cast<const float4*>(a.part_o)[(s * (D / 8) + (c >> 1)) * 64 + (c & 1) * 32 + r];
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          if (j0 + k * J >= np) break;
+          const float mn = fmaxf(m, mj[k]), mu = mn == -INFINITY ? 0.f : mn;
+          const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(mj[k] - mu);
+          m = mn;
+          l = l * f0 + lj[k] * f1;
+          acc.x = acc.x * f0 + xj[k].x * f1;
+          acc.y = acc.y * f0 + xj[k].y * f1;
+          acc.z = acc.z * f0 + xj[k].z * f1;
+          acc.w = acc.w * f0 + xj[k].w * f1;
+        }
       }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (j0 + k * J >= np) break;
-        const float mn = fmaxf(m, mj[k]), mu = mn == -INFINITY ? 0.f : mn;
-        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(mj[k] - mu);
+    if (J > 1) {                                   // all items at once
+      part[tid] = acc;
+      ml[tid] = make_float2(m, l);
+      __syncthreads();
+      for (int k = 1; jg == 0 && k < J; ++k) {
+        const float2 o = ml[k * items + it];
+        const float4 y = part[k * items + it];
+        const float mn = fmaxf(m, o.x), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(o.x - mu);
         m = mn;
-        l = l * f0 + lj[k] * f1;
-        acc.x = acc.x * f0 + xj[k].x * f1;
-        acc.y = acc.y * f0 + xj[k].y * f1;
-        acc.z = acc.z * f0 + xj[k].z * f1;
-        acc.w = acc.w * f0 + xj[k].w * f1;
+        l = l * f0 + o.y * f1;
+        acc.x = acc.x * f0 + y.x * f1;
+        acc.y = acc.y * f0 + y.y * f1;
+        acc.z = acc.z * f0 + y.z * f1;
+        acc.w = acc.w * f0 + y.w * f1;
       }
     }
-  if (J > 1) {
-    part[tid] = acc;
-    ml[tid] = make_float2(m, l);
-    __syncthreads();
-    if (jg > 0) return;
-    for (int k = 1; k < J; ++k) {
-      const float2 o = ml[k * items + it];
-      const float4 x = part[k * items + it];
-      const float mn = fmaxf(m, o.x), mu = mn == -INFINITY ? 0.f : mn;
-      const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(o.x - mu);
-      m = mn;
-      l = l * f0 + o.y * f1;
-      acc.x = acc.x * f0 + x.x * f1;
-      acc.y = acc.y * f0 + x.y * f1;
-      acc.z = acc.z * f0 + x.z * f1;
-      acc.w = acc.w * f0 + x.w * f1;
-    }
+    const LaneRow me = lane_row(a, u, qq * 32 + r);
+    if (jg > 0 || it >= items || !me.on) continue;
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    store_out<T>(out_row(a, u, me, b, hk), (c >> 3) * 32 + ((c >> 1) & 3) * 8 + (c & 1) * 4, acc.x * inv, acc.y * inv,
+                 acc.z * inv, acc.w * inv);
   }
-  const LaneRow me = lane_row(a, u, qq * 32 + r);
-  if (jg > 0 || !me.on) return;
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
-  store_out<T>(out_row(a, u, me, b, hk), dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 template <typename T, int D, bool PAGED>
@@ -548,13 +731,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM, GB = 16 * ROWB;
   __shared__ __attribute__((aligned(1024))) char lds[2][2][TILE];   // [K, V][buffer]
   Piece pc;
-  {
-    // XCD x (workgroups x, x + 8, ..) takes a run of consecutive pieces: row tiles of one head, whose keys its L2 then serves
-    const int total = (a.pieces != nullptr ? scalar_load(a.head, 0) : a.B * a.row_tiles) * a.Hk, per = (total + 7) / 8;
-    const int p = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || !find_piece(a, p, pc)) return;
-  }
-  const RowTile u = row_tile<128, TK>(a, pc.b, pc.rt);
+  if (!find_piece(a, pc)) return;
+  const RowTile u = row_tile<128, TK>(a, lengths_of(a, pc.b), pc.rt);
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const LaneRow me = lane_row(a, u, wave * 32 + l32);
@@ -755,19 +933,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                    o[dt][4 * g4 + 3] * inv);
 }
 
-// The pieces of one call, for one KV head (all have the same): row tiles of every request, and the
-// number of key tiles per piece that ends soonest.  With W key tiles in all, N pieces of at most c
-// and S workgroups at a time, a call takes about min(ceil(N / S) c, W / S + c) tiles' time, a start per
-// round of pieces and, where sums are joined, the joining.  16 choices of c are tried, one by each wave: the
-// longest row tile's i-th part, and the c that gives about i rounds.
-// One workgroup; its lists are read by the attention and the joining kernel.
+// many_kernel's pieces of one KV head (all have the same), as a list.  The 16 choices of key tiles per piece are tried by a wave
+// each.  One workgroup; its lists are read by the attention and the joining kernel.
 template <int M, int TK>
 __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a, int4* pieces, int4* pairs, int4* splits,
                                                                    int32_t* head, int max_pairs, int max_pieces,
                                                                    int max_parts, int slots) {
   constexpr int NW = kPlanThreads / 64;
   constexpr int kHeld = 8192;                      // row tiles whose key tiles are kept in LDS
-  constexpr float kStart = 1.5f, kJoin = 2.0f;     // in tiles' time
   __shared__ int base[kMaxRequests + 1], tiles[kHeld];
   __shared__ int wsum[3][NW];
   __shared__ float wtot[NW], cost[NW];
@@ -798,7 +971,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
     int n = 0;
-    if (b < a.B) n = a.table != nullptr ? min(max(a.cu[b + 1] - a.cu[b], 0), a.T) : a.Lq;
+    if (b < a.B) n = max(lengths_of(a, b).n, 0);
     n = min((int)(((int64_t)n * a.G + M - 1) / M), max_pairs);
     int x[3] = {n, 0, 0}, all[3];
     scan(x, all, 1);
@@ -817,7 +990,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
       else hi = m;
     }
     const int rt = base[lo + 1] - 1 - i;           // the last row tiles, whose keys are the most, first
-    const int nt = row_tile<M, TK>(a, lo, rt).nt;
+    const int nt = row_tile<M, TK>(a, lengths_of(a, lo), rt).nt;
     pairs[i] = make_int4(lo, rt, nt, 0);
     if (i < kHeld) tiles[i] = nt;
     total += (float)nt;
@@ -836,24 +1009,18 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
     longest = max(longest, wsum[0][w]);
   }
   const float W = total * (float)a.Hk;
-  auto chunk_of = [&](int i) {
-    if (i < 8) return (longest + i) / (i + 1);
-    const float s = (float)slots * (float)(i - 7);
-    return max(1, min(longest, (int)ceilf(W / (s - 0.5f * fminf((float)R * (float)a.Hk, s)))));
-  };
-  auto parts = [](int nt, int c) { return max((int)((float)(nt + c - 1) / (float)c), 1); };   // exact below 2^22
+  auto chunk_of = [&](int i) { return chunk_choice(i, longest, W, (float)R * (float)a.Hk, (float)slots); };
   {
     const int c = chunk_of(wave);
     int n = 0, sp = 0;
     for (int i = lane; i < R; i += 64) {
-      const int np = parts(i < kHeld ? tiles[i] : pairs[i].z, c);
+      const int np = parts_of(i < kHeld ? tiles[i] : pairs[i].z, c);
       n += np;
       sp += np > 1 ? np : 0;
     }
     n = wave_sum_i(n);
     sp = wave_sum_i(sp);
-    const float rounds = ceilf((float)n * (float)a.Hk / (float)slots);
-    float t = fminf(rounds * (float)c, W / (float)slots + (float)c) + rounds * kStart + (sp ? kJoin : 0.f);
+    float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, sp > 0);
     if (wave > 0 && (n > max_pieces || (int64_t)sp * a.Hk > max_parts)) t = INFINITY;
     if (lane == 0) cost[wave] = t;
   }
@@ -866,7 +1033,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
   for (int i0 = 0; i0 < R; i0 += kPlanThreads) {
     const int i = i0 + tid;
     const int4 pr = i < R ? pairs[i] : make_int4(0, 0, 0, 0);
-    const int np = i < R ? parts(pr.z, c) : 0, sp = np > 1 ? np : 0;
+    const int np = i < R ? parts_of(pr.z, c) : 0, sp = np > 1 ? np : 0;
     int x[3] = {np, sp, sp > 0}, all[3];
     scan(x, all, 3);
     if (i < R) {
@@ -899,7 +1066,7 @@ static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
   Work w;
   w.rows = few ? 32 : 128;
   w.max_pairs = (int)(T * G / w.rows + B);
-  w.max_parts = few ? kPartsFew : kPartsMany;
+  w.max_parts = few ? 2 * few_slots(D) : kPartsMany;
   w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
   w.max_splits = std::min(w.max_pairs, std::max(w.max_parts / (2 * Hk), 1));
   w.pairs = 256;
@@ -910,38 +1077,43 @@ static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
   w.bytes = w.o + (size_t)w.max_parts * w.rows * D * 4;
   return w;
 }
-// Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.
-static bool few_rows(int64_t max_new, int G) { return max_new * G <= 32; }
+// Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.  few_kernel counts key tiles of
+// row tiles in 32 bits.
+static bool few_rows(int64_t max_new, int G, int64_t T, int B, int Hk, int64_t keys) {
+  return max_new * G <= 32 && (T * G / 32 + B) * Hk < (1ll << 30) / (keys / 32 + 2);
+}
 
 template <typename T, int D, bool PAGED>
 static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, int B, int Lq, hipStream_t s, const char* fn) {
   const int64_t rows = (int64_t)Lq * k.G;
   k.row_tiles = (int)((rows + w.rows - 1) / w.rows);
   int64_t grid = (int64_t)B * k.row_tiles * k.Hk;
-  if (plan) {
-    int4* pairs = reinterpret_cast<int4*>(work + w.pairs);
-    int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
-    int4* splits = reinterpret_cast<int4*>(work + w.splits);
-    int32_t* head = reinterpret_cast<int32_t*>(work);
-    auto plan_pieces = few ? plan_pieces_kernel<32, 32 * kFewWaves> : plan_pieces_kernel<128, 64>;
-    plan_pieces<<<1, kPlanThreads, 0, s>>>(k, pieces, pairs, splits, head, w.max_pairs, w.max_pieces, w.max_parts,
-                                           few ? few_slots(D) : kSlotsMany);
-    if (int rc = fs_host::launch_status(fn)) return rc;
-    k.pieces = pieces;
-    k.splits = splits;
-    k.max_splits = w.max_splits;
-    k.head = head;
+  if (few || plan) {
     k.part_ml = reinterpret_cast<float*>(work + w.ml);
     k.part_o = reinterpret_cast<float*>(work + w.o);
-    grid = (int64_t)w.max_pieces * k.Hk;
   }
-  if (few) few_kernel<T, D, PAGED, kFewWaves><<<(unsigned)grid, 64 * kFewWaves, 0, s>>>(k);
-  else many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
+  if (few) {
+    k.slots = few_slots(D);
+    few_kernel<T, D, PAGED, kFewWaves><<<k.slots, 64 * kFewWaves, 0, s>>>(k);
+    if (int rc = fs_host::launch_status(fn)) return rc;
+    combine_kernel<T, D, 32><<<k.slots - 1, kJoinThreads, 0, s>>>(k);
+    return fs_host::launch_status(fn);
+  }
+  if (plan) {
+    int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
+    k.splits = reinterpret_cast<int4*>(work + w.splits);
+    k.head = reinterpret_cast<int32_t*>(work);
+    k.max_splits = w.max_splits;
+    grid = (int64_t)w.max_pieces * k.Hk;
+    plan_pieces_kernel<128, 64><<<1, kPlanThreads, 0, s>>>(k, pieces, reinterpret_cast<int4*>(work + w.pairs), k.splits,
+                                                           k.head, w.max_pairs, w.max_pieces, w.max_parts, kSlotsMany);
+    if (int rc = fs_host::launch_status(fn)) return rc;
+    k.pieces = pieces;
+  }
+  many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    const unsigned parts = (unsigned)((int64_t)w.max_splits * k.Hk * (w.rows / 32) * (D / 32));
-    if (few) combine_kernel<T, D, 32><<<parts, 256, 0, s>>>(k);
-    else combine_kernel<T, D, 128><<<parts, 256, 0, s>>>(k);
+    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4), kJoinThreads, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;
@@ -983,11 +1155,15 @@ static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int B,
 
 // the most new tokens of one request
 static int64_t most_new(const fs_paged_attn_args& a) { return a.max_new > 0 && a.max_new < a.T ? a.max_new : a.T; }
-static Work work_of(const fs_paged_attn_args& a) {
-  return work_of(few_rows(most_new(a), a.Hq / a.Hk), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D);
+static bool few_rows(const fs_paged_attn_args& a) {
+  return few_rows(most_new(a), a.Hq / a.Hk, a.T, a.B, a.Hk, (int64_t)a.P * a.page_size);
 }
+static bool few_rows(const fs_window_attn_args& a) {
+  return few_rows(a.Lq, a.Hq / a.Hk, (int64_t)a.B * a.Lq, a.B, a.Hk, a.Lk);
+}
+static Work work_of(const fs_paged_attn_args& a) { return work_of(few_rows(a), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D); }
 static Work work_of(const fs_window_attn_args& a) {
-  return work_of(few_rows(a.Lq, a.Hq / a.Hk), (int64_t)a.B * a.Lq, a.B, a.Hk, a.Hq / a.Hk, a.D);
+  return work_of(few_rows(a), (int64_t)a.B * a.Lq, a.B, a.Hk, a.Hq / a.Hk, a.D);
 }
 
 extern "C" size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a) {
@@ -1031,7 +1207,7 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
   const uint32_t groups = a->page_size / 16;       // x / groups for x < 2^22, groups <= 256: mulhi is exact
   k.page_magic = groups > 1 ? (uint32_t)((1ull << 32) / groups + 1) : 0;
-  const bool few = few_rows(most_new(*a), a->Hq / a->Hk);
+  const bool few = few_rows(*a);
   return run<true>(k, a->dtype, a->D, few, true, work_of(*a), static_cast<char*>(a->work), a->B, a->T, (hipStream_t)stream, fn);
 }
 
@@ -1058,11 +1234,11 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   k.num_pages = a->B; k.B = a->B; k.Hq = a->Hq; k.Hk = a->Hk; k.Lq = a->Lq; k.Lk = a->Lk; k.page_size = a->Lk;
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
   k.T = a->Lq;
-  const bool few = few_rows(a->Lq, a->Hq / a->Hk);
+  const bool few = few_rows(*a);
   const Work w = work_of(*a);
   // Every sequence is as long here: whether splitting keys can pay is known.
   const int64_t tiles = ((int64_t)a->Lq * (a->Hq / a->Hk) + w.rows - 1) / w.rows * a->B * a->Hk;
   const int64_t keys = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
-  const bool plan = tiles < (few ? few_slots(a->D) : kSlotsMany) && keys >= 1024;
+  const bool plan = !few && tiles < kSlotsMany && keys >= 1024;
   return run<false>(k, a->dtype, a->D, few, plan, w, static_cast<char*>(a->work), a->B, a->Lq, (hipStream_t)stream, fn);
 }

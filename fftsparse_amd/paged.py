@@ -34,60 +34,74 @@ _INT32_MAX = 2 ** 31 - 1
 
 
 def _inference_only(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or on detached tensors")
 
 
-def _strides(t: torch.Tensor) -> list[int]:
+def _strides(t: torch.Tensor):
     """Element strides, 0 for dimensions of size 1 (whose stride says nothing)."""
-    return [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
+    st, shape = t.stride(), t.shape
+    return [s if n > 1 else 0 for n, s in zip(shape, st)] if 1 in shape else st
 
 
-def _aligned(t: torch.Tensor) -> bool:
+def _aligned(t: torch.Tensor, st) -> bool:
     """Whether the kernels can read t as it is: d contiguous, 16-byte rows."""
-    st = _strides(t)
-    return st[-1] == 1 and not any(s % 8 for s in st[:-1]) and t.data_ptr() % 16 == 0
+    bits = t.data_ptr() >> 1 if st[-1] == 1 else 1
+    for s in st[:-1]:
+        bits |= s
+    return not bits & 7
 
 
-def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
-    """[T, H, D] input, copied if its layout cannot be read."""
+def _rows(t: torch.Tensor, name: str):
+    """[T, H, D] input, copied if its layout cannot be read, and its strides."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be a [T, H, D] tensor, got shape {tuple(t.shape)}")
-    return t if _aligned(t) else t.contiguous()
+    st = _strides(t)
+    if not _aligned(t, st):
+        t = t.contiguous()
+        st = _strides(t)
+    return t, st
 
 
-def _written(t: torch.Tensor, name: str, shape, dtype) -> torch.Tensor:
-    """A tensor the kernels write: as it is, or not at all."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+def _written(t: torch.Tensor, name: str, shape, dtype):
+    """Strides of a tensor that the kernels read or write as it is, or not at all."""
+    if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} must be a {list(shape)} {dtype} tensor, got {t.dtype} {tuple(t.shape)}")
-    if t.numel() and (not _aligned(t) or any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride()))):
-        raise ValueError(f"{name} must have d contiguous, strides that are multiples of 8 elements and 16-byte "
-                         f"alignment, and no broadcast dimension, got strides {t.stride()}")
-    return t
+    st = _strides(t)
+    if not _aligned(t, st) or (0 in st and any(n > 1 and s == 0 for n, s in zip(shape, st))):
+        if t.numel():
+            raise ValueError(f"{name} must have d contiguous, strides that are multiples of 8 elements and 16-byte "
+                             f"alignment, and no broadcast dimension, got strides {t.stride()}")
+    return st
 
 
 def _ints(t: torch.Tensor, name: str, shape, dtypes=(torch.int32,)) -> torch.Tensor:
-    if tuple(t.shape) != tuple(shape) or t.dtype not in dtypes or not t.is_contiguous():
+    if t.shape != shape or t.dtype not in dtypes or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {list(shape)} tensor of {' or '.join(map(str, dtypes))}, got "
                          f"{t.dtype} {tuple(t.shape)}")
     return t
 
 
-def _table(t: torch.Tensor) -> torch.Tensor:
+def _table(t: torch.Tensor):
+    """[B, P] block table -> B, P, row stride."""
     if t.dim() != 2 or t.dtype != torch.int32 or not t.numel() or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"block_table must be an int32 [requests, pages] tensor with contiguous rows, got {t.dtype} "
                          f"{tuple(t.shape)}")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    B, P = t.shape
+    if B > 1 and t.stride(0) < P:
         raise ValueError("block_table's rows overlap")
-    return t
+    return B, P, t.stride(0) if B > 1 else P
 
 
 def _caches(k: torch.Tensor, v: torch.Tensor, dtype, Hk=None, D=None):
-    """k_cache and v_cache as views the kernels read and write."""
-    if k.dim() != 4 or not k.numel():
-        raise ValueError(f"k_cache must be a [pages, page_size, Hk, D] tensor, got shape {tuple(k.shape)}")
-    shape = (k.shape[0], k.shape[1], k.shape[2] if Hk is None else Hk, k.shape[3] if D is None else D)
-    return _written(k, "k_cache", shape, dtype), _written(v, "v_cache", shape, dtype)
+    """Shape and strides of k_cache and v_cache, views that the kernels read and write as they are."""
+    shape = k.shape
+    if len(shape) != 4 or not k.numel():
+        raise ValueError(f"k_cache must be a [pages, page_size, Hk, D] tensor, got shape {tuple(shape)}")
+    want = (shape[0], shape[1], shape[2] if Hk is None else Hk, shape[3] if D is None else D)
+    return want, _written(k, "k_cache", want, dtype), _written(v, "v_cache", want, dtype)
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -124,8 +138,8 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
     ``free_count`` are not: take them from the result for the next step.  A
     step whose ``lacking`` is not 0 is undone by not using its result.
     ``out``: a former result to write into, whose tensors are not this call's inputs."""
-    t = _table(block_table)
-    B, P = t.shape
+    t = block_table
+    B, P, t_sb = _table(t)
     _ints(seq_lens, "seq_lens", (B,))
     _ints(new_lens, "new_lens", (B,))
     if free_pages.dim() != 1 or not free_pages.numel():
@@ -137,21 +151,20 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
         raise ValueError(f"page_size {page_size} and num_tokens {num_tokens} out of range for a table of {P} pages")
     dev = _lib.same_device(t, seq_lens, new_lens, free_pages, free_count)
     if out is None:
-        i32 = dict(dtype=torch.int32, device=dev)
-        out = StepPlan(torch.empty(B + 1, **i32), torch.empty(B, **i32), torch.empty(num_tokens, **i32),
-                       torch.empty(num_tokens, dtype=torch.int64, device=dev), torch.empty(1, **i32),
-                       torch.empty(1, **i32))
+        cu_lens, after, positions, count, lacking = torch.empty(
+            2 * B + 3 + num_tokens, dtype=torch.int32, device=dev).split((B + 1, B, num_tokens, 1, 1))
+        out = StepPlan(cu_lens, after, positions, torch.empty(num_tokens, dtype=torch.int64, device=dev), count, lacking)
     else:
         outs = [_ints(out.cu_lens, "out.cu_lens", (B + 1,)), _ints(out.seq_lens, "out.seq_lens", (B,)),
                 _ints(out.positions, "out.positions", (num_tokens,)),
                 _ints(out.slots, "out.slots", (num_tokens,), (torch.int64,)),
                 _ints(out.free_count, "out.free_count", (1,)), _ints(out.lacking, "out.lacking", (1,))]
         _lib.same_device(t, *outs)
-        if any(_overlap(o, i) for o in outs for i in (seq_lens, new_lens, free_pages, free_count)):
+        if any(_overlap(o, i) for o in outs for i in (seq_lens, new_lens, free_pages, free_count, t)):
             raise ValueError("out shares storage with an input of the step: the lengths and the free count of a step "
                              "are read while its result is written")
     _lib.call("fs_plan", PlanArgs(
-        block_table=t.data_ptr(), t_sb=t.stride(0) if B > 1 else P, seq_lens=seq_lens.data_ptr(),
+        block_table=t.data_ptr(), t_sb=t_sb, seq_lens=seq_lens.data_ptr(),
         new_lens=new_lens.data_ptr(), free_pages=free_pages.data_ptr(), free_count=free_count.data_ptr(), B=B, P=P,
         F=free_pages.numel(), page_size=page_size, T=num_tokens, cu_lens=out.cu_lens.data_ptr(),
         seq_lens_out=out.seq_lens.data_ptr(), positions=out.positions.data_ptr() or 16,
@@ -193,15 +206,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     for any value, the right one is faster.  Rows behind cu_lens[B] are left as
     they were (unset in a new tensor).  A page number outside the cache holds no
     token; a row that sees no token is 0."""
-    q = _rows(q, "q")
+    q, qs = _rows(q, "q")
     T, Hq, D = q.shape
     _attn_dtype(q, k_cache, v_cache)
-    _caches(k_cache, v_cache, q.dtype, D=D)
-    pages, ps, Hk = k_cache.shape[:3]
+    (pages, ps, Hk, _), ks, vs = _caches(k_cache, v_cache, q.dtype, D=D)
     if Hk == 0 or Hq % Hk or Hq == 0:
         raise ValueError(f"query heads {Hq} must be a multiple of key heads {Hk}")
-    t = _table(block_table)
-    B, P = t.shape
+    t = block_table
+    B, P, t_sb = _table(t)
     _ints(cu_lens, "cu_lens", (B + 1,))
     _ints(seq_lens, "seq_lens", (B,))
     window, sinks = _window(window, sinks)
@@ -210,17 +222,18 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _inference_only("paged_attention", q, k_cache, v_cache)
     if out is None:
         dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens)
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        os_ = (Hq * D, D)
     else:
-        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, _written(out, "out", (T, Hq, D), q.dtype))
+        os_ = _written(out, "out", (T, Hq, D), q.dtype)
+        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, out)
     if T == 0:
         return out
-    qs, os_, ks, vs = _strides(q), _strides(out), _strides(k_cache), _strides(v_cache)
     args = PagedAttnArgs(
         q=q.data_ptr(), q_st=qs[0], q_sh=qs[1], out=out.data_ptr(), o_st=os_[0], o_sh=os_[1],
         k_cache=k_cache.data_ptr(), k_sp=ks[0], k_ss=ks[1], k_sh=ks[2],
         v_cache=v_cache.data_ptr(), v_sp=vs[0], v_ss=vs[1], v_sh=vs[2],
-        block_table=t.data_ptr(), t_sb=t.stride(0) if B > 1 else P, cu_lens=cu_lens.data_ptr(),
+        block_table=t.data_ptr(), t_sb=t_sb, cu_lens=cu_lens.data_ptr(),
         seq_lens=seq_lens.data_ptr(), dtype=_lib.FS_DTYPE[q.dtype], B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=P, page_size=ps,
         num_pages=pages, max_new=0 if max_new is None else min(int(max_new), T), window=window, sinks=sinks,
         softmax_scale=1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale))
@@ -253,11 +266,9 @@ def window_attention(query_states: torch.Tensor, key_states: torch.Tensor, value
     window, sinks = _window(window, sinks)
     _inference_only("window_attention", q, k, v)
     if out is None:
-        dev = _lib.same_device(q, k, v)
-        out = torch.empty(B, Lq, Hq, D, dtype=q.dtype, device=q.device)
-    else:
-        dev = _lib.same_device(q, k, v, _written(out, "out", (B, Lq, Hq, D), q.dtype))
-    qs, ks, vs, os_ = (_strides(x) for x in (q, k, v, out))
+        out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _written(out, "out", (B, Lq, Hq, D), q.dtype)
+    dev = _lib.same_device(q, k, v, out)
     args = WindowAttnArgs(
         q=q.data_ptr(), q_sb=qs[0], q_sh=qs[1], q_sl=qs[2], k=k.data_ptr(), k_sb=ks[0], k_sh=ks[1], k_sl=ks[2],
         v=v.data_ptr(), v_sb=vs[0], v_sh=vs[1], v_sl=vs[2], out=out.data_ptr(), o_sb=os_[0], o_sl=os_[1], o_sh=os_[2],

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import RopeArgs
-from .paged import _caches, _inference_only, _ints, _rows, _strides, _written
+from .paged import _caches, _inference_only, _ints, _rows, _written
 
 
 def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -71,7 +71,8 @@ def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | N
 
 
 def _common(name, q, k, positions, inv_freq):
-    q, k = _rows(q, "q"), _rows(k, "k")
+    q, qs = _rows(q, "q")
+    k, ks = _rows(k, "k")
     T, Hq, D = q.shape
     if k.shape[0] != T or k.shape[2] != D or not Hq or not k.shape[1] or not D:
         raise ValueError(f"query {tuple(q.shape)} and key {tuple(k.shape)} shapes do not match")
@@ -82,11 +83,19 @@ def _common(name, q, k, positions, inv_freq):
         raise ValueError(f"inv_freq must hold half of at most {D} rotated dims, got {inv_freq.dtype} "
                          f"{tuple(inv_freq.shape)}")
     _inference_only(name, q, k)
-    return q, k, inv_freq.to(torch.float64).contiguous()
+    if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.to(torch.float64).contiguous()
+    return q, qs, k, ks, inv_freq
 
 
-def _args(q, k, q_out, positions, inv_freq, attention_factor, interleaved) -> RopeArgs:
-    qs, ks, os_ = _strides(q), _strides(k), _strides(q_out)
+def _out(out, name, like):
+    """The given output (checked) or a new one, and its strides."""
+    if out is None:
+        out = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+    return out, _written(out, name, like.shape, like.dtype)
+
+
+def _args(q, qs, k, ks, q_out, os_, positions, inv_freq, attention_factor, interleaved) -> RopeArgs:
     return RopeArgs(q=q.data_ptr(), q_st=qs[0], q_sh=qs[1], k=k.data_ptr(), k_st=ks[0], k_sh=ks[1],
                     positions=positions.data_ptr(), inv_freq=inv_freq.data_ptr(),
                     attention_factor=float(attention_factor), pos_bytes=positions.element_size(),
@@ -102,13 +111,12 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
     (int32 or int64 [T]): the first 2 len(inv_freq) dims of every head are rotated, in pairs (i, i + half) or,
     ``interleaved``, (2 i, 2 i + 1); the others are copied.  Angles in 64 bits, rounded once.  Returns (q_rot,
     k_rot); ``q_out`` / ``k_out`` may be q / k themselves.  Rows with a negative position are left as they were."""
-    q, k, inv_freq = _common("rope", q, k, positions, inv_freq)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else _written(q_out, "q_out", q.shape, q.dtype)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else _written(k_out, "k_out", k.shape, k.dtype)
+    q, qs, k, ks, inv_freq = _common("rope", q, k, positions, inv_freq)
+    q_out, os_ = _out(q_out, "q_out", q)
+    k_out, st = _out(k_out, "k_out", k)
     dev = _lib.same_device(q, k, positions, inv_freq, q_out, k_out)
     if q.shape[0]:
-        a = _args(q, k, q_out, positions, inv_freq, attention_factor, interleaved)
-        st = _strides(k_out)
+        a = _args(q, qs, k, ks, q_out, os_, positions, inv_freq, attention_factor, interleaved)
         a.k_out, a.ko_st, a.ko_sh = k_out.data_ptr(), st[0], st[1]
         _lib.call("fs_rope", a, dev)
     return q_out, k_out
@@ -121,21 +129,20 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     ``plan_step``: page * page_size + slot, all different) of ``k_cache`` / ``v_cache`` [pages, page_size, Hk, D].
     Returns q_rot.  A slot outside the cache (-1: none) is not written; a row with a negative position is left as it
     was, in the cache too."""
-    q, k, inv_freq = _common("rope_cache", q, k, positions, inv_freq)
-    v = _rows(v, "v")
+    q, qs, k, ks, inv_freq = _common("rope_cache", q, k, positions, inv_freq)
+    v, vs = _rows(v, "v")
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"value {v.dtype} {tuple(v.shape)} must be like key {k.dtype} {tuple(k.shape)}")
     _ints(slots, "slots", (q.shape[0],), (torch.int64,))
-    _caches(k_cache, v_cache, q.dtype, k.shape[1], k.shape[2])
+    shape, kc, vc = _caches(k_cache, v_cache, q.dtype, k.shape[1], k.shape[2])
     _inference_only("rope_cache", v, k_cache, v_cache)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else _written(q_out, "q_out", q.shape, q.dtype)
+    q_out, os_ = _out(q_out, "q_out", q)
     dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out)
     if q.shape[0]:
-        a = _args(q, k, q_out, positions, inv_freq, attention_factor, interleaved)
-        vs, kc, vc = _strides(v), _strides(k_cache), _strides(v_cache)
+        a = _args(q, qs, k, ks, q_out, os_, positions, inv_freq, attention_factor, interleaved)
         a.v, a.v_st, a.v_sh, a.slots = v.data_ptr(), vs[0], vs[1], slots.data_ptr()
-        a.k_cache, a.kc_sp, a.kc_ss, a.kc_sh = k_cache.data_ptr(), *kc[:3]
-        a.v_cache, a.vc_sp, a.vc_ss, a.vc_sh = v_cache.data_ptr(), *vc[:3]
-        a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[1]
+        a.k_cache, a.kc_sp, a.kc_ss, a.kc_sh = k_cache.data_ptr(), kc[0], kc[1], kc[2]
+        a.v_cache, a.vc_sp, a.vc_ss, a.vc_sh = v_cache.data_ptr(), vc[0], vc[1], vc[2]
+        a.num_pages, a.page_size = shape[0], shape[1]
         _lib.call("fs_rope", a, dev)
     return q_out
