@@ -37,7 +37,7 @@
 namespace fs {
 
 #ifndef FEW_WAVES
-#define FEW_WAVES 2
+#define FEW_WAVES 4
 #endif
 constexpr int kFewWaves = FEW_WAVES;                // of a workgroup of few_kernel
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
@@ -58,8 +58,8 @@ struct PagedKArgs {
   const int32_t* table;                         // null: contiguous, the page of request b is b
   const int32_t* cu;
   const int32_t* lens;
-  int64_t t_sb, num_pages;
-  int B, T, Hq, Hk, G, Lq, Lk, P, page_size, window, sinks;
+  int64_t t_sb;
+  int num_pages, B, T, Hq, Hk, G, Lq, Lk, P, page_size, window, sinks;
   uint32_t page_magic;                          // x / (page_size / 16) = mulhi(x, magic); 0: x
   float scale;
   // pieces, the last row tiles of a request first
@@ -123,7 +123,11 @@ struct GroupCopy {
   static constexpr int NI = 16 / RPR;              // copies of a group
   uint32_t koff[NI], voff[NI];
   const uint16_t *kp, *vp;
-  __device__ __forceinline__ GroupCopy(const PagedKArgs& a, int hk, int lane) {
+  const int32_t* row;                              // of the table
+  int page;                                        // contiguous: the request
+  __device__ __forceinline__ GroupCopy(const PagedKArgs& a, int b, int hk, int lane) {
+    row = PAGED ? a.table + b * a.t_sb : nullptr;
+    page = b;
     kp = a.k + hk * a.k_sh;
     vp = a.v + hk * a.v_sh;
 #pragma unroll
@@ -135,31 +139,35 @@ struct GroupCopy {
   }
   static __device__ __forceinline__ int kchunk(int r, int lane) { return (lane & SWM) ^ ((D == 128 ? r : r >> 1) & SWM); }
   static __device__ __forceinline__ int vchunk(int r, int lane) { return (lane & SWM) ^ v_swz<D>(r); }
-  // the table's entry for the group of key k0 (a multiple of 16), -1 where the tile sees no key of it
-  static __device__ __forceinline__ int entry(const PagedKArgs& a, const RowTile& u, int b, int k0) {
-    const int last = k0 + 15;
-    if (k0 >= u.kend || (last < u.kbeg && k0 >= a.sinks)) return -1;
-    if constexpr (!PAGED) return b;
+  // the page of the table's row that holds key k0 (a multiple of 16), and the key's slot there
+  static __device__ __forceinline__ int page_of(const PagedKArgs& a, int k0, int& slot) {
+    if constexpr (!PAGED) {
+      slot = k0;
+      return 0;
+    }
     const uint32_t x = (uint32_t)k0 >> 4;
     const uint32_t pg = a.page_magic ? __umulhi(x, a.page_magic) : x;
-    const int e = scalar_load(a.table, (int64_t)b * a.t_sb + pg);
-    return e >= 0 && e < a.num_pages ? e : -1;
+    slot = k0 - (int)pg * a.page_size;
+    return (int)pg;
   }
-  static __device__ __forceinline__ int slot_of(const PagedKArgs& a, int k0) {
-    if constexpr (!PAGED) return k0;
-    const uint32_t x = (uint32_t)k0 >> 4;
-    const uint32_t pg = a.page_magic ? __umulhi(x, a.page_magic) : x;
-    return k0 - (int)pg * a.page_size;
+  // the entry of page pg: the page's number in the cache, -1 for none
+  __device__ __forceinline__ int entry(int pg) const { return PAGED ? scalar_load(row, pg) : page; }
+  static __device__ __forceinline__ bool is_page(const PagedKArgs& a, int e) { return !PAGED || (uint32_t)e < (uint32_t)a.num_pages; }
+  // some row of the tile sees some key of the group of key k0
+  static __device__ __forceinline__ bool seen(const PagedKArgs& a, const RowTile& u, int k0) {
+    return k0 < u.kend && (k0 + 15 >= u.kbeg || k0 < a.sinks);
   }
-  // every key of the group is seen by some row of the tile
-  static __device__ __forceinline__ bool whole(const PagedKArgs& a, const RowTile& u, int e, int k0) {
-    return e >= 0 && k0 + 16 <= u.kend && (k0 >= u.kbeg || k0 + 16 <= a.sinks);
+  // every key of n from k0 on is seen by some row
+  static __device__ __forceinline__ bool whole(const PagedKArgs& a, const RowTile& u, int k0, int n) {
+    return k0 + n <= u.kend && (k0 >= u.kbeg || k0 + n <= a.sinks);
   }
+  // copies the group of key k0, at `slot` of page e (no page: e < 0); all: every key of it is seen
   template <bool V>
-  __device__ __forceinline__ void issue(const PagedKArgs& a, const RowTile& u, uint32_t lds, int e, int k0) const {
-    const int64_t st = V ? a.v_ss : a.k_ss;
-    const uint16_t* base = (V ? vp : kp) + max(e, 0) * (V ? a.v_sp : a.k_sp) + slot_of(a, k0) * st;
-    if (whole(a, u, e, k0)) {
+  __device__ __forceinline__ void issue(const PagedKArgs& a, const RowTile& u, uint32_t lds, int e, int slot, int k0,
+                                        bool all) const {
+    const int st = V ? a.v_ss : a.k_ss;
+    const uint16_t* base = (V ? vp : kp) + max(e, 0) * (V ? a.v_sp : a.k_sp) + (int64_t)slot * st;
+    if (all) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) dma16s(lds + i * 1024, base, V ? voff[i] : koff[i]);
     } else {
@@ -213,24 +221,41 @@ __device__ __forceinline__ void load_q(const PagedKArgs& a, const RowTile& u, co
   }
 }
 
-// -inf for the scores of 32 keys from key0 (register r: key (r >> 2) * 8 + (r & 3) + hi * 4) that the row at p
-// does not see; v0, v1: whether the two groups of 16 are there
-__device__ __forceinline__ void mask_keys(const PagedKArgs& a, const RowTile& u, f32x16_t& s, int p, int key0, int hi,
-                                          bool v0, bool v1) {
-  const int k = key0 + hi * 4;
-  const int last = p - k;                          // c <= last
-  const int first = a.window ? p - a.window - k : INT_MIN;   // c > first, or c < sink
-  const int sink = a.window ? a.sinks - k : INT_MIN;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int c = (r >> 2) * 8 + (r & 3);
-    const bool ok = c <= last && (c > first || c < sink) && (r < 8 ? v0 : v1);
-    if (!ok) s[r] = -INFINITY;
-  }
-}
 // whether some row of positions p_lo .. p_hi does not see some key of key0 .. key0 + n - 1
 __device__ __forceinline__ bool needs_mask(const PagedKArgs& a, int p_lo, int p_hi, int key0, int n) {
   return key0 + n - 1 > p_lo || (a.window && key0 <= p_hi - a.window && key0 + n > a.sinks);
+}
+// -inf for the scores of 32 keys from key0 (register r: key (r >> 2) * 8 + (r & 3) + hi * 4) that the row at p does
+// not see; p_lo, p_hi: positions of the wave's first and last row; v0, v1: whether the two groups of 16 are there.  Each of the
+// edges (the diagonal, the window's start) costs two instructions per score, so it is looked at where some row has it.
+__device__ __forceinline__ void mask_keys(const PagedKArgs& a, f32x16_t& s, int p, int p_lo, int p_hi, int key0, int hi,
+                                          bool v0, bool v1) {
+  const int k = key0 + hi * 4;
+  if (key0 + 31 > p_lo) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if ((r >> 2) * 8 + (r & 3) > p - k) s[r] = -INFINITY;
+  }
+  if (a.window && key0 <= p_hi - a.window && key0 + 32 > a.sinks) {
+    const int first = p - a.window - k;
+    if (key0 >= a.sinks) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if ((r >> 2) * 8 + (r & 3) <= first) s[r] = -INFINITY;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if ((r >> 2) * 8 + (r & 3) <= first && (r >> 2) * 8 + (r & 3) >= a.sinks - k) s[r] = -INFINITY;
+    }
+  }
+  if (!v0) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s[r] = -INFINITY;
+  }
+  if (!v1) {
+#pragma unroll
+    for (int r = 8; r < 16; ++r) s[r] = -INFINITY;
+  }
 }
 
 // O^T of one row (this lane's dims dt * 32 + g4 * 8 + hi * 4 .. + 3) to the output
@@ -242,9 +267,31 @@ __device__ __forceinline__ void store_out(uint16_t* op, int d0, float x0, float 
   w.y = (uint32_t)Ops::bits(x2) | ((uint32_t)Ops::bits(x3) << 16);
   *reinterpret_cast<uint2*>(op + d0) = w;
 }
-__device__ __forceinline__ uint16_t* out_row(const PagedKArgs& a, const RowTile& u, const LaneRow& w, int b, int hk) {
+template <typename A>
+__device__ __forceinline__ uint16_t* out_row(const A& a, const RowTile& u, const LaneRow& w, int b, int hk) {
   return a.out + b * a.o_sb + (int64_t)(u.row0 + w.tok) * a.o_st + (int64_t)(hk * a.G + w.g) * a.o_sh;
 }
+
+// What a kernel's end needs of its arguments, read from them only then.
+struct LateArgs {
+  uint16_t* out;
+  int64_t o_sb, o_st, o_sh;
+  float *part_o, *part_ml;
+  int T, G;
+  __device__ __forceinline__ LateArgs() {
+    typedef const __attribute__((address_space(4))) PagedKArgs* kptr;
+    kptr a = (kptr)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(a));
+    out = a->out;
+    o_sb = a->o_sb;
+    o_st = a->o_st;
+    o_sh = a->o_sh;
+    part_o = a->part_o;
+    part_ml = a->part_ml;
+    T = a->T;
+    G = a->G;
+  }
+};
 
 // The piece of workgroup p: KV head, request, row tile, first key tile, key tiles, slot (-1: no other piece).
 struct Piece {
@@ -252,11 +299,11 @@ struct Piece {
 };
 
 // How long a call takes, in key tiles' time: N pieces of at most c tiles of the W in all, `slots` at a time; a start
-// per round of pieces and, where sums are joined, the joining.
-__device__ __forceinline__ float call_time(float N, float c, float W, float slots, bool joined) {
-  constexpr float kStart = 1.5f, kJoin = 2.0f;
+// per round of pieces and, where sums are joined, a launch and their writing and reading.
+__device__ __forceinline__ float call_time(float N, float c, float W, float slots, float joined) {
+  constexpr float kStart = 1.5f, kJoin = 2.0f, kPiece = 0.014f;
   const float rounds = ceilf(N / slots);
-  return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined ? kJoin : 0.f);
+  return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined > 0.f ? kJoin + joined * kPiece : 0.f);
 }
 // The 16 numbers of key tiles per piece that are tried: an i-th part of the longest row tile's, and what gives about i
 // rounds of pieces (U row tiles, of which each may leave a shorter piece).
@@ -428,7 +475,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     pos += count;
     const RowTile u = row_tile<32, 32 * NW>(a, at.x, at.rt);
     const LaneRow me = lane_row(a, u, l32);
-    const Copy cp(a, at.hk, lane);
+    const Copy cp(a, at.b, at.hk, lane);
     V8 qf[D / 16];
     load_q<V8, D>(a, u, me, at.b, at.hk, hi, qf);
 
@@ -439,28 +486,34 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     };
     int cnt = min(count, u.nt - begin);
     if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
+    // pages of the two groups of a step's keys (-1: none) and the keys' slots there
     struct Ent {
-      int e[2];
+      int e[2], slot[2];
     };
     auto load_ent = [&](int i) {
-      Ent x{{-1, -1}};
-      if (i < cnt) {
-        const int k = key_of(i);
-        x.e[0] = Copy::entry(a, u, at.b, k);
-        x.e[1] = Copy::entry(a, u, at.b, k + 16);
+      Ent x{{-1, -1}, {0, 0}};
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const int k = key_of(i) + 16 * g;
+        if (i < cnt && Copy::seen(a, u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, x.slot[g]));
       }
       return x;
     };
-    auto issue_k = [&](int i, const Ent& x) {
-      const uint32_t at = ring0 + (i & 1) * TILE;
-      cp.template issue<false>(a, u, at, x.e[0], key_of(i));
-      cp.template issue<false>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+    auto there = [&](Ent& x) {                     // looked at a step after it is loaded
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (!Copy::is_page(a, x.e[g])) x.e[g] = -1;
     };
-    auto issue_v = [&](int i, const Ent& x) {
-      const uint32_t at = ring0 + (2 + (i & 1)) * TILE;
-      cp.template issue<true>(a, u, at, x.e[0], key_of(i));
-      cp.template issue<true>(a, u, at + TILE / 2, x.e[1], key_of(i) + 16);
+    auto issue = [&](auto v, int i, const Ent& x) {
+      constexpr bool V = decltype(v)::value;
+      const uint32_t at = ring0 + ((V ? 2 : 0) + (i & 1)) * TILE;
+      const int k = key_of(i);
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        cp.template issue<V>(a, u, at + g * TILE / 2, x.e[g], x.slot[g], k + 16 * g, x.e[g] >= 0 && Copy::whole(a, u, k + 16 * g, 16));
     };
+    auto issue_k = [&](int i, const Ent& x) { issue(std::integral_constant<bool, false>(), i, x); };
+    auto issue_v = [&](int i, const Ent& x) { issue(std::integral_constant<bool, true>(), i, x); };
     constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
     const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
     const int vrow = hi * 4 + ((lane & 15) >> 2);
@@ -477,6 +530,8 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this
     // order; K(i+2) and V(i+2) are requested as soon as their place is read.
     Ent x0 = load_ent(0), x1 = load_ent(1), x2 = load_ent(2);
+    there(x0);
+    there(x1);
     if (cnt > 0) {
       issue_k(0, x0);
       issue_v(0, x0);
@@ -495,14 +550,14 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
       for (int r = 0; r < 16; ++r) s[r] = 0.f;
 #pragma unroll
       for (int st = 0; st < D / 16; ++st) s = Ops::mma(__builtin_bit_cast(V8, lds16(kt, k_lane ^ (uint32_t)(st << 5))), qf[st], s);
+      there(x2);
       const Ent x3 = load_ent(i + 3);
       if (i + 2 < cnt) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         issue_k(i + 2, x2);
       }
       const int key0 = key_of(i);
-      if (x0.e[0] < 0 || x0.e[1] < 0 || needs_mask(a, u.p_lo, u.p_hi, key0, 32))
-        mask_keys(a, u, s, me.p, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+      mask_keys(a, s, me.p, u.p_lo, u.p_hi, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
       float mx = s[0], h0, h1;
 #pragma unroll
       for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -600,18 +655,18 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
   }
 }
 
-// The pieces' sums joined: 32 rows of a split row tile per workgroup.  A thread adds 4 dims of one row over every J-th
+// The pieces' sums joined: 32 rows and 32 dims of a split row tile per workgroup.  A thread adds 4 dims of one row over every J-th
 // piece (J as many threads as there are for an item), then the J sums are added in LDS; always in the same
 // order.  Wave 0 looks up what the workgroup joins (mostly nothing).
-constexpr int kJoinThreads = 512;
+constexpr int join_threads(int M) { return M == 32 ? 256 : 512; }
 template <typename T, int D, int M>
-__global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
-  constexpr int QW = M / 32, AHEAD = 8;
+__global__ __launch_bounds__(join_threads(M)) void combine_kernel(PagedKArgs a) {
+  constexpr int QW = M / 32, NV = D / 32, NT = join_threads(M), AHEAD = 8;
   constexpr bool FEW = M == 32;
-  __shared__ float4 part[kJoinThreads];
-  __shared__ float2 ml[kJoinThreads];
+  __shared__ float4 part[NT];
+  __shared__ float2 ml[NT];
   __shared__ int job[10];                          // pieces, first slot, second slot, KV head, request, row tile, lengths
-  const int tid = threadIdx.x, qq = blockIdx.x % QW, w = blockIdx.x / QW;
+  const int tid = threadIdx.x, dt = blockIdx.x % NV, qq = blockIdx.x / NV % QW, w = blockIdx.x / (NV * QW);
   if (tid < 64) {
     int np = 0;
     if constexpr (FEW) {
@@ -665,61 +720,57 @@ __global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
   const RowTile u = row_tile<M, 64>(a, x, __builtin_amdgcn_readfirstlane(job[5]));
   const int rows = min(u.nrows - qq * 32, 32);
   if (rows <= 0) return;
-  const int items = rows * (D / 4);                // an item: row, and 4 dims: 32 dt + 8 g4 + 4 hi ..
-  const int J = max(kJoinThreads / items, 1);
+  const int items = rows * 8, J = NT / items;      // an item: row, and 4 dims: 32 dt + 4 c ..
   auto slot_of = [&](int j) { return (int64_t)(j == 0 ? s0 : s1 + (j - 1) * (FEW ? 2 : QW)); };
-  for (int i0 = 0; i0 < items; i0 += kJoinThreads) {
-    const int jg = items < kJoinThreads ? tid / items : 0, it = items < kJoinThreads ? tid - jg * items : i0 + tid;
-    const int c = it / rows, r = it - c * rows;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (jg < J && it < items)
-      for (int j0 = jg; j0 < np; j0 += AHEAD * J) {
-        float mj[AHEAD], lj[AHEAD];
-        float4 xj[AHEAD];
+  const int jg = tid / items, it = tid - jg * items;
+  const int c = it / rows, r = it - c * rows;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (jg < J)
+    for (int j0 = jg; j0 < np; j0 += AHEAD * J) {
+      float mj[AHEAD], lj[AHEAD];
+      float4 xj[AHEAD];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          const int64_t s = slot_of(min(j0 + k * J, np - 1));
-          mj[k] = a.part_ml[s * 64 + r];
-          lj[k] = a.part_ml[s * 64 + 32 + r];
-          xj[k] = reinterpret_cast<const float4*>(a.part_o)[(s * (D / 8) + (c >> 1)) * 64 + (c & 1) * 32 + r];
-        }
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          if (j0 + k * J >= np) break;
-          const float mn = fmaxf(m, mj[k]), mu = mn == -INFINITY ? 0.f : mn;
-          const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(mj[k] - mu);
-          m = mn;
-          l = l * f0 + lj[k] * f1;
-          acc.x = acc.x * f0 + xj[k].x * f1;
-          acc.y = acc.y * f0 + xj[k].y * f1;
-          acc.z = acc.z * f0 + xj[k].z * f1;
-          acc.w = acc.w * f0 + xj[k].w * f1;
-        }
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t s = slot_of(min(j0 + k * J, np - 1));
+        mj[k] = a.part_ml[s * 64 + r];
+        lj[k] = a.part_ml[s * 64 + 32 + r];
+        xj[k] = reinterpret_cast<const float4*>(a.part_o)[((s * NV + dt) * 4 + (c >> 1)) * 64 + (c & 1) * 32 + r];
       }
-    if (J > 1) {                                   // all items at once
-      part[tid] = acc;
-      ml[tid] = make_float2(m, l);
-      __syncthreads();
-      for (int k = 1; jg == 0 && k < J; ++k) {
-        const float2 o = ml[k * items + it];
-        const float4 y = part[k * items + it];
-        const float mn = fmaxf(m, o.x), mu = mn == -INFINITY ? 0.f : mn;
-        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(o.x - mu);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (j0 + k * J >= np) break;
+        const float mn = fmaxf(m, mj[k]), mu = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(mj[k] - mu);
         m = mn;
-        l = l * f0 + o.y * f1;
-        acc.x = acc.x * f0 + y.x * f1;
-        acc.y = acc.y * f0 + y.y * f1;
-        acc.z = acc.z * f0 + y.z * f1;
-        acc.w = acc.w * f0 + y.w * f1;
+        l = l * f0 + lj[k] * f1;
+        acc.x = acc.x * f0 + xj[k].x * f1;
+        acc.y = acc.y * f0 + xj[k].y * f1;
+        acc.z = acc.z * f0 + xj[k].z * f1;
+        acc.w = acc.w * f0 + xj[k].w * f1;
       }
     }
-    const LaneRow me = lane_row(a, u, qq * 32 + r);
-    if (jg > 0 || it >= items || !me.on) continue;
-    const float inv = l != 0.f ? 1.0f / l : 0.f;
-    store_out<T>(out_row(a, u, me, b, hk), (c >> 3) * 32 + ((c >> 1) & 3) * 8 + (c & 1) * 4, acc.x * inv, acc.y * inv,
-                 acc.z * inv, acc.w * inv);
+  if (J > 1) {
+    part[tid] = acc;
+    ml[tid] = make_float2(m, l);
+    __syncthreads();
+    for (int k = 1; jg == 0 && k < J; ++k) {
+      const float2 o = ml[k * items + it];
+      const float4 y = part[k * items + it];
+      const float mn = fmaxf(m, o.x), mu = mn == -INFINITY ? 0.f : mn;
+      const float f0 = __builtin_amdgcn_exp2f(m - mu), f1 = __builtin_amdgcn_exp2f(o.x - mu);
+      m = mn;
+      l = l * f0 + o.y * f1;
+      acc.x = acc.x * f0 + y.x * f1;
+      acc.y = acc.y * f0 + y.y * f1;
+      acc.z = acc.z * f0 + y.z * f1;
+      acc.w = acc.w * f0 + y.w * f1;
+    }
   }
+  const LaneRow me = lane_row(a, u, qq * 32 + r);
+  if (jg > 0 || !me.on) return;
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  store_out<T>(out_row(a, u, me, b, hk), dt * 32 + c * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 template <typename T, int D, bool PAGED>
@@ -729,7 +780,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   using Copy = GroupCopy<D, PAGED>;
   constexpr int TK = 64, TILE = TK * D * 2;        // bytes of a K or V tile
   constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM, GB = 16 * ROWB;
-  __shared__ __attribute__((aligned(1024))) char lds[2][2][TILE];   // [K, V][buffer]
+  // K tiles ahead (V: DK - 2): 64 KiB of LDS either way, so two workgroups share a CU.  A tile of head dim 64 is consumed in half
+  // the time, in which its copies' latency has to fit.
+  constexpr int DK = 2;
+  __shared__ __attribute__((aligned(1024))) char lds[2][DK][TILE];   // [K, V][buffer]
   Piece pc;
   if (!find_piece(a, pc)) return;
   const RowTile u = row_tile<128, TK>(a, lengths_of(a, pc.b), pc.rt);
@@ -739,28 +793,64 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // positions of this wave's first and last row
   const int w_lo = u.L - u.n + (u.r0 + min(wave * 32, max(u.nrows, 1) - 1)) / a.G;
   const int w_hi = u.L - u.n + (u.r0 + min(wave * 32 + 31, max(u.nrows, 1) - 1)) / a.G;
-  const Copy cp(a, pc.hk, lane);
+  const Copy cp(a, pc.b, pc.hk, lane);
   const int cnt = min(pc.count, u.nt - pc.begin);
   auto key_of = [&](int i) {
     const int o = pc.begin + i;
     return (o < u.ns ? o : u.t0 + o - u.ns) * TK;
   };
-  // the table's entries of a tile's four groups; wave w copies group w
-  struct Ent {
-    int e[4];
+  // A tile's place: its first key, and, kept as one number, the page of the group that this wave copies (group w of each
+  // tile), whether all of its keys are seen by some row (bit 4) and which groups are there (bits 0 - 3).  The table's
+  // entries are loaded a step before they are looked at.  The loop's scalar instructions cost as vector ones do, so a
+  // tile that is seen as a whole in a page of whole tiles takes the short way (3-4% of a chunk's time).
+  struct Raw {
+    int key0, slot, e[4], all;
   };
-  auto load_ent = [&](int i) {
-    Ent x{{-1, -1, -1, -1}};
-    if (i < cnt) {
+  struct Tile {
+    int key0, slot, page;
+  };
+  const bool wide = !PAGED || a.page_size % TK == 0;
+  auto load_raw = [&](int i) {
+    Raw x;
+    x.key0 = key_of(i);
+    x.all = i < cnt && Copy::whole(a, u, x.key0, TK);
+    if (wide && x.all) {
+      x.e[0] = x.e[1] = x.e[2] = x.e[3] = cp.entry(Copy::page_of(a, x.key0, x.slot));
+      x.slot += 16 * wave;
+      return x;
+    }
+    x.slot = 0;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) x.e[g] = Copy::entry(a, u, pc.b, key_of(i) + 16 * g);
+    for (int g = 0; g < 4; ++g) {
+      const int k = x.key0 + 16 * g;
+      int slot = 0;
+      x.e[g] = -1;
+      if (i < cnt && Copy::seen(a, u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, slot));
+      if (g == wave) x.slot = slot;
     }
     return x;
   };
+  auto pack = [&](const Raw& x) {
+    int own = x.e[0], there = (x.e[0] >= 0 && Copy::is_page(a, x.e[0])) ? 1 : 0;
+    if (wide && x.all) {
+      there *= 15;
+    } else {
+#pragma unroll
+      for (int g = 1; g < 4; ++g) {
+        there |= (x.e[g] >= 0 && Copy::is_page(a, x.e[g])) ? 1 << g : 0;
+        own = wave == g ? x.e[g] : own;
+      }
+    }
+    return Tile{x.key0, x.slot, ((there >> wave & 1) ? own << 5 : -32) | (x.all ? 16 : 0) | there};
+  };
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&lds[0][0][0]) + wave * GB;
-  auto own = [&](const Ent& x) { return wave == 0 ? x.e[0] : wave == 1 ? x.e[1] : wave == 2 ? x.e[2] : x.e[3]; };
-  auto issue_k = [&](int i, const Ent& x) { cp.template issue<false>(a, u, lds0 + (i & 1) * TILE, own(x), key_of(i) + 16 * wave); };
-  auto issue_v = [&](int i, const Ent& x) { cp.template issue<true>(a, u, lds0 + (2 + (i & 1)) * TILE, own(x), key_of(i) + 16 * wave); };
+  auto issue = [&](auto v, int i, const Tile& x) {
+    constexpr bool V = decltype(v)::value;
+    cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, x.page >> 5, x.slot, x.key0 + 16 * wave,
+                         (x.page & 31) == 31);
+  };
+  auto issue_k = [&](int i, const Tile& x) { issue(std::integral_constant<bool, false>(), i, x); };
+  auto issue_v = [&](int i, const Tile& x) { issue(std::integral_constant<bool, true>(), i, x); };
 
   V8 qf[D / 16];
   load_q<V8, D>(a, u, me, pc.b, pc.hk, hi, qf);
@@ -789,13 +879,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s[kt] = Ops::mma(__builtin_bit_cast(V8, lds16(lds[0][buf] + kt * 32 * ROWB, lo)), qf[st], s[kt]);
     }
   };
-  auto mask = [&](int i, f32x16_t* s, const Ent& x) {
-    const int key0 = key_of(i);
-    const bool gone = x.e[0] < 0 || x.e[1] < 0 || x.e[2] < 0 || x.e[3] < 0;
-    if (gone || needs_mask(a, w_lo, w_hi, key0, TK)) {
-      mask_keys(a, u, s[0], me.p, key0, hi, x.e[0] >= 0, x.e[1] >= 0);
-      mask_keys(a, u, s[1], me.p, key0 + 32, hi, x.e[2] >= 0, x.e[3] >= 0);
-    }
+  auto mask = [&](f32x16_t* s, const Tile& t) {
+    const int key0 = t.key0, x = t.page;
+    if ((x & 15) == 15 && !needs_mask(a, w_lo, w_hi, key0, TK)) return;   // one test in most steps
+    mask_keys(a, s[0], me.p, w_lo, w_hi, key0, hi, x & 1, x & 2);
+    mask_keys(a, s[1], me.p, w_lo, w_hi, key0 + 32, hi, x & 4, x & 8);
   };
   auto exps = [&](const f32x16_t* s, V8* pb, float m_use) {
     float rs = 0.f;
@@ -819,24 +907,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                          pb[kk], o[dt]);
       }
   };
-  // Step t: wait for K(t+1) and V(t-1), one barrier, copy K(t+2) over K(t) and V(t) over V(t-2); then S(t+1) and
+  // Step t: wait for K(t+1) and V(t-1), one barrier, copy K(t+DK) over K(t) and V(t+DK-2) over V(t-2); then S(t+1) and
   // P V(t-1) on MFMA between the exponentials of tile t; then O's rescale (rare) and the masks of tile t+1.
   f32x16_t sa[2], sb[2];
   V8 pa[4], pb[4];
-  Ent x0{}, x1{}, x2{}, x3{};                      // of tiles t .. t+3
+  Tile x[DK + 1];                                  // of tiles t .. t+DK, the last one packed from
+  Raw raw;                                         // its entries
   typedef std::integral_constant<bool, true> yes;
   typedef std::integral_constant<bool, false> no;
   auto iter = [&](int t, f32x16_t* s_next, f32x16_t* s_cur, V8* p_prev, V8* p_cur, auto hasS, auto hasPV, auto hasE) {
     __builtin_amdgcn_s_setprio(0);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // the copies of the last DK - 2 steps may stay on their way (there are as many unless the end is near)
+    if (DK > 2 && t - 1 + DK < cnt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((DK - 2) * 2 * Copy::NI) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (t + 2 < cnt) issue_k(t + 2, x2);
-    if (t < cnt) issue_v(t, x0);
-    x3 = load_ent(t + 3);
+    x[DK] = pack(raw);
+    if (t + DK < cnt) issue_k(t + DK, x[DK]);
+    if (t + DK - 2 < cnt) issue_v(t + DK - 2, x[DK - 2]);
+    raw = load_raw(t + DK + 1);
     __builtin_amdgcn_s_setprio(2);
     float rs = 0.f, al = 1.0f;
-    if constexpr (decltype(hasS)::value) compute_s((t + 1) & 1, s_next);
-    if constexpr (decltype(hasPV)::value) pv_mma((t - 1) & 1, p_prev);
+    if constexpr (decltype(hasS)::value) compute_s((t + 1) & (DK - 1), s_next);
+    if constexpr (decltype(hasPV)::value) pv_mma((t - 1) & (DK - 1), p_prev);
     if constexpr (decltype(hasE)::value) {
       float mx = s_cur[0][0], m0, m1;
 #pragma unroll
@@ -851,8 +943,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       rs = exps(s_cur, p_cur, (m_run == -INFINITY ? 0.f : m_run) - kBias<T>);
     }
     if constexpr (decltype(hasS)::value && decltype(hasPV)::value && decltype(hasE)::value) {
-      // one MFMA, then three VALU instructions, operand reads six MFMAs ahead (as measured for bsattn_kernel)
-      constexpr int NS = 2 * (D / 16), NM = NS + 4 * (D / 32), LA = 6, VPM = 3;
+      // one MFMA, then three VALU instructions, operand reads eight MFMAs ahead (6: 1.9% slower, 10: 65%; VPM 4: 0.5%)
+      constexpr int NS = 2 * (D / 16), NM = NS + 4 * (D / 32), LA = 8, VPM = 3;
       __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
 #pragma unroll
       for (int i = 0; i < NM; ++i) {
@@ -873,23 +965,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int r = 0; r < 16; ++r) o[dt][r] *= al;   // O holds P V up to t-1 now
       }
     }
-    if constexpr (decltype(hasS)::value) mask(t + 1, s_next, x1);
-    x0 = x1;
-    x1 = x2;
-    x2 = x3;
+    if constexpr (decltype(hasS)::value) mask(s_next, x[1]);
+#pragma unroll
+    for (int i = 0; i < DK; ++i) x[i] = x[i + 1];
   };
-  if (cnt > 0) {
-    x0 = load_ent(0);
-    x1 = load_ent(1);
-    x2 = load_ent(2);
-    issue_k(0, x0);
-    if (cnt > 1) issue_k(1, x1);
+#pragma unroll
+  for (int i = 0; i < DK; ++i) x[i] = pack(load_raw(i));
+  raw = load_raw(DK);
+#pragma unroll
+  for (int i = 0; i < DK; ++i) {
+    if (i < cnt) issue_k(i, x[i]);
+    if (i < DK - 2 && i < cnt) issue_v(i, x[i]);
   }
   __builtin_amdgcn_s_waitcnt(0);
   if (cnt > 0) {
     __builtin_amdgcn_s_barrier();
     compute_s(0, sa);
-    mask(0, sa, x0);
+    mask(sa, x[0]);
     if (cnt > 1) iter(0, sb, sa, pb, pa, yes(), no(), yes());
     else iter(0, sb, sa, pb, pa, no(), no(), yes());
     int t = 1;
@@ -908,23 +1000,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       iter(t, sa, sb, pa, pb, no(), yes(), no());
     }
   }
-  if (!me.on) return;
+  // this lane's row again, and the output's arguments: neither held a register in the loop
+  int ln = lane;
+  asm volatile("" : "+v"(ln));
+  const LateArgs late;
+  const LaneRow mine = lane_row(late, u, wave * 32 + (ln & 31));
+  if (!mine.on) return;
   if (pc.slot >= 0) {
     const int64_t s = (int64_t)pc.slot * 4 + wave;
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4)
-        reinterpret_cast<float4*>(a.part_o)[((s * (D / 32) + dt) * 4 + g4) * 64 + lane] =
+        reinterpret_cast<float4*>(late.part_o)[((s * (D / 32) + dt) * 4 + g4) * 64 + lane] =
             make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
     if (hi == 0) {
-      a.part_ml[s * 64 + l32] = m_run;
-      a.part_ml[s * 64 + 32 + l32] = l_run;
+      late.part_ml[s * 64 + l32] = m_run;
+      late.part_ml[s * 64 + 32 + l32] = l_run;
     }
     return;
   }
   const float inv = l_run != 0.f ? 1.0f / l_run : 0.f;
-  uint16_t* op = out_row(a, u, me, pc.b, pc.hk);
+  uint16_t* op = out_row(late, u, mine, pc.b, pc.hk);
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -1020,7 +1117,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
     }
     n = wave_sum_i(n);
     sp = wave_sum_i(sp);
-    float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, sp > 0);
+    float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, (float)sp * (float)a.Hk);
     if (wave > 0 && (n > max_pieces || (int64_t)sp * a.Hk > max_parts)) t = INFINITY;
     if (lane == 0) cost[wave] = t;
   }
@@ -1096,7 +1193,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
     k.slots = few_slots(D);
     few_kernel<T, D, PAGED, kFewWaves><<<k.slots, 64 * kFewWaves, 0, s>>>(k);
     if (int rc = fs_host::launch_status(fn)) return rc;
-    combine_kernel<T, D, 32><<<k.slots - 1, kJoinThreads, 0, s>>>(k);
+    combine_kernel<T, D, 32><<<(k.slots - 1) * (D / 32), join_threads(32), 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   if (plan) {
@@ -1113,7 +1210,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
   many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4), kJoinThreads, 0, s>>>(k);
+    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4 * (D / 32)), join_threads(128), 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;
@@ -1182,6 +1279,7 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
                "%s: B=%d T=%d P=%d num_pages=%lld max_new=%d", fn, a->B, a->T, a->P, (long long)a->num_pages, a->max_new);
   FS_CHECK_SUPPORTED(a->page_size >= 16 && a->page_size <= 4096 && a->page_size % 16 == 0,
                      "%s: page size %d unsupported (multiples of 16 up to 4096)", fn, a->page_size);
+  FS_CHECK_SUPPORTED(a->num_pages < (1 << 27), "%s: %lld pages unsupported", fn, (long long)a->num_pages);
   FS_CHECK_SUPPORTED((int64_t)a->P * a->page_size <= (1 << 26), "%s: %d pages of %d tokens per request unsupported",
                      fn, a->P, a->page_size);
   if (a->T == 0) return FS_OK;
@@ -1202,7 +1300,7 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   k.out = static_cast<uint16_t*>(a->out);
   k.q_st = a->q_st; k.q_sh = a->q_sh; k.o_st = a->o_st; k.o_sh = a->o_sh;
   k.k_sp = a->k_sp; k.k_ss = (int)a->k_ss; k.k_sh = a->k_sh; k.v_sp = a->v_sp; k.v_ss = (int)a->v_ss; k.v_sh = a->v_sh;
-  k.table = a->block_table; k.cu = a->cu_lens; k.lens = a->seq_lens; k.t_sb = a->t_sb; k.num_pages = a->num_pages;
+  k.table = a->block_table; k.cu = a->cu_lens; k.lens = a->seq_lens; k.t_sb = a->t_sb; k.num_pages = (int)a->num_pages;
   k.B = a->B; k.T = a->T; k.Hq = a->Hq; k.Hk = a->Hk; k.P = a->P; k.page_size = a->page_size;
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
   const uint32_t groups = a->page_size / 16;       // x / groups for x < 2^22, groups <= 256: mulhi is exact
