@@ -6,7 +6,8 @@
 // So a single token fills a tile with the G heads that read the same keys, and a
 // chunk's tile of 128 rows reads each key once for all of them.  A row tile sees
 // the keys kbeg .. kend - 1 (the union of its rows' windows) and the first
-// `sinks`; tiles of keys in between are not visited.
+// `sinks`; groups of 16 keys in between are not visited, and a key tile is four groups of the
+// others in a row (the first tokens cost a group, not a tile).
 //
 // Pieces.  A row tile's keys are taken in pieces of at most `chunk` key tiles by
 // workgroups of their own where that fills the GPU better (plan_in_wave, from the
@@ -85,7 +86,9 @@ struct RowTile {
   int r0, nrows;             // rows r0 .. r0 + nrows - 1 of the request
   int p_lo, p_hi;            // positions of its first and last row
   int kbeg, kend;            // keys kbeg .. kend - 1 (and the first `sinks`) are seen by some row
-  int ns, t0, nt;            // key tiles: 0 .. ns - 1, then t0 ..; nt in all
+  int ns, t0, nt;            // groups of 16 keys: 0 .. ns - 1, then t0 ..; nt tiles in all
+  // first key of the i-th group that is visited
+  __device__ __forceinline__ int key_of(int i) const { return (i < ns ? i : t0 + i - ns) * 16; }
 };
 struct Lengths {
   int row0, n, L;
@@ -107,10 +110,11 @@ __device__ __forceinline__ RowTile row_tile(const PagedKArgs& a, const Lengths& 
   u.p_hi = u.L - u.n + (u.r0 + max(u.nrows, 1) - 1) / a.G;
   u.kend = u.nrows > 0 ? max(u.p_hi + 1, 0) : 0;
   u.kbeg = a.window ? max(u.p_lo - a.window + 1, 0) : 0;
-  u.ns = (min(a.sinks, u.kbeg) + TK - 1) / TK;
-  u.t0 = u.kbeg / TK;
+  u.ns = (min(a.sinks, u.kbeg) + 15) / 16;
+  u.t0 = u.kbeg / 16;
+  if (a.table != nullptr) u.t0 -= (u.t0 - u.ns) & 3;   // runs of 64 keys that pages of so many do not cut
   if (u.ns >= u.t0) u.ns = u.t0 = 0;
-  u.nt = u.kend > 0 ? u.ns + (u.kend + TK - 1) / TK - u.t0 : 0;
+  u.nt = u.kend > 0 ? (u.ns + (u.kend + 15) / 16 - u.t0 + TK / 16 - 1) / (TK / 16) : 0;
   return u;
 }
 
@@ -225,36 +229,23 @@ __device__ __forceinline__ void load_q(const PagedKArgs& a, const RowTile& u, co
 __device__ __forceinline__ bool needs_mask(const PagedKArgs& a, int p_lo, int p_hi, int key0, int n) {
   return key0 + n - 1 > p_lo || (a.window && key0 <= p_hi - a.window && key0 + n > a.sinks);
 }
-// -inf for the scores of 32 keys from key0 (register r: key (r >> 2) * 8 + (r & 3) + hi * 4) that the row at p does
-// not see; p_lo, p_hi: positions of the wave's first and last row; v0, v1: whether the two groups of 16 are there.  Each of the
-// edges (the diagonal, the window's start) costs two instructions per score, so it is looked at where some row has it.
-__device__ __forceinline__ void mask_keys(const PagedKArgs& a, f32x16_t& s, int p, int p_lo, int p_hi, int key0, int hi,
-                                          bool v0, bool v1) {
-  const int k = key0 + hi * 4;
-  if (key0 + 31 > p_lo) {
+// -inf for the scores of the groups of 16 keys k0 and k1 (registers 0 - 7 and 8 - 15; register r: key ((r >> 2) & 1) * 8 +
+// (r & 3) + hi * 4) that the row at p does not see; v0, v1: whether the groups are there.  A key of a group is hidden past
+// `last`, and for n keys from `from` on (between the first tokens and the window).  Written without branches: with one for
+// each edge the loop of many_kernel spilled 51 vector registers.
+__device__ __forceinline__ void mask_keys(const PagedKArgs& a, f32x16_t& s, int p, int k0, int k1, int hi, bool v0, bool v1) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      if ((r >> 2) * 8 + (r & 3) > p - k) s[r] = -INFINITY;
-  }
-  if (a.window && key0 <= p_hi - a.window && key0 + 32 > a.sinks) {
-    const int first = p - a.window - k;
-    if (key0 >= a.sinks) {
+  for (int g = 0; g < 2; ++g) {
+    __builtin_amdgcn_sched_barrier(0);             // the compares of one group at a time: they take scalar registers
+    const int k = (g ? k1 : k0) + hi * 4, last = (g ? v1 : v0) ? p - k : -1;
+    const int from = a.window ? max(a.sinks - k, 0) : 16;
+    const uint32_t n = a.window ? (uint32_t)max(p - a.window - k + 1 - from, 0) : 0u;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if ((r >> 2) * 8 + (r & 3) <= first) s[r] = -INFINITY;
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if ((r >> 2) * 8 + (r & 3) <= first && (r >> 2) * 8 + (r & 3) >= a.sinks - k) s[r] = -INFINITY;
+    for (int r = 0; r < 8; ++r) {
+      const int c = (r >> 2) * 8 + (r & 3);
+      s[8 * g + r] = c > last ? -INFINITY : s[8 * g + r];
+      s[8 * g + r] = (uint32_t)(c - from) < n ? -INFINITY : s[8 * g + r];
     }
-  }
-  if (!v0) {
-#pragma unroll
-    for (int r = 0; r < 8; ++r) s[r] = -INFINITY;
-  }
-  if (!v1) {
-#pragma unroll
-    for (int r = 8; r < 16; ++r) s[r] = -INFINITY;
   }
 }
 
@@ -365,7 +356,7 @@ struct Ranges {
     r.nt = all;                                    // its last row's keys; a row tile that sees none is written too
     if (a.window) {
       if (r.rts <= 1) r.nt = max(row_tile<M, TK>(a, r.x, 0).nt, 1);
-      else r.nt = min(all, (a.sinks + TK - 1) / TK + (a.window + (M + a.G - 2) / a.G + TK - 2) / TK + 1);
+      else r.nt = min(all, ((a.sinks + 15) / 16 + (a.window + (M + a.G - 2) / a.G + 14) / 16 + TK / 16) / (TK / 16) + 1);
     }
     return r;
   }
@@ -479,13 +470,10 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     V8 qf[D / 16];
     load_q<V8, D>(a, u, me, at.b, at.hk, hi, qf);
 
-    // this wave's 32 keys of each of the piece's tiles
-    auto key_of = [&](int i) {
-      const int o = begin + i;
-      return (o < u.ns ? o : u.t0 + o - u.ns) * (32 * NW) + 32 * wave;
-    };
+    // this wave's two groups of keys of each of the piece's tiles: the first one's place among those visited
+    auto group_of = [&](int i) { return (begin + i) * (2 * NW) + 2 * wave; };
     int cnt = min(count, u.nt - begin);
-    if (cnt > 0 && key_of(cnt - 1) >= u.kend) --cnt;  // the last tile ends before this wave's keys
+    if (cnt > 0 && u.key_of(group_of(cnt - 1)) >= u.kend) --cnt;   // the last tile ends before this wave's keys
     // pages of the two groups of a step's keys (-1: none) and the keys' slots there
     struct Ent {
       int e[2], slot[2];
@@ -494,7 +482,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
       Ent x{{-1, -1}, {0, 0}};
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const int k = key_of(i) + 16 * g;
+        const int k = u.key_of(group_of(i) + g);
         if (i < cnt && Copy::seen(a, u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, x.slot[g]));
       }
       return x;
@@ -507,10 +495,11 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     auto issue = [&](auto v, int i, const Ent& x) {
       constexpr bool V = decltype(v)::value;
       const uint32_t at = ring0 + ((V ? 2 : 0) + (i & 1)) * TILE;
-      const int k = key_of(i);
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-        cp.template issue<V>(a, u, at + g * TILE / 2, x.e[g], x.slot[g], k + 16 * g, x.e[g] >= 0 && Copy::whole(a, u, k + 16 * g, 16));
+      for (int g = 0; g < 2; ++g) {
+        const int k = u.key_of(group_of(i) + g);
+        cp.template issue<V>(a, u, at + g * TILE / 2, x.e[g], x.slot[g], k, x.e[g] >= 0 && Copy::whole(a, u, k, 16));
+      }
     };
     auto issue_k = [&](int i, const Ent& x) { issue(std::integral_constant<bool, false>(), i, x); };
     auto issue_v = [&](int i, const Ent& x) { issue(std::integral_constant<bool, true>(), i, x); };
@@ -556,8 +545,11 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         issue_k(i + 2, x2);
       }
-      const int key0 = key_of(i);
-      mask_keys(a, s, me.p, u.p_lo, u.p_hi, key0, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+      {
+        const int k0 = u.key_of(group_of(i)), k1 = u.key_of(group_of(i) + 1);
+        if (x0.e[0] < 0 || x0.e[1] < 0 || k1 != k0 + 16 || needs_mask(a, u.p_lo, u.p_hi, k0, 32))
+          mask_keys(a, s, me.p, k0, k1, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+      }
       float mx = s[0], h0, h1;
 #pragma unroll
       for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -795,44 +787,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int w_hi = u.L - u.n + (u.r0 + min(wave * 32 + 31, max(u.nrows, 1) - 1)) / a.G;
   const Copy cp(a, pc.b, pc.hk, lane);
   const int cnt = min(pc.count, u.nt - pc.begin);
-  auto key_of = [&](int i) {
-    const int o = pc.begin + i;
-    return (o < u.ns ? o : u.t0 + o - u.ns) * TK;
-  };
-  // A tile's place: its first key, and, kept as one number, the page of the group that this wave copies (group w of each
-  // tile), whether all of its keys are seen by some row (bit 4) and which groups are there (bits 0 - 3).  The table's
+  // A tile's place: its first key (the first of this wave's group, where the tile's keys are not one run), and, kept as one
+  // number, the page of the group that this wave copies (group w of each tile), whether the tile is one run of keys that
+  // are all seen by some row (bit 4) and which groups are there (bits 0 - 3).  The table's
   // entries are loaded a step before they are looked at.  The loop's scalar instructions cost as vector ones do, so a
-  // tile that is seen as a whole in a page of whole tiles takes the short way (3-4% of a chunk's time).
+  // tile that is seen as a whole and lies in one page takes the short way (3-4% of a chunk's time).
   struct Raw {
-    int key0, slot, e[4], all;
+    int key0, slot, e[4], all, one;                // one: all in one page
   };
   struct Tile {
     int key0, slot, page;
   };
-  const bool wide = !PAGED || a.page_size % TK == 0;
   auto load_raw = [&](int i) {
     Raw x;
-    x.key0 = key_of(i);
-    x.all = i < cnt && Copy::whole(a, u, x.key0, TK);
-    if (wide && x.all) {
-      x.e[0] = x.e[1] = x.e[2] = x.e[3] = cp.entry(Copy::page_of(a, x.key0, x.slot));
+    const int g0 = (pc.begin + i) * 4;
+    x.key0 = u.key_of(g0);
+    x.all = i < cnt && (g0 >= u.ns || g0 + 4 <= u.ns) && Copy::whole(a, u, x.key0, TK);
+    const int page = Copy::page_of(a, x.key0, x.slot);
+    x.one = x.all && (!PAGED || x.slot + TK <= a.page_size);
+    if (x.one) {
+      x.e[0] = x.e[1] = x.e[2] = x.e[3] = cp.entry(page);
       x.slot += 16 * wave;
       return x;
     }
     x.slot = 0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int k = x.key0 + 16 * g;
+      const int k = u.key_of(g0 + g);
       int slot = 0;
       x.e[g] = -1;
       if (i < cnt && Copy::seen(a, u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, slot));
-      if (g == wave) x.slot = slot;
+      if (g == wave) {
+        x.slot = slot;
+        if (!x.all) x.key0 = k;
+      }
     }
     return x;
   };
   auto pack = [&](const Raw& x) {
     int own = x.e[0], there = (x.e[0] >= 0 && Copy::is_page(a, x.e[0])) ? 1 : 0;
-    if (wide && x.all) {
+    if (x.one) {
       there *= 15;
     } else {
 #pragma unroll
@@ -846,7 +840,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&lds[0][0][0]) + wave * GB;
   auto issue = [&](auto v, int i, const Tile& x) {
     constexpr bool V = decltype(v)::value;
-    cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, x.page >> 5, x.slot, x.key0 + 16 * wave,
+    cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, x.page >> 5, x.slot, x.key0,
                          (x.page & 31) == 31);
   };
   auto issue_k = [&](int i, const Tile& x) { issue(std::integral_constant<bool, false>(), i, x); };
@@ -879,11 +873,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         s[kt] = Ops::mma(__builtin_bit_cast(V8, lds16(lds[0][buf] + kt * 32 * ROWB, lo)), qf[st], s[kt]);
     }
   };
-  auto mask = [&](f32x16_t* s, const Tile& t) {
-    const int key0 = t.key0, x = t.page;
-    if ((x & 15) == 15 && !needs_mask(a, w_lo, w_hi, key0, TK)) return;   // one test in most steps
-    mask_keys(a, s[0], me.p, w_lo, w_hi, key0, hi, x & 1, x & 2);
-    mask_keys(a, s[1], me.p, w_lo, w_hi, key0 + 32, hi, x & 4, x & 8);
+  auto mask = [&](int i, f32x16_t* s, const Tile& t) {
+    const int x = t.page, g0 = (pc.begin + i) * 4;
+    if ((x & 31) == 31 && !needs_mask(a, w_lo, w_hi, t.key0, TK)) return;   // one test in most steps
+    mask_keys(a, s[0], me.p, u.key_of(g0), u.key_of(g0 + 1), hi, x & 1, x & 2);
+    mask_keys(a, s[1], me.p, u.key_of(g0 + 2), u.key_of(g0 + 3), hi, x & 4, x & 8);
   };
   auto exps = [&](const f32x16_t* s, V8* pb, float m_use) {
     float rs = 0.f;
@@ -965,7 +959,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           for (int r = 0; r < 16; ++r) o[dt][r] *= al;   // O holds P V up to t-1 now
       }
     }
-    if constexpr (decltype(hasS)::value) mask(s_next, x[1]);
+    if constexpr (decltype(hasS)::value) mask(t + 1, s_next, x[1]);
 #pragma unroll
     for (int i = 0; i < DK; ++i) x[i] = x[i + 1];
   };
@@ -978,10 +972,28 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     if (i < DK - 2 && i < cnt) issue_v(i, x[i]);
   }
   __builtin_amdgcn_s_waitcnt(0);
+  if (wave * 32 >= u.nrows) {
+    // a wave without rows (single tokens, a request's last rows) only copies, in step with the others
+    auto copy = [&](auto v, int i) {
+      constexpr bool V = decltype(v)::value;
+      const int k = u.key_of((pc.begin + i) * 4 + wave);
+      int slot = 0, e = Copy::seen(a, u, k) ? cp.entry(Copy::page_of(a, k, slot)) : -1;
+      if (!Copy::is_page(a, e)) e = -1;
+      cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, e, slot, k, e >= 0 && Copy::whole(a, u, k, 16));
+    };
+    if (cnt > 0) __builtin_amdgcn_s_barrier();
+    for (int t = 0; cnt > 0 && t <= cnt; ++t) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      if (t + DK < cnt) copy(std::integral_constant<bool, false>(), t + DK);
+      if (t + DK - 2 < cnt) copy(std::integral_constant<bool, true>(), t + DK - 2);
+    }
+    return;
+  }
   if (cnt > 0) {
     __builtin_amdgcn_s_barrier();
     compute_s(0, sa);
-    mask(sa, x[0]);
+    mask(0, sa, x[0]);
     if (cnt > 1) iter(0, sb, sa, pb, pa, yes(), no(), yes());
     else iter(0, sb, sa, pb, pa, no(), no(), yes());
     int t = 1;
