@@ -650,10 +650,10 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
 // The pieces' sums joined: 32 rows and 32 dims of a split row tile per workgroup.  A thread adds 4 dims of one row over every J-th
 // piece (J as many threads as there are for an item), then the J sums are added in LDS; always in the same
 // order.  Wave 0 looks up what the workgroup joins (mostly nothing).
-constexpr int join_threads(int M) { return M == 32 ? 256 : 512; }
+constexpr int kJoinThreads = 256;
 template <typename T, int D, int M>
-__global__ __launch_bounds__(join_threads(M)) void combine_kernel(PagedKArgs a) {
-  constexpr int QW = M / 32, NV = D / 32, NT = join_threads(M), AHEAD = 8;
+__global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
+  constexpr int QW = M / 32, NV = D / 32, NT = kJoinThreads, AHEAD = M == 32 ? 8 : 16;
   constexpr bool FEW = M == 32;
   __shared__ float4 part[NT];
   __shared__ float2 ml[NT];
@@ -1051,44 +1051,41 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
   constexpr int NW = kPlanThreads / 64;
   constexpr int kHeld = 8192;                      // row tiles whose key tiles are kept in LDS
   __shared__ int base[kMaxRequests + 1], tiles[kHeld];
-  __shared__ int wsum[3][NW];
+  __shared__ int wsum[3][NW], wmax[NW], falls;
   __shared__ float wtot[NW], cost[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  // inclusive prefix sums over the workgroup of three values, held at 2^30; sums of all in all[]
-  auto sum = [](int x, int y) { return (int)min((unsigned)x + (unsigned)y, 1u << 30); };
-  auto scan = [&](int (&x)[3], int (&all)[3], int n) {
-    for (int k = 0; k < n; ++k)
-      for (int o = 1; o < 64; o <<= 1) {
-        const int p = __shfl_up(x[k], o, 64);
-        if (lane >= o) x[k] = sum(x[k], p);
-      }
-    __syncthreads();
-    if (lane == 63)
-      for (int k = 0; k < n; ++k) wsum[k][wave] = x[k];
-    __syncthreads();
-    for (int k = 0; k < n; ++k) {
-      int before = 0;
-      all[k] = 0;
-      for (int w = 0; w < NW; ++w) {
-        if (w == wave) before = all[k];
-        all[k] = sum(all[k], wsum[k][w]);
-      }
-      x[k] = sum(x[k], before);
+  // inclusive prefix sum over the workgroup; the sum of all in `all`.  Barriers by the caller: one before and one after wsum[k]
+  // is written
+  auto upto = [&](int k, int x, int& all) {
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      before = w == wave ? all : before;
+      all += wsum[k][w];
     }
+    return x + before;
   };
+  if (tid == 0) falls = 0;
+  __syncthreads();
   int R = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
-    int n = 0;
-    if (b < a.B) n = max(lengths_of(a, b).n, 0);
-    n = min((int)(((int64_t)n * a.G + M - 1) / M), max_pairs);
-    int x[3] = {n, 0, 0}, all[3];
-    scan(x, all, 1);
-    if (b < a.B) base[b] = min(R + x[0] - n, max_pairs);
-    R = min(sum(R, all[0]), max_pairs);            // more only for row numbers that do not rise
+    int n = b < a.B ? lengths_of(a, b).n : 0;
+    if (n < 0) falls = 1;                          // row numbers that fall: no row is written
+    n = n > 0 ? (n * a.G + M - 1) / M : 0;
+    const int x = wave_prefix(n);
+    if (b0) __syncthreads();
+    if (lane == 63) wsum[0][wave] = x;
+    __syncthreads();
+    int all;
+    const int at = R + upto(0, x, all) - n;
+    if (b < a.B) base[b] = at;
+    R += all;
   }
   if (tid == 0) base[a.B] = R;
   __syncthreads();
+  if (falls) R = 0;
   float total = 0.f;                               // an estimate: its rounding does not matter
   int longest = 1;
   for (int i = tid; i < R; i += kPlanThreads) {
@@ -1109,13 +1106,14 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
   for (int o = 32; o > 0; o >>= 1) longest = max(longest, __shfl_xor(longest, o, 64));
   if (lane == 0) {
     wtot[wave] = total;
-    wsum[0][wave] = longest;
+    wmax[wave] = longest;
   }
   __syncthreads();
   total = 0.f;
+#pragma unroll
   for (int w = 0; w < NW; ++w) {
     total += wtot[w];
-    longest = max(longest, wsum[0][w]);
+    longest = max(longest, wmax[w]);
   }
   const float W = total * (float)a.Hk;
   auto chunk_of = [&](int i) { return chunk_choice(i, longest, W, (float)R * (float)a.Hk, (float)slots); };
@@ -1127,32 +1125,44 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
       n += np;
       sp += np > 1 ? np : 0;
     }
-    n = wave_sum_i(n);
-    sp = wave_sum_i(sp);
+    n = wave_prefix(n);
+    sp = wave_prefix(sp);
     float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, (float)sp * (float)a.Hk);
     if (wave > 0 && (n > max_pieces || (int64_t)sp * a.Hk > max_parts)) t = INFINITY;
-    if (lane == 0) cost[wave] = t;
+    if (lane == 63) cost[wave] = t;
   }
   __syncthreads();
   int best = 0;
-  for (int w = 1; w < NW; ++w)
-    if (cost[w] < cost[best]) best = w;
+  float least = cost[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    const float t = cost[w];
+    best = t < least ? w : best;
+    least = fminf(t, least);
+  }
   const int c = chunk_of(best);
   int N = 0, S = 0, Q = 0;
   for (int i0 = 0; i0 < R; i0 += kPlanThreads) {
     const int i = i0 + tid;
     const int4 pr = i < R ? pairs[i] : make_int4(0, 0, 0, 0);
     const int np = i < R ? parts_of(pr.z, c) : 0, sp = np > 1 ? np : 0;
-    int x[3] = {np, sp, sp > 0}, all[3];
-    scan(x, all, 3);
+    const int x0 = wave_prefix(np), x1 = wave_prefix(sp), x2 = wave_prefix(sp > 0);
+    if (i0) __syncthreads();
+    if (lane == 63) {
+      wsum[0][wave] = x0;
+      wsum[1][wave] = x1;
+      wsum[2][wave] = x2;
+    }
+    __syncthreads();
+    int all0, all1, all2;
+    const int n0 = N + upto(0, x0, all0) - np, s0 = S + upto(1, x1, all1) - sp, q = Q + upto(2, x2, all2) - 1;
     if (i < R) {
-      const int n0 = N + x[0] - np, s0 = S + x[1] - sp;
-      if (sp) splits[Q + x[2] - 1] = make_int4(pr.x, pr.y, np, s0);
+      if (sp) splits[q] = make_int4(pr.x, pr.y, np, s0);
       for (int j = 0; j < np; ++j) pieces[n0 + j] = make_int4(pr.x, pr.y, j * c, sp ? s0 + j : -1);
     }
-    N += all[0];
-    S += all[1];
-    Q += all[2];
+    N += all0;
+    S += all1;
+    Q += all2;
   }
   if (tid == 0) {
     head[0] = N;
@@ -1205,7 +1215,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
     k.slots = few_slots(D);
     few_kernel<T, D, PAGED, kFewWaves><<<k.slots, 64 * kFewWaves, 0, s>>>(k);
     if (int rc = fs_host::launch_status(fn)) return rc;
-    combine_kernel<T, D, 32><<<(k.slots - 1) * (D / 32), join_threads(32), 0, s>>>(k);
+    combine_kernel<T, D, 32><<<(k.slots - 1) * (D / 32), kJoinThreads, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   if (plan) {
@@ -1222,7 +1232,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
   many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4 * (D / 32)), join_threads(128), 0, s>>>(k);
+    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4 * (D / 32)), kJoinThreads, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;

@@ -10,7 +10,11 @@
 //
 // One pass over q, k and v.  A workgroup takes a few tokens: their angles, one
 // per (token, pair), go to LDS once and serve every head; then each thread moves
-// 16-byte pieces (both of a pair's pieces where they are apart).
+// 16-byte pieces (both of a pair's pieces where they are apart).  A thread keeps its
+// place in the head and goes from head to head, so that no piece costs a
+// division (found by one, the pieces' places cost more than their bytes in the
+// interleaved layout, where a piece is 16 bytes and not two times 16).
+#include <algorithm>
 #include <climits>
 
 #include "common.h"
@@ -55,14 +59,29 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
 // V: elements of a piece, 16 bytes where every run of dims allows it, else 1.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
+  constexpr bool TWO = !INTER || V == 1;           // a pair's elements are apart: two loads, two stores
   const fs_rope_args& a = ka.a;
   __shared__ float2 cs[kRopeMaxTokens * kRopeMaxHalf];
+  __shared__ int64_t place[kRopeMaxTokens][2];     // a token's rows in the caches; -1: it has none
+  __shared__ int taken[kRopeMaxTokens];            // 0: a row behind the last request
   const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * ka.tokens, nt = min(ka.tokens, a.T - t0);
+  const int64_t t0 = (int64_t)blockIdx.x * ka.tokens;
+  const int nt = (int)min((int64_t)ka.tokens, a.T - t0);
   auto pos_of = [&](int t) -> int64_t {
     return a.pos_bytes == 8 ? static_cast<const int64_t*>(a.positions)[t0 + t]
                             : (int64_t)static_cast<const int32_t*>(a.positions)[t0 + t];
   };
+  if (tid < nt) {
+    taken[tid] = pos_of(tid) >= 0;
+    if (a.slots != nullptr) {
+      const int64_t slot = a.slots[t0 + tid];
+      const bool ok = slot >= 0 && slot < a.num_pages * a.page_size;
+      const int64_t page = !ok ? 0 : slot <= INT_MAX ? (uint32_t)slot / (uint32_t)a.page_size : slot / a.page_size;
+      const int64_t off = slot - page * a.page_size;
+      place[tid][0] = ok ? page * a.kc_sp + off * a.kc_ss : -1;
+      place[tid][1] = ok ? page * a.vc_sp + off * a.vc_ss : -1;
+    }
+  }
   for (int i = tid; i < nt * a.half; i += kRopeThreads) {
     const int t = i / a.half;
     double turns = (double)pos_of(t) * a.inv_freq[i - t * a.half] * 0.15915494309189533577;   // 1 / (2 pi)
@@ -75,93 +94,100 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
   // pieces of a rotated head: one per pair of pieces (half layout) or per piece
   // (interleaved; single elements: per pair), then the dims that are copied
   const int rot = INTER ? (V > 1 ? 2 * a.half / V : a.half) : a.half / V;
-  const int head = rot + (a.D - 2 * a.half) / V, vhead = a.D / V;
-  const int rotated = (a.Hq + a.Hk) * head, token = rotated + (a.v != nullptr ? a.Hk * vhead : 0);
-  for (int i = tid; i < nt * token; i += kRopeThreads) {
-    const int tl = i / token, it = i - tl * token;
-    const int64_t t = t0 + tl;
-    if (pos_of(tl) < 0) continue;                  // a row behind the last request
-    int64_t page = 0, off = 0;
-    if (a.slots != nullptr && it >= a.Hq * head) {
-      const int64_t slot = a.slots[t];
-      page = slot / a.page_size;
-      off = slot - page * a.page_size;
-      if (slot < 0 || page >= a.num_pages) continue;   // no place in the cache
+  const int head = rot + (a.D - 2 * a.half) / V;
+  const int apart = INTER ? 1 : a.half;            // elements between a pair's two loads
+  // The rows of nt tokens of `rows` heads, `pieces` threads to a row: run(token, head, piece).  The workgroups of one
+  // token (gridDim.y) share its rows, v's from the last one on.
+  const int parts = gridDim.y, part = blockIdx.y;
+  auto each = [&](int rows, int pieces, int part, auto&& run) {
+    const int side = pieces < kRopeThreads ? kRopeThreads / pieces : 1;   // rows side by side
+    const int mine = pieces < kRopeThreads ? tid / pieces : 0;
+    if (mine >= side) return;
+    for (int c = tid - mine * pieces; c < pieces; c += kRopeThreads) {
+      int t = 0, h = mine + part * side;
+      while (true) {
+        while (h >= rows) {
+          h -= rows;
+          ++t;
+        }
+        if (t >= nt) break;
+        if (taken[t]) run(t, h, c);
+        h += parts * side;
+      }
     }
+  };
+  each(a.Hq + a.Hk, head, part, [&](int t, int h, int c) {
+    const bool turn = c < rot;
+    const int d = turn ? (INTER ? c * (V > 1 ? V : 2) : c * V) : 2 * a.half + (c - rot) * V;
     const T* src;
     T* dst;
-    int c;
-    bool turn = true;
-    if (it < rotated) {
-      const int h = it / head;
-      c = it - h * head;
-      turn = c < rot;
-      if (h < a.Hq) {
-        src = static_cast<const T*>(a.q) + t * a.q_st + h * a.q_sh;
-        dst = static_cast<T*>(a.q_out) + t * a.qo_st + h * a.qo_sh;
+    if (h < a.Hq) {
+      src = static_cast<const T*>(a.q) + (t0 + t) * a.q_st + h * a.q_sh + d;
+      dst = static_cast<T*>(a.q_out) + (t0 + t) * a.qo_st + h * a.qo_sh + d;
+    } else {
+      h -= a.Hq;
+      src = static_cast<const T*>(a.k) + (t0 + t) * a.k_st + h * a.k_sh + d;
+      if (a.slots != nullptr) {
+        const int64_t at = place[t][0];
+        if (at < 0) return;                        // no place in the cache
+        dst = static_cast<T*>(a.k_cache) + at + h * a.kc_sh + d;
       } else {
-        const int hk = h - a.Hq;
-        src = static_cast<const T*>(a.k) + t * a.k_st + hk * a.k_sh;
-        dst = a.slots != nullptr ? static_cast<T*>(a.k_cache) + page * a.kc_sp + off * a.kc_ss + hk * a.kc_sh
-                                 : static_cast<T*>(a.k_out) + t * a.ko_st + hk * a.ko_sh;
+        dst = static_cast<T*>(a.k_out) + (t0 + t) * a.ko_st + h * a.ko_sh + d;
       }
-    } else {
-      const int hk = (it - rotated) / vhead;
-      c = it - rotated - hk * vhead;
-      turn = false;
-      src = static_cast<const T*>(a.v) + t * a.v_st + hk * a.v_sh;
-      dst = static_cast<T*>(a.v_cache) + page * a.vc_sp + off * a.vc_ss + hk * a.vc_sh;
     }
-    const float2* w = cs + tl * a.half;
+    float x1[V], y1[V];
+    load_piece<T, V>(src, x1);
     if (!turn) {
-      const int d = it < rotated ? 2 * a.half + (c - rot) * V : c * V;
-      float x[V];
-      load_piece<T, V>(src + d, x);
-      store_piece<T, V>(dst + d, x);
-    } else if constexpr (INTER) {
-      constexpr int P = V > 1 ? V : 2;
-      float x[P], y[P];
-      if constexpr (V > 1) load_piece<T, V>(src + c * V, x);
-      else {
-        x[0] = to_f32(src[2 * c]);
-        x[1] = to_f32(src[2 * c + 1]);
-      }
-#pragma unroll
-      for (int e = 0; e < P / 2; ++e) {
-        const float2 f = w[c * (P / 2) + e];
-        y[2 * e] = x[2 * e] * f.x - x[2 * e + 1] * f.y;
-        y[2 * e + 1] = x[2 * e + 1] * f.x + x[2 * e] * f.y;
-      }
-      if constexpr (V > 1) store_piece<T, V>(dst + c * V, y);
-      else {
-        dst[2 * c] = Conv<T>::store(y[0]);
-        dst[2 * c + 1] = Conv<T>::store(y[1]);
-      }
-    } else {
-      float x1[V], x2[V], y1[V], y2[V];
-      load_piece<T, V>(src + c * V, x1);
-      load_piece<T, V>(src + a.half + c * V, x2);
+      store_piece<T, V>(dst, x1);
+      return;
+    }
+    if constexpr (TWO) {
+      const float2* w = cs + t * a.half + c * V;
+      float x2[V], y2[V];
+      load_piece<T, V>(src + apart, x2);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float2 f = w[c * V + e];
+        const float2 f = w[e];
         y1[e] = x1[e] * f.x - x2[e] * f.y;
         y2[e] = x2[e] * f.x + x1[e] * f.y;
       }
-      store_piece<T, V>(dst + c * V, y1);
-      store_piece<T, V>(dst + a.half + c * V, y2);
+      store_piece<T, V>(dst, y1);
+      store_piece<T, V>(dst + apart, y2);
+    } else {
+      const float2* w = cs + t * a.half + c * (V / 2);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        const float2 f = w[e];
+        y1[2 * e] = x1[2 * e] * f.x - x1[2 * e + 1] * f.y;
+        y1[2 * e + 1] = x1[2 * e + 1] * f.x + x1[2 * e] * f.y;
+      }
+      store_piece<T, V>(dst, y1);
     }
-  }
+  });
+  if (a.v == nullptr) return;
+  each(a.Hk, a.D / V, parts - 1 - part, [&](int t, int h, int c) {
+    const int64_t at = place[t][1];
+    if (at < 0) return;
+    float x[V];
+    load_piece<T, V>(static_cast<const T*>(a.v) + (t0 + t) * a.v_st + h * a.v_sh + c * V, x);
+    store_piece<T, V>(static_cast<T*>(a.v_cache) + at + h * a.vc_sh + c * V, x);
+  });
 }
 
 template <typename T>
 static int launch_rope(const fs_rope_args& a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  RopeKArgs k{a, a.T >= 2048 ? kRopeMaxTokens : 1};
-  const unsigned grid = (unsigned)((a.T + k.tokens - 1) / k.tokens);
   const bool wide = a.D % V == 0 && (a.interleaved ? 2 * a.half : a.half) % V == 0;
   auto f = a.interleaved ? (wide ? rope_kernel<T, V, true> : rope_kernel<T, 1, true>)
                          : (wide ? rope_kernel<T, V, false> : rope_kernel<T, 1, false>);
-  f<<<grid, kRopeThreads, 0, s>>>(k);
+  // Long calls: 2 tokens to a workgroup, 4 where a piece is 16 bytes (32768 tokens, half: 126 us against 131 with 4; 8191
+  // interleaved, half of the head: 29.7 against 32.0 with 2).  Few tokens: their heads over several workgroups, so that a
+  // thread has one piece to wait for.
+  RopeKArgs k{a, a.T < 2048 ? 1 : a.interleaved ? 4 : 2};
+  const int pieces = (wide && a.interleaved ? 2 * a.half / V : wide ? a.half / V : a.half) + (a.D - 2 * a.half) / (wide ? V : 1);
+  const int side = std::max(kRopeThreads / pieces, 1);
+  const int parts = a.T >= 1024 ? 1 : std::min((a.Hq + a.Hk + side - 1) / side, 16);
+  f<<<dim3((a.T + k.tokens - 1) / k.tokens, parts), kRopeThreads, 0, s>>>(k);
   return fs_host::launch_status("fs_rope");
 }
 
@@ -179,7 +205,7 @@ extern "C" int fs_rope(const fs_rope_args* a, void* stream) {
   FS_CHECK_SUPPORTED(a->half <= kRopeMaxHalf && a->D <= 512 && a->D % 8 == 0,
                      "fs_rope: head_dim %d, rotary dim %d unsupported (multiples of 8 up to 512, up to %d)", a->D,
                      2 * a->half, 2 * kRopeMaxHalf);
-  FS_CHECK_SUPPORTED((int64_t)(a->Hq + 2 * (int64_t)a->Hk) * a->D <= (1 << 22), "fs_rope: %d + %d heads unsupported",
+  FS_CHECK_SUPPORTED((a->Hq + 2 * (int64_t)a->Hk) * a->D <= (1 << 20), "fs_rope: %d + %d heads unsupported",
                      a->Hq, a->Hk);
   if (a->T == 0) return FS_OK;
   FS_CHECK_ARG(a->q && a->k && a->q_out && a->positions && a->inv_freq, "fs_rope: null tensor pointer");
