@@ -16,7 +16,9 @@
 // forms the prefix sums by itself (B <= 4096 lengths: 32 KiB from L2) instead of
 // waiting for one that does, any number of workgroups shares the tokens, and a
 // call repeated on the same inputs writes the same values.
+#include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "common.h"
 
@@ -24,28 +26,49 @@ namespace fs {
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxRequests = 4096;
-constexpr int kPlanTokensPerGroup = 1024;
 constexpr int kPlanMaxGroups = 256;
+constexpr uint32_t kMost = INT_MAX;                // sums stop here
 
+__device__ __forceinline__ uint32_t sum(uint32_t x, uint32_t y) { return min(x + y, kMost); }
+
+// A request's step; everything fits 32 bits (P * page_size < 2^31).
 struct PlanReq {
-  int64_t l0, l1;
-  int n, p0, p1;
+  uint32_t l0, l1, n, p0, p1;
+  __device__ __forceinline__ PlanReq(const fs_plan_args& a, int b) {
+    const uint32_t ps = a.page_size, cap = (uint32_t)a.P * ps;
+    const int d = a.new_lens[b];
+    l0 = min((uint32_t)max(a.seq_lens[b], 0), cap);
+    n = max(d, 0);
+    l1 = d >= 0 ? l0 + n : l0 - min(l0, 0u - (uint32_t)d);
+    p0 = pages(l0, ps);
+    p1 = min(pages(l1, ps), (uint32_t)a.P);
+  }
+  static __device__ __forceinline__ uint32_t pages(uint32_t tokens, uint32_t ps) {
+    const uint32_t q = tokens / ps;
+    return q + (q * ps != tokens);
+  }
+  __device__ __forceinline__ uint32_t grow() const { return p1 > p0 ? p1 - p0 : 0; }
+  __device__ __forceinline__ uint32_t give() const { return p0 > p1 ? p0 - p1 : 0; }
 };
 
-__device__ __forceinline__ PlanReq plan_req(const fs_plan_args& a, int b) {
-  PlanReq r;
-  const int64_t cap = (int64_t)a.P * a.page_size;
-  r.l0 = min(max((int64_t)a.seq_lens[b], (int64_t)0), cap);
-  const int64_t d = a.new_lens[b];
-  r.l1 = max(r.l0 + d, (int64_t)0);
-  r.n = (int)max(d, (int64_t)0);
-  r.p0 = (int)((r.l0 + a.page_size - 1) / a.page_size);
-  r.p1 = (int)min((r.l1 + a.page_size - 1) / a.page_size, (int64_t)a.P);
-  return r;
+// Inclusive prefix sum over the wave, held at kMost.
+__device__ __forceinline__ uint32_t wave_upto(uint32_t x) {
+  auto from = [&](auto ctrl, auto rows) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+#define FS_STEP(ctrl, rows) x = sum(x, from(std::integral_constant<int, ctrl>(), std::integral_constant<int, rows>()))
+  FS_STEP(0x111, 0xf);                             // row_shr 1, 2, 4, 8: rows of 16 lanes
+  FS_STEP(0x112, 0xf);
+  FS_STEP(0x114, 0xf);
+  FS_STEP(0x118, 0xf);
+  FS_STEP(0x142, 0xa);                             // row_bcast 15, 31: the rows below
+  FS_STEP(0x143, 0xc);
+#undef FS_STEP
+  return x;
 }
 
 // Largest b with cum[b] <= x, for an exclusive prefix cum[0..B] with cum[B] > x.
-__device__ __forceinline__ int owner(const int* cum, int B, int x) {
+__device__ __forceinline__ int owner(const uint32_t* cum, int B, uint32_t x) {
   int lo = 0, hi = B;                              // cum[lo] <= x < cum[hi]
   while (hi - lo > 1) {
     const int m = (lo + hi) >> 1;
@@ -56,119 +79,120 @@ __device__ __forceinline__ int owner(const int* cum, int B, int x) {
 }
 
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(fs_plan_args a) {
-  // exclusive prefixes of new tokens, pages needed and pages given back; the
-  // sums are formed in 64 bits and held at most at INT_MAX
-  extern __shared__ int lds[];
-  int* cu = lds;
-  int* go = cu + a.B + 1;
-  int* ro = go + a.B + 1;
-  __shared__ int64_t part[3][kPlanThreads / 64];
-  __shared__ int64_t lost_part[kPlanThreads / 64];
+  constexpr int NW = kPlanThreads / 64;
+  // exclusive prefix sums of new tokens, pages needed and pages given back, and each request's tokens and pages before
+  extern __shared__ uint32_t lds[];
+  uint32_t *cu = lds, *go = cu + a.B + 1, *ro = go + a.B + 1, *l0 = ro + a.B + 1, *p0 = l0 + a.B;
+  __shared__ uint32_t part[3][NW], lost_part[NW];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (a.B + kPlanThreads - 1) / kPlanThreads;
   const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
-  int64_t s[3] = {0, 0, 0};
+  const int fc = min(max(a.free_count[0], 0), a.F);
+  uint32_t s[3] = {0, 0, 0};
   for (int b = b0; b < b1; ++b) {
-    const PlanReq r = plan_req(a, b);
-    s[0] += r.n;
-    s[1] += max(r.p1 - r.p0, 0);
-    s[2] += max(r.p0 - r.p1, 0);
+    const PlanReq r(a, b);
+    l0[b] = r.l0;
+    p0[b] = r.p0;
+    cu[b] = r.n;                                   // until the sums are known
+    go[b] = r.l1;
+    ro[b] = r.p1;
+    s[0] = sum(s[0], r.n);
+    s[1] = sum(s[1], r.grow());
+    s[2] = sum(s[2], r.give());
   }
-  int64_t inc[3];
+  uint32_t at[3], tot[3];
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    inc[i] = s[i];
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(inc[i], o, 64);
-      if (lane >= o) inc[i] += v;
-    }
-    if (lane == 63) part[i][wave] = inc[i];
+    const uint32_t x = wave_upto(s[i]);
+    if (lane == 63) part[i][wave] = x;
+    at[i] = __builtin_amdgcn_update_dpp(0, (int)x, 0x138, 0xf, 0xf, false);   // wave_shr 1: the lanes below
   }
   __syncthreads();
-  int64_t pos[3], tot[3];
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
-    int64_t before = 0, all = 0;
+    uint32_t before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
-      if (w < wave) before += part[i][w];
-      all += part[i][w];
+    for (int w = 0; w < NW; ++w) {
+      before = w == wave ? all : before;
+      all = sum(all, part[i][w]);
     }
-    pos[i] = before + inc[i] - s[i];
+    at[i] = sum(at[i], before);
     tot[i] = all;
   }
-  auto cap = [](int64_t v) { return (int)min(v, (int64_t)INT_MAX); };
-  const int fc = min(max(a.free_count[0], 0), a.F);
-  const int avail = (int)min((int64_t)fc + tot[2], (int64_t)a.F);
-  int64_t lost = 0;
+  const uint32_t avail = min(sum(fc, tot[2]), (uint32_t)a.F), ps = a.page_size;
+  uint32_t lost = 0;
   for (int b = b0; b < b1; ++b) {
-    const PlanReq r = plan_req(a, b);
-    cu[b] = cap(pos[0]);
-    go[b] = cap(pos[1]);
-    ro[b] = cap(pos[2]);
-    const int64_t grow = max(r.p1 - r.p0, 0);
-    const int64_t got = min(max((int64_t)avail - pos[1], (int64_t)0), grow);
-    lost += max(r.l1 - max(r.l0, (r.p0 + got) * a.page_size), (int64_t)0);
+    const uint32_t n = cu[b], l1 = go[b], q0 = p0[b], q1 = ro[b], grow = q1 > q0 ? q1 - q0 : 0;
+    const uint32_t got = min(avail > at[1] ? avail - at[1] : 0, grow), held = max(l0[b], (q0 + got) * ps);
+    lost = sum(lost, l1 > held ? min(l1 - held, kMost) : 0);
     if (blockIdx.x == 0) {
-      a.cu_lens[b] = cap(pos[0]);
-      a.seq_lens_out[b] = cap(r.l1);
+      a.cu_lens[b] = at[0];
+      a.seq_lens_out[b] = min(l1, kMost);
     }
-    pos[0] += r.n;
-    pos[1] += grow;
-    pos[2] += max(r.p0 - r.p1, 0);
+    cu[b] = at[0];
+    go[b] = at[1];
+    ro[b] = at[2];
+    at[0] = sum(at[0], n);
+    at[1] = sum(at[1], grow);
+    at[2] = sum(at[2], q0 > q1 ? q0 - q1 : 0);
   }
   if (tid == 0) {
-    cu[a.B] = cap(tot[0]);
-    go[a.B] = cap(tot[1]);
-    ro[a.B] = cap(tot[2]);
+    cu[a.B] = tot[0];
+    go[a.B] = tot[1];
+    ro[a.B] = tot[2];
   }
-  if (blockIdx.x == 0) {
-    for (int o = 32; o > 0; o >>= 1) lost += __shfl_xor(lost, o, 64);
-    if (lane == 0) lost_part[wave] = lost;
-  }
+  lost = wave_upto(lost);
+  if (lane == 63) lost_part[wave] = lost;
   __syncthreads();
   if (blockIdx.x == 0 && tid == 0) {
-    int64_t l = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) l += lost_part[w];
-    a.cu_lens[a.B] = cap(tot[0]);
-    a.lacking[0] = cap(l);
-    a.free_count_out[0] = (int)max((int64_t)avail - tot[1], (int64_t)0);
+    uint32_t l = 0;
+    for (int w = 0; w < NW; ++w) l = sum(l, lost_part[w]);
+    a.cu_lens[a.B] = tot[0];
+    a.lacking[0] = l;
+    a.free_count_out[0] = avail > tot[1] ? avail - tot[1] : 0;
   }
-  const int total = cu[a.B], grown = go[a.B], given = ro[a.B];
+  // pages that request b keeps or comes to (one of the two sums stands still)
+  auto pages_after = [&](int b) { return p0[b] + (go[b + 1] - go[b]) - (ro[b + 1] - ro[b]); };
   // entry r of the pages given back: its owner's row of the table, above what the owner keeps
-  auto given_page = [&](int r) {
+  auto given_page = [&](uint32_t r) {
     const int b = owner(ro, a.B, r);
-    return a.block_table[(int64_t)b * a.t_sb + plan_req(a, b).p1 + r - ro[b]];
+    return a.block_table[(int64_t)b * a.t_sb + pages_after(b) + r - ro[b]];
   };
   // the g-th page taken, -1 past the stack's end
-  auto taken_page = [&](int g) {
-    const int at = avail - 1 - g;
-    if (at < 0) return -1;
-    return at < fc ? a.free_pages[at] : given_page(at - fc);
+  auto taken_page = [&](uint32_t g) {
+    if (g >= avail) return -1;
+    const uint32_t k = avail - 1 - g;
+    return k < (uint32_t)fc ? a.free_pages[k] : given_page(k - fc);
   };
-  const int step = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
-  for (int j = first; j < a.T; j += step) {
-    int p = -1;
-    int64_t slot = -1;
-    if (j < total) {
-      const int b = owner(cu, a.B, j);
-      const PlanReq r = plan_req(a, b);
-      const int64_t at = r.l0 + (j - cu[b]);
-      const int64_t pg = at / a.page_size;
-      int page = -1;
-      if (pg < r.p0) page = a.block_table[(int64_t)b * a.t_sb + pg];
-      else if (pg < r.p1) page = taken_page(go[b] + (int)pg - r.p0);
-      p = cap(at);
-      if (page >= 0) slot = (int64_t)page * a.page_size + at % a.page_size;
+  // The tokens, the pages taken and those given back are one list of items: few threads have more than one, so
+  // their searches and loads wait side by side.
+  const uint32_t T = a.T;
+  const uint64_t items = (uint64_t)T + tot[1] + tot[2];
+  for (uint64_t x = (uint64_t)blockIdx.x * kPlanThreads + tid; x < items; x += (uint64_t)gridDim.x * kPlanThreads) {
+    if (x < T) {
+      const uint32_t j = (uint32_t)x;
+      int p = -1;
+      int64_t slot = -1;
+      if (j < tot[0]) {
+        const int b = owner(cu, a.B, j);
+        const uint32_t pos = l0[b] + (j - cu[b]), pg = pos / ps;   // below 2^32
+        int page = -1;
+        if (pg < p0[b]) page = a.block_table[(int64_t)b * a.t_sb + pg];
+        else if (pg < pages_after(b)) page = taken_page(go[b] + pg - p0[b]);
+        p = min(pos, kMost);
+        if (page >= 0) slot = (int64_t)page * ps + (pos - pg * ps);
+      }
+      a.positions[j] = p;
+      a.slots[j] = slot;
+    } else if (x - T < tot[1]) {
+      const uint32_t g = (uint32_t)(x - T);
+      const int b = owner(go, a.B, g);
+      a.block_table[(int64_t)b * a.t_sb + p0[b] + g - go[b]] = taken_page(g);
+    } else {
+      const uint32_t r = (uint32_t)(x - T - tot[1]);
+      if (fc + r < (uint32_t)a.F) a.free_pages[fc + r] = given_page(r);
     }
-    a.positions[j] = p;
-    a.slots[j] = slot;
   }
-  for (int64_t g = first; g < grown; g += step) {
-    const int b = owner(go, a.B, (int)g);
-    a.block_table[(int64_t)b * a.t_sb + plan_req(a, b).p0 + (int)g - go[b]] = taken_page((int)g);
-  }
-  for (int64_t r = first; r < given && fc + r < a.F; r += step) a.free_pages[fc + r] = given_page((int)r);
 }
 
 }  // namespace fs
@@ -185,8 +209,11 @@ extern "C" int fs_plan(const fs_plan_args* a, void* stream) {
   FS_CHECK_ARG(a->page_size >= 1 && (int64_t)a->P * a->page_size <= INT_MAX && a->t_sb >= a->P,
                "fs_plan: page size %d, table of %d pages with row stride %lld", a->page_size, a->P, (long long)a->t_sb);
   FS_CHECK_SUPPORTED(a->B <= kPlanMaxRequests, "fs_plan: %d requests > %d", a->B, kPlanMaxRequests);
-  const int groups = min(max((a->T + kPlanTokensPerGroup - 1) / kPlanTokensPerGroup, 1), kPlanMaxGroups);
-  const size_t bytes = 3 * (size_t)(a->B + 1) * sizeof(int);
+  // an item to a thread, with some for the pages that change hands
+  const int64_t items = (int64_t)a->T + a->T / a->page_size + a->B;
+  const int groups = (int)std::min<int64_t>((items + kPlanThreads - 1) / kPlanThreads, kPlanMaxGroups);
+  const size_t bytes = (5 * (size_t)a->B + 3) * sizeof(uint32_t);
+  if (int rc = fs_host::allow_dynamic_lds(plan_kernel, bytes, "fs_plan")) return rc;
   plan_kernel<<<groups, kPlanThreads, bytes, (hipStream_t)stream>>>(*a);
   return fs_host::launch_status("fs_plan");
 }
