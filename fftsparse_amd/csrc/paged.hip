@@ -43,7 +43,7 @@ namespace fs {
 constexpr int kFewWaves = FEW_WAVES;                // of a workgroup of few_kernel
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
 constexpr int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
-constexpr int kLeastTiles = 2;                      // of a workgroup of few_kernel
+constexpr int kLeastTiles = 1;                      // of a workgroup of few_kernel
 constexpr int kPartsMany = 1024;                    // split pieces that the workspace holds
 constexpr int kMaxRequests = 4096;
 constexpr int kPlanThreads = 1024;
@@ -129,11 +129,13 @@ struct GroupCopy {
   const uint16_t *kp, *vp;
   const int32_t* row;                              // of the table
   int page;                                        // contiguous: the request
-  __device__ __forceinline__ GroupCopy(const PagedKArgs& a, int b, int hk, int lane) {
+  __device__ __forceinline__ void place(const PagedKArgs& a, int b, int hk) {
     row = PAGED ? a.table + b * a.t_sb : nullptr;
     page = b;
     kp = a.k + hk * a.k_sh;
     vp = a.v + hk * a.v_sh;
+  }
+  __device__ __forceinline__ GroupCopy(const PagedKArgs& a, int lane) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int r = RPR * i + (lane >> LCPR);
@@ -452,63 +454,86 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
   constexpr int RING = 4 * TILE;                   // of a wave: two K tiles, two V tiles
   constexpr int NI = 2 * Copy::NI;                 // copies of 32 keys
   __shared__ __attribute__((aligned(1024))) char lds[NW * RING];
+  __shared__ float2 ml[NW][64];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   char* ring = lds + wave * RING;
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
   const Ranges<32, 32 * NW> ranges(a, gridDim.x);
   const int first = blockIdx.x * ranges.per, end = min(first + ranges.per, ranges.W);
-  for (int pos = first; pos < end;) {
-    const auto at = ranges.find(pos);
-    const int begin = pos - at.start, count = min(at.start + at.nt, end) - pos;
-    // where the sums of a part go: a range's first piece or, not starting with it, its last
-    const int slot = count == at.nt ? -1 : 2 * blockIdx.x + (pos != first);
-    pos += count;
-    const RowTile u = row_tile<32, 32 * NW>(a, at.x, at.rt);
-    const LaneRow me = lane_row(a, u, l32);
-    const Copy cp(a, at.b, at.hk, lane);
-    V8 qf[D / 16];
-    load_q<V8, D>(a, u, me, at.b, at.hk, hi, qf);
+  if (first >= end) return;
 
-    // this wave's two groups of keys of each of the piece's tiles: the first one's place among those visited
-    auto group_of = [&](int i) { return (begin + i) * (2 * NW) + 2 * wave; };
-    int cnt = min(count, u.nt - begin);
-    if (cnt > 0 && u.key_of(group_of(cnt - 1)) >= u.kend) --cnt;   // the last tile ends before this wave's keys
-    // pages of the two groups of a step's keys (-1: none) and the keys' slots there
-    struct Ent {
-      int e[2], slot[2];
-    };
-    auto load_ent = [&](int i) {
-      Ent x{{-1, -1}, {0, 0}};
+  // A piece: a row tile, or the part of its keys that lies in the range.
+  struct Seg {
+    int hk, b, begin, cnt, slot;                   // slot: where a part's sums go (-1: the whole row tile)
+    RowTile u;
+    LaneRow me;
+  } sg;
+  V8 qf[D / 16];
+  Copy cp(a, lane);
+  // pages of the two groups of a step's keys (-1: none) and the keys' slots there
+  struct Ent {
+    int e[2], slot[2];
+  } x0, x1, x2;
+  // this wave's two groups of keys of each of the piece's tiles: the first one's place among those visited
+  auto group_of = [&](int i) { return (sg.begin + i) * (2 * NW) + 2 * wave; };
+  auto load_ent = [&](int i) {
+    Ent x{{-1, -1}, {0, 0}};
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int k = u.key_of(group_of(i) + g);
-        if (i < cnt && Copy::seen(a, u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, x.slot[g]));
-      }
-      return x;
-    };
-    auto there = [&](Ent& x) {                     // looked at a step after it is loaded
+    for (int g = 0; g < 2; ++g) {
+      const int k = sg.u.key_of(group_of(i) + g);
+      if (i < sg.cnt && Copy::seen(a, sg.u, k)) x.e[g] = cp.entry(Copy::page_of(a, k, x.slot[g]));
+    }
+    return x;
+  };
+  auto there = [&](Ent& x) {                     // looked at a step after it is loaded
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (!Copy::is_page(a, x.e[g])) x.e[g] = -1;
-    };
-    auto issue = [&](auto v, int i, const Ent& x) {
-      constexpr bool V = decltype(v)::value;
-      const uint32_t at = ring0 + ((V ? 2 : 0) + (i & 1)) * TILE;
+    for (int g = 0; g < 2; ++g)
+      if (!Copy::is_page(a, x.e[g])) x.e[g] = -1;
+  };
+  auto issue = [&](auto v, int i, const Ent& x) {
+    constexpr bool V = decltype(v)::value;
+    const uint32_t at = ring0 + ((V ? 2 : 0) + (i & 1)) * TILE;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int k = u.key_of(group_of(i) + g);
-        cp.template issue<V>(a, u, at + g * TILE / 2, x.e[g], x.slot[g], k, x.e[g] >= 0 && Copy::whole(a, u, k, 16));
-      }
-    };
-    auto issue_k = [&](int i, const Ent& x) { issue(std::integral_constant<bool, false>(), i, x); };
-    auto issue_v = [&](int i, const Ent& x) { issue(std::integral_constant<bool, true>(), i, x); };
-    constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
-    const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
-    const int vrow = hi * 4 + ((lane & 15) >> 2);
-    const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
-                                       (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
-    const float sc = a.scale * kLog2e;
+    for (int g = 0; g < 2; ++g) {
+      const int k = sg.u.key_of(group_of(i) + g);
+      cp.template issue<V>(a, sg.u, at + g * TILE / 2, x.e[g], x.slot[g], k, x.e[g] >= 0 && Copy::whole(a, sg.u, k, 16));
+    }
+  };
+  auto issue_k = [&](int i, const Ent& x) { issue(std::integral_constant<bool, false>(), i, x); };
+  auto issue_v = [&](int i, const Ent& x) { issue(std::integral_constant<bool, true>(), i, x); };
+  // Begins the piece at tile pos: its rows of Q and its first two K tiles are requested.  Returns its tiles.
+  auto open = [&](int pos) {
+    const auto at = ranges.find(pos);
+    const int count = min(at.start + at.nt, end) - pos;
+    sg.hk = at.hk;
+    sg.b = at.b;
+    sg.begin = pos - at.start;
+    sg.slot = count == at.nt ? -1 : 2 * blockIdx.x + (pos != first);   // a range's first piece or, not starting with it, its last
+    sg.u = row_tile<32, 32 * NW>(a, at.x, at.rt);
+    sg.me = lane_row(a, sg.u, l32);
+    sg.cnt = min(count, sg.u.nt - sg.begin);
+    if (sg.cnt > 0 && sg.u.key_of(group_of(sg.cnt - 1)) >= sg.u.kend) --sg.cnt;   // the last tile ends before this wave's keys
+    cp.place(a, sg.b, sg.hk);
+    load_q<V8, D>(a, sg.u, sg.me, sg.b, sg.hk, hi, qf);
+    x0 = load_ent(0);
+    x1 = load_ent(1);
+    x2 = load_ent(2);
+    there(x0);
+    there(x1);
+    if (sg.cnt > 0) issue_k(0, x0);
+    if (sg.cnt > 1) issue_k(1, x1);
+    return count;
+  };
+  constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM;
+  const uint32_t k_lane = (uint32_t)(l32 * ROWB + ((hi ^ ((D == 128 ? l32 : l32 >> 1) & SWM)) << 4));
+  const int vrow = hi * 4 + ((lane & 15) >> 2);
+  const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
+                                     (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
+  const float sc = a.scale * kLog2e;
+  int pos = first;
+  pos += open(pos);
+  while (true) {
     float m_run = -INFINITY, l_run = 0.f;
     f32x16_t o[D / 32];
 #pragma unroll
@@ -516,23 +541,16 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
 
-    // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this
-    // order; K(i+2) and V(i+2) are requested as soon as their place is read.
-    Ent x0 = load_ent(0), x1 = load_ent(1), x2 = load_ent(2);
-    there(x0);
-    there(x1);
-    if (cnt > 0) {
-      issue_k(0, x0);
-      issue_v(0, x0);
-    }
-    if (cnt > 1) {
-      issue_k(1, x1);
-      issue_v(1, x1);
-    }
-    __builtin_amdgcn_s_waitcnt(0);                   // Q's loads too: the loop's waits then count copies only
-    for (int i = 0; i < cnt; ++i) {
-      if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
-      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+    // Copies on their way at the top of step i: K(i), V(i), K(i+1), V(i+1), in this order (step 0: K(0), K(1), V(0), V(1));
+    // K(i+2) and V(i+2) are requested as soon as their place is read.
+#pragma unroll
+    for (int st = 0; st < D / 16; ++st) asm volatile("" : "+v"(qf[st]));   // Q is here: the loop's waits count copies only
+    if (sg.cnt > 0) issue_v(0, x0);
+    if (sg.cnt > 1) issue_v(1, x1);
+    for (int i = 0; i < sg.cnt; ++i) {
+      if (i + 1 >= sg.cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+      else if (i == 0) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
       const char* kt = ring + (i & 1) * TILE;
       f32x16_t s;
 #pragma unroll
@@ -541,14 +559,14 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
       for (int st = 0; st < D / 16; ++st) s = Ops::mma(__builtin_bit_cast(V8, lds16(kt, k_lane ^ (uint32_t)(st << 5))), qf[st], s);
       there(x2);
       const Ent x3 = load_ent(i + 3);
-      if (i + 2 < cnt) {
+      if (i + 2 < sg.cnt) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         issue_k(i + 2, x2);
       }
       {
-        const int k0 = u.key_of(group_of(i)), k1 = u.key_of(group_of(i) + 1);
-        if (x0.e[0] < 0 || x0.e[1] < 0 || k1 != k0 + 16 || needs_mask(a, u.p_lo, u.p_hi, k0, 32))
-          mask_keys(a, s, me.p, k0, k1, hi, x0.e[0] >= 0, x0.e[1] >= 0);
+        const int k0 = sg.u.key_of(group_of(i)), k1 = sg.u.key_of(group_of(i) + 1);
+        if (x0.e[0] < 0 || x0.e[1] < 0 || k1 != k0 + 16 || needs_mask(a, sg.u.p_lo, sg.u.p_hi, k0, 32))
+          mask_keys(a, s, sg.me.p, k0, k1, hi, x0.e[0] >= 0, x0.e[1] >= 0);
       }
       float mx = s[0], h0, h1;
 #pragma unroll
@@ -577,9 +595,10 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[dt][r] *= al;
       }
-      if (i + 2 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
-      else if (i + 1 < cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (i + 1 >= sg.cnt) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      else if (i == 0 && i + 2 >= sg.cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+      else if (i == 0 || i + 2 >= sg.cnt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * NI) : "memory");
       const char* vt = ring + (2 + (i & 1)) * TILE;
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
@@ -588,7 +607,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
           const uint32_t lo = (v_lane ^ (uint32_t)(dt << 6)) + kk * 16 * ROWB;
           o[dt] = Ops::mma(__builtin_bit_cast(V8, join8(lds_tr8(vt, lo), lds_tr8(vt, lo + 8 * ROWB))), pb[kk], o[dt]);
         }
-      if (i + 2 < cnt) {
+      if (i + 2 < sg.cnt) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         issue_v(i + 2, x2);
       }
@@ -596,32 +615,35 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
       x1 = x2;
       x2 = x3;
     }
-    // ---- the waves' sums joined through LDS, wave w taking dims 32 w, 32 (w + NW) ..
+    // ---- the waves' sums joined through LDS (the V tiles' place), wave w taking dims 32 w, 32 (w + NW) ..; the next piece's
+    // first copies go out before
     constexpr int NV = D / 32;
-    float* own = reinterpret_cast<float*>(ring);     // [D / 32][4][64 lanes] 4 floats, then m and l
+    constexpr int SUMS = 2 * TILE;                 // of a wave's ring: [D / 32][4][64 lanes] 4 floats
+    static_assert(NV * 4 * 64 * 16 == 2 * TILE, "the sums take the place of two V tiles");
 #pragma unroll
     for (int dt = 0; dt < NV; ++dt)
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4)
-        reinterpret_cast<float4*>(own)[(dt * 4 + g4) * 64 + lane] =
+        reinterpret_cast<float4*>(ring + SUMS)[(dt * 4 + g4) * 64 + lane] =
             make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
-    constexpr int ML = NV * 4 * 64 * 4;
-    own[ML + lane] = m_run;
-    own[ML + 64 + lane] = l_run;
+    ml[wave][lane] = make_float2(m_run, l_run);
+    const LaneRow me = sg.me;
+    const int slot = sg.slot;
+    uint16_t* op = out_row(a, sg.u, me, sg.b, sg.hk);
+    const bool more = pos < end;
+    if (more) pos += open(pos);
     __syncthreads();
     if (me.on) {
       float m = -INFINITY, l = 0.f, f[NW];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) m = fmaxf(m, reinterpret_cast<const float*>(lds + w * RING)[ML + lane]);
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w][lane].x);
       const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float* x = reinterpret_cast<const float*>(lds + w * RING) + ML;
-        f[w] = __builtin_amdgcn_exp2f(x[lane] - mu);
-        l += x[64 + lane] * f[w];
+        f[w] = __builtin_amdgcn_exp2f(ml[w][lane].x - mu);
+        l += ml[w][lane].y * f[w];
       }
       const float inv = l != 0.f ? 1.0f / l : 0.f;
-      uint16_t* op = out_row(a, u, me, at.b, at.hk);
 #pragma unroll
       for (int dt = wave; dt < NV; dt += NW)
 #pragma unroll
@@ -629,7 +651,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int w = 0; w < NW; ++w) {
-            const float4 x = reinterpret_cast<const float4*>(lds + w * RING)[(dt * 4 + g4) * 64 + lane];
+            const float4 x = reinterpret_cast<const float4*>(lds + w * RING + SUMS)[(dt * 4 + g4) * 64 + lane];
             acc.x += x.x * f[w];
             acc.y += x.y * f[w];
             acc.z += x.z * f[w];
@@ -643,7 +665,8 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
         a.part_ml[(int64_t)slot * 64 + 32 + l32] = l;
       }
     }
-    __syncthreads();                               // the rings are read: the next row tile's copies may come
+    if (!more) return;
+    __syncthreads();                               // the sums are read: V tiles may come
   }
 }
 
@@ -785,7 +808,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // positions of this wave's first and last row
   const int w_lo = u.L - u.n + (u.r0 + min(wave * 32, max(u.nrows, 1) - 1)) / a.G;
   const int w_hi = u.L - u.n + (u.r0 + min(wave * 32 + 31, max(u.nrows, 1) - 1)) / a.G;
-  const Copy cp(a, pc.b, pc.hk, lane);
+  Copy cp(a, lane);
+  cp.place(a, pc.b, pc.hk);
   const int cnt = min(pc.count, u.nt - pc.begin);
   // A tile's place: its first key (the first of this wave's group, where the tile's keys are not one run), and, kept as one
   // number, the page of the group that this wave copies (group w of each tile), whether the tile is one run of keys that

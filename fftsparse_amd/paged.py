@@ -104,9 +104,9 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype, Hk=None, D=None):
     return want, _written(k, "k_cache", want, dtype), _written(v, "v_cache", want, dtype)
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    return a0 < b0 + b.numel() * b.element_size() and b0 < a0 + a.numel() * a.element_size()
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    p = t.data_ptr()
+    return p, p + t.numel() * t.element_size()
 
 
 @dataclass
@@ -160,7 +160,9 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
                 _ints(out.slots, "out.slots", (num_tokens,), (torch.int64,)),
                 _ints(out.free_count, "out.free_count", (1,)), _ints(out.lacking, "out.lacking", (1,))]
         _lib.same_device(t, *outs)
-        if any(_overlap(o, i) for o in outs for i in (seq_lens, new_lens, free_pages, free_count, t)):
+        read = [_span(x) for x in (seq_lens, new_lens, free_pages, free_count)]
+        read.append((t.data_ptr(), t.data_ptr() + 4 * ((B - 1) * t_sb + P)))
+        if any(lo < end and start < hi for lo, hi in map(_span, outs) for start, end in read):
             raise ValueError("out shares storage with an input of the step: the lengths and the free count of a step "
                              "are read while its result is written")
     _lib.call("fs_plan", PlanArgs(
