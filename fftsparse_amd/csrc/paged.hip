@@ -9,20 +9,30 @@
 // `sinks`; groups of 16 keys in between are not visited, and a key tile is four groups of the
 // others in a row (the first tokens cost a group, not a tile).
 //
-// Pieces.  A row tile's keys are taken in pieces of at most `chunk` key tiles by
-// workgroups of their own where that fills the GPU better (plan_in_wave, from the
-// lengths on the device); the pieces' unnormalised sums are then joined by
-// combine_kernel, in an order of their own.
+// few_kernel (calls whose requests have at most 32 rows per KV head: single tokens) is bound by
+// the cache being read.  256 workgroups (512 at head dim 64) take equal runs of all the call's key tiles
+// (Ranges), so that they end together whatever the lengths are.  Each of a workgroup's 4
+// waves streams keys of its own, 32 at a time, through a ring of two LDS tiles that
+// only it uses: no barrier in the loop, and 24 to 32 KiB per wave are always on their way
+// (96 KiB and more per CU).  S^T = K Q^T, P in registers, O^T += V^T P on
+// v_mfma_f32_32x32x16, of which a single token uses G of 32 columns (about a tenth of the
+// MFMA rate is taken); V is read transposed from LDS as it is stored.  Measured
+// (bf16, D = 128, 32 / 8 heads): 32 requests of 16384 tokens 5.3 TB/s, 64 of 64 - 8192 4.4 TB/s,
+// one of 131072 4.7 TB/s; a copy of 4 GiB takes 4.9 TB/s on the same card.
 //
-// few_kernel (row tiles of at most 32 rows: single tokens) is bound by the cache
-// being read.  Each of its 4 waves streams keys of its own, 32 at a time, through
-// a ring of two LDS tiles that only it uses: no barrier, so 24 to 32 KiB per wave
-// are always on their way (96 KiB and more per CU).  S^T = K Q^T, P in registers, O^T += V^T P
-// on v_mfma_f32_32x32x16; V is read transposed from LDS as it is stored.
+// many_kernel (tiles of 128 rows) is bound by MFMA: 4 waves of 32 rows share tiles of 64 keys,
+// two tiles deep: S of the next tile and P V of the last one are interleaved with the
+// exponentials of the current one.  A row tile's keys are taken in several pieces
+// where that fills the GPU better (plan_pieces_kernel, from the lengths on the device).  Measured: 2048 new
+// tokens over 32768 1.09 PFLOP/s; an 8192^3 GEMM takes 1.18 on the same card.
 //
-// many_kernel (128 rows) is bound by MFMA: 4 waves of 32 rows share tiles of 64 keys, two
-// tiles deep, as in bsattn_kernel: S of the next tile and P V of the last one are
-// interleaved with the exponentials of the current one.
+// Both leave the unnormalised sums of a row tile that was cut in the workspace, in
+// 32 bits, with each row's maximum and sum; combine_kernel joins them, in an order that
+// depends on the lengths only.
+//
+// Rounding: scores, maxima, sums and O are in 32 bits; P is rounded to the input type for the
+// second product (its relative error, at most half a step of the type, averages out over the keys as the
+// values' own does), and the row sum adds the rounded P, so that weights add up to one.
 //
 // Groups of 16 keys are never split by a page (its size is a multiple of 16): a
 // copy of one is addressed by one entry of the table.  A group that not all rows
@@ -37,10 +47,7 @@
 
 namespace fs {
 
-#ifndef FEW_WAVES
-#define FEW_WAVES 4
-#endif
-constexpr int kFewWaves = FEW_WAVES;                // of a workgroup of few_kernel
+constexpr int kFewWaves = 4;                        // of a workgroup of few_kernel
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
 constexpr int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
 constexpr int kLeastTiles = 1;                      // of a workgroup of few_kernel
@@ -795,10 +802,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   using Copy = GroupCopy<D, PAGED>;
   constexpr int TK = 64, TILE = TK * D * 2;        // bytes of a K or V tile
   constexpr int ROWB = Copy::ROWB, SWM = Copy::SWM, GB = 16 * ROWB;
-  // K tiles ahead (V: DK - 2): 64 KiB of LDS either way, so two workgroups share a CU.  A tile of head dim 64 is consumed in half
-  // the time, in which its copies' latency has to fit.
-  constexpr int DK = 2;
-  __shared__ __attribute__((aligned(1024))) char lds[2][DK][TILE];   // [K, V][buffer]
+  // 64 KiB, so two workgroups share a CU (four tiles deep at head dim 64, in as much: 47.8 us against 44.8 for a batch of
+  // windows)
+  __shared__ __attribute__((aligned(1024))) char lds[2][2][TILE];   // [K, V][buffer]
   Piece pc;
   if (!find_piece(a, pc)) return;
   const RowTile u = row_tile<128, TK>(a, lengths_of(a, pc.b), pc.rt);
@@ -864,7 +870,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)&lds[0][0][0]) + wave * GB;
   auto issue = [&](auto v, int i, const Tile& x) {
     constexpr bool V = decltype(v)::value;
-    cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, x.page >> 5, x.slot, x.key0,
+    cp.template issue<V>(a, u, lds0 + ((V ? 2 : 0) + (i & 1)) * TILE, x.page >> 5, x.slot, x.key0,
                          (x.page & 31) == 31);
   };
   auto issue_k = [&](int i, const Tile& x) { issue(std::integral_constant<bool, false>(), i, x); };
@@ -925,28 +931,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
                          pb[kk], o[dt]);
       }
   };
-  // Step t: wait for K(t+1) and V(t-1), one barrier, copy K(t+DK) over K(t) and V(t+DK-2) over V(t-2); then S(t+1) and
+  // Step t: wait for K(t+1) and V(t-1), one barrier, copy K(t+2) over K(t) and V(t) over V(t-2); then S(t+1) and
   // P V(t-1) on MFMA between the exponentials of tile t; then O's rescale (rare) and the masks of tile t+1.
   f32x16_t sa[2], sb[2];
   V8 pa[4], pb[4];
-  Tile x[DK + 1];                                  // of tiles t .. t+DK, the last one packed from
+  Tile x[3];                                       // of tiles t .. t+2, the last one packed from
   Raw raw;                                         // its entries
   typedef std::integral_constant<bool, true> yes;
   typedef std::integral_constant<bool, false> no;
   auto iter = [&](int t, f32x16_t* s_next, f32x16_t* s_cur, V8* p_prev, V8* p_cur, auto hasS, auto hasPV, auto hasE) {
     __builtin_amdgcn_s_setprio(0);
-    // the copies of the last DK - 2 steps may stay on their way (there are as many unless the end is near)
-    if (DK > 2 && t - 1 + DK < cnt) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((DK - 2) * 2 * Copy::NI) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    x[DK] = pack(raw);
-    if (t + DK < cnt) issue_k(t + DK, x[DK]);
-    if (t + DK - 2 < cnt) issue_v(t + DK - 2, x[DK - 2]);
-    raw = load_raw(t + DK + 1);
+    x[2] = pack(raw);
+    if (t + 2 < cnt) issue_k(t + 2, x[2]);
+    if (t < cnt) issue_v(t, x[0]);
+    raw = load_raw(t + 3);
     __builtin_amdgcn_s_setprio(2);
     float rs = 0.f, al = 1.0f;
-    if constexpr (decltype(hasS)::value) compute_s((t + 1) & (DK - 1), s_next);
-    if constexpr (decltype(hasPV)::value) pv_mma((t - 1) & (DK - 1), p_prev);
+    if constexpr (decltype(hasS)::value) compute_s((t + 1) & 1, s_next);
+    if constexpr (decltype(hasPV)::value) pv_mma((t - 1) & 1, p_prev);
     if constexpr (decltype(hasE)::value) {
       float mx = s_cur[0][0], m0, m1;
 #pragma unroll
@@ -984,33 +988,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     if constexpr (decltype(hasS)::value) mask(t + 1, s_next, x[1]);
-#pragma unroll
-    for (int i = 0; i < DK; ++i) x[i] = x[i + 1];
+    x[0] = x[1];
+    x[1] = x[2];
   };
-#pragma unroll
-  for (int i = 0; i < DK; ++i) x[i] = pack(load_raw(i));
-  raw = load_raw(DK);
-#pragma unroll
-  for (int i = 0; i < DK; ++i) {
-    if (i < cnt) issue_k(i, x[i]);
-    if (i < DK - 2 && i < cnt) issue_v(i, x[i]);
-  }
+  x[0] = pack(load_raw(0));
+  x[1] = pack(load_raw(1));
+  raw = load_raw(2);
+  if (cnt > 0) issue_k(0, x[0]);
+  if (cnt > 1) issue_k(1, x[1]);
   __builtin_amdgcn_s_waitcnt(0);
   if (wave * 32 >= u.nrows) {
-    // a wave without rows (single tokens, a request's last rows) only copies, in step with the others
+    // A wave without rows (beside a single token, a request's last rows) only copies, in step with the others.  (The same for the
+    // steps in which a wave's rows see nothing, at a window's edges, spilled registers in the loop: 5-25% slower.)
     auto copy = [&](auto v, int i) {
       constexpr bool V = decltype(v)::value;
       const int k = u.key_of((pc.begin + i) * 4 + wave);
       int slot = 0, e = Copy::seen(a, u, k) ? cp.entry(Copy::page_of(a, k, slot)) : -1;
       if (!Copy::is_page(a, e)) e = -1;
-      cp.template issue<V>(a, u, lds0 + ((V ? DK : 0) + (i & (DK - 1))) * TILE, e, slot, k, e >= 0 && Copy::whole(a, u, k, 16));
+      cp.template issue<V>(a, u, lds0 + ((V ? 2 : 0) + (i & 1)) * TILE, e, slot, k, e >= 0 && Copy::whole(a, u, k, 16));
     };
     if (cnt > 0) __builtin_amdgcn_s_barrier();
     for (int t = 0; cnt > 0 && t <= cnt; ++t) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
-      if (t + DK < cnt) copy(std::integral_constant<bool, false>(), t + DK);
-      if (t + DK - 2 < cnt) copy(std::integral_constant<bool, true>(), t + DK - 2);
+      if (t + 2 < cnt) copy(std::integral_constant<bool, false>(), t + 2);
+      if (t < cnt) copy(std::integral_constant<bool, true>(), t);
     }
     return;
   }
@@ -1325,7 +1327,7 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
                "%s: B=%d T=%d P=%d num_pages=%lld max_new=%d", fn, a->B, a->T, a->P, (long long)a->num_pages, a->max_new);
   FS_CHECK_SUPPORTED(a->page_size >= 16 && a->page_size <= 4096 && a->page_size % 16 == 0,
                      "%s: page size %d unsupported (multiples of 16 up to 4096)", fn, a->page_size);
-  FS_CHECK_SUPPORTED(a->num_pages < (1 << 27), "%s: %lld pages unsupported", fn, (long long)a->num_pages);
+  FS_CHECK_SUPPORTED(a->num_pages < (1 << 26), "%s: %lld pages unsupported", fn, (long long)a->num_pages);
   FS_CHECK_SUPPORTED((int64_t)a->P * a->page_size <= (1 << 26), "%s: %d pages of %d tokens per request unsupported",
                      fn, a->P, a->page_size);
   if (a->T == 0) return FS_OK;

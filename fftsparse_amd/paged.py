@@ -207,7 +207,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     request has, if the caller knows it (1 in a decoding step); the result is right
     for any value, the right one is faster.  Rows behind cu_lens[B] are left as
     they were (unset in a new tensor).  A page number outside the cache holds no
-    token; a row that sees no token is 0."""
+    token; a row that sees no token is 0.  Slots that no row sees may hold anything;
+    a value of v that is not finite may reach rows of its request that do not see
+    it.  ``out`` may be q.  Up to 4096 requests of 2^26 tokens."""
     q, qs = _rows(q, "q")
     T, Hq, D = q.shape
     _attn_dtype(q, k_cache, v_cache)

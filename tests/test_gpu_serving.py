@@ -175,6 +175,31 @@ def test_strided_queries_and_output():
     b.check(b.gpu(q=odd[..., 1:129]))
 
 
+@pytest.mark.parametrize("lens", [DECODE, CHUNKS], ids=["decode", "chunks"])
+def test_output_in_the_queries_place_and_a_wide_table(lens):
+    b = Batch(lens, ps=48, seed=22)
+    want = b.gpu()
+    q = b.q.to(DEV)
+    wide = torch.full((b.table.shape[0], b.table.shape[1] + 9), 5, dtype=I32, device=DEV)
+    wide[:, 4:-5] = b.table.to(DEV)
+    got = fa.paged_attention(q, b.kc.to(DEV), b.vc.to(DEV), wide[:, 4:-5], b.cu.to(DEV), _i32(b.total), out=q)
+    assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    x = torch.randn(1, 4, 700, 128, generator=torch.Generator().manual_seed(2)).to(BF).to(DEV)
+    k = torch.randn(1, 2, 700, 128, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
+    want = fa.window_attention(x, k, k, window=90, sinks=4)
+    assert torch.equal(fa.window_attention(x, k, k, window=90, sinks=4, out=x.transpose(1, 2)), want)
+
+
+def test_row_numbers_that_fall_write_nothing():
+    b = Batch([(100, 1), (60, 40), (3, 1)], seed=23)
+    for cu in ([0, 5, 2, 42], [0, 1, -7, 42], [40, 0, 41, 42]):
+        for max_new in (None, 1):
+            out = torch.full(b.q.shape, 7.0, dtype=BF, device=DEV)
+            fa.paged_attention(b.q.to(DEV), b.kc.to(DEV), b.vc.to(DEV), b.table.to(DEV), _i32(cu), _i32(b.total), max_new=max_new,
+                               out=out)
+            assert bool((out == 7.0).all())
+
+
 @pytest.mark.parametrize("max_new", [None, 1])
 def test_pages_outside_the_cache_hold_no_token(max_new):
     lens = [(700, 1), (10, 1), (200, 30), (100, 1)]

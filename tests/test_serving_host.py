@@ -4,12 +4,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import re
 
 import pytest
 import torch
 
 import fftsparse_amd as fa
 from fftsparse_amd import _lib
+from tests.test_isa_hazards import CSRC, HIPCC, _compile
 
 BF = torch.bfloat16
 
@@ -151,7 +153,8 @@ def test_c_abi_refuses_without_a_launch():
                              (-1, "16-byte", dict(q=8)), (-1, "multiples of 8", dict(k_ss=100)),
                              (-1, "null tensor", dict(work=None)), (-1, "4-byte", dict(cu_lens=18)),
                              (-1, "row stride", dict(t_sb=3)), (-1, "num_pages=0", dict(num_pages=0)),
-                             (-2, "rows of", dict(T=1 << 29))]:
+                             (-2, "rows of", dict(T=1 << 29)), (-2, "67108864 pages", dict(num_pages=1 << 26)),
+                             (-2, "4097 requests", dict(B=4097)), (-2, "slot stride", dict(v_ss=1 << 23))]:
         got, said = _rc("fs_paged_attn", paged(), **change)
         assert (got, text in said) == (rc, True), (change, got, said)
     assert _rc("fs_paged_attn", paged(), T=0)[0] == 0                     # no token: nothing to do
@@ -221,3 +224,38 @@ def test_frequencies_agree_with_transformers(scaling, extra, head_dim, base):
                                           length=length, device="cpu", **extra)
     assert math.isclose(got_factor, want_factor, rel_tol=1e-6)
     assert torch.allclose(got.float(), want, rtol=16 * 2.0 ** -24 * math.log(base) * 2, atol=0)
+
+
+def _paged_bytes(T, B, max_new=0, Hq=32, Hk=8, D=128):
+    a = _lib.PagedAttnArgs(dtype=1, B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=64, page_size=64, max_new=max_new)
+    return _lib.load().fs_paged_attn_work_bytes(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("Hq,Hk,D", [(32, 8, 128), (28, 4, 64), (4, 1, 128), (32, 32, 64)])
+def test_workspaces_never_fall(Hq, Hk, D):
+    """One sized for the largest step serves every smaller one."""
+    sizes = sorted({n + d for n in (1, 8, 32, 33, 64, 256, 4096, 100000) for d in (-1, 0, 1) if n + d > 0})
+    for B in (1, 8, 256, 4096):
+        for m in (0, 1, 8, 100):
+            n = [_paged_bytes(T, B, m, Hq, Hk, D) for T in sizes]
+            assert n == sorted(n) and n[0] > 0
+    for T in (1, 64, 5000):
+        n = [_paged_bytes(T, B, 1, Hq, Hk, D) for B in range(1, 4097, 13)]
+        assert n == sorted(n)
+        n = [_paged_bytes(T, 16, m, Hq, Hk, D) for m in [*range(1, 200), 0]]
+        assert n == sorted(n)
+    lib = _lib.load()
+    n = [lib.fs_window_attn_work_bytes(ctypes.byref(_lib.WindowAttnArgs(dtype=1, B=2, Hq=Hq, Hk=Hk, Lq=L, Lk=L, D=D, window=100)))
+         for L in sizes]
+    assert n == sorted(n) and n[0] > 0
+
+
+@pytest.mark.skipif(HIPCC is None, reason="hipcc is not installed")
+def test_paged_attention_spills_no_vector_registers(tmp_path):
+    """many_kernel's loop holds all that 256 registers can; a spilled one cost it a quarter of its rate."""
+    asm = _compile(CSRC / "paged.hip", tmp_path / "paged.s")
+    spills = {}
+    for meta in asm.split("  - .agpr_count:")[1:]:
+        spills[re.search(r"\.name: +(\S+)", meta)[1]] = int(re.search(r"\.vgpr_spill_count: +(\d+)", meta)[1])
+    assert sum("many_kernel" in n for n in spills) == sum("few_kernel" in n for n in spills) == 8
+    assert {n: s for n, s in spills.items() if s} == {}
