@@ -840,6 +840,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       x.slot += 16 * wave;
       return x;
     }
+    if (PAGED && x.all && x.slot == 0 && a.page_size <= 32) {
+      // four pages of 16 or two of 32, all below the request's last one
+      const int two = a.page_size >> 5;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x.e[g] = cp.entry(page + (g >> two));
+      x.slot = (16 * wave) & (a.page_size - 1);
+      return x;
+    }
     x.slot = 0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
