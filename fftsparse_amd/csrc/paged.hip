@@ -47,10 +47,9 @@
 
 namespace fs {
 
-constexpr int kFewWaves = 4;                        // of a workgroup of few_kernel
+constexpr int kFewWaves = 4;                        // of a workgroup of few_kernel (1 or 2, as many in all: 10% slower)
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
 constexpr int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
-constexpr int kLeastTiles = 1;                      // of a workgroup of few_kernel
 constexpr int kPartsMany = 1024;                    // split pieces that the workspace holds
 constexpr int kMaxRequests = 4096;
 constexpr int kPlanThreads = 1024;
@@ -386,7 +385,7 @@ struct Ranges {
     W1 = __builtin_amdgcn_readlane(upto, 63);
     W = W1 * a.Hk;
     const int sh = 31 - __builtin_clz(groups);
-    per = max((W + groups - 1) >> sh, kLeastTiles);
+    per = max((W + groups - 1) >> sh, 1);          // at least 2 or 4: one request of 1000 tokens 13.8, 17.2 us, not 12.2
   }
   // The row tile that tile `pos` (< W) of all belongs to: its first tile's place `start`, its key tiles nt.
   struct Place {
@@ -1230,8 +1229,9 @@ static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
   w.bytes = w.o + (size_t)w.max_parts * w.rows * D * 4;
   return w;
 }
-// Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.  few_kernel counts key tiles of
-// row tiles in 32 bits.
+// Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.  At 64 rows few_kernel reads the keys
+// twice: 16 tokens of one request of 2048 20 us against 33, but of 32 requests of 4096 201 against 117.  It counts key
+// tiles of row tiles in 32 bits.
 static bool few_rows(int64_t max_new, int G, int64_t T, int B, int Hk, int64_t keys) {
   return max_new * G <= 32 && (T * G / 32 + B) * Hk < (1ll << 30) / (keys / 32 + 2);
 }
