@@ -40,6 +40,7 @@
 // page that is none) is copied row by row, zeros in place of the rows that no row
 // of the tile sees: nothing stands there that could spoil a sum.
 #include <algorithm>
+#include <cmath>
 #include <climits>
 #include <type_traits>
 
@@ -449,6 +450,9 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // f16 holds weights down to 2^-24; taken 2^7 times as large they reach from 2^15 (past the slack) to 2^-31 of the
 // running maximum's weight
 template <typename T> constexpr float kBias = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
+// log2 e times the scale, above 0: a hidden key's -inf stays one.  (Scales below 0, whose sign would have to go into Q, made
+// single tokens 4% slower and are refused.)
+__device__ __forceinline__ float score_scale(const PagedKArgs& a) { return fmaxf(a.scale * kLog2e, 1e-30f); }
 constexpr float kSlack = 8.0f;                     // a row's running max is raised past 2^8 only: few rescales of O
 
 template <typename T, int D, bool PAGED, int NW>
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
   const int vrow = hi * 4 + ((lane & 15) >> 2);
   const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
                                      (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
-  const float sc = a.scale * kLog2e;
+  const float sc = score_scale(a);
   int pos = first;
   pos += open(pos);
   while (true) {
@@ -889,7 +893,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int vrow = hi * 4 + ((lane & 15) >> 2);
   const uint32_t v_lane = (uint32_t)(vrow * ROWB + (lane & 1) * 8 +
                                      (((((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) ^ v_swz<D>(vrow)) << 4));
-  const float sc = a.scale * kLog2e;
+  const float sc = score_scale(a);
   float m_run = -INFINITY, l_run = 0.f;
   f32x16_t o[D / 32];
 #pragma unroll
@@ -1289,12 +1293,13 @@ static int run(PagedKArgs k, int dtype, int D, bool few, bool plan, const Work& 
 using namespace fs;
 
 // checks that both entry points share
-static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int B, int window, int sinks, int64_t rows,
-                        const int64_t* strides, int ns, const void* const* ptrs, int np) {
+static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int B, int window, int sinks, float scale,
+                        int64_t rows, const int64_t* strides, int ns, const void* const* ptrs, int np) {
   FS_CHECK_ARG(Hq >= 1 && Hk >= 1 && Hq % Hk == 0, "%s: Hq=%d must be a multiple of Hk=%d", fn, Hq, Hk);
   FS_CHECK_SUPPORTED(D == 128 || D == 64, "%s: head_dim %d unsupported (64 or 128)", fn, D);
   FS_CHECK_SUPPORTED(dtype == FS_DTYPE_BF16 || dtype == FS_DTYPE_F16, "%s: dtype %d unsupported (bf16/f16)", fn, dtype);
   FS_CHECK_ARG(window >= 0 && sinks >= 0, "%s: window %d and sinks %d must not be negative", fn, window, sinks);
+  FS_CHECK_ARG(std::isfinite(scale) && scale >= 0.f, "%s: softmax_scale %g must be finite and not negative", fn, scale);
   FS_CHECK_SUPPORTED(rows * Hq < (1ll << 30) && Hk <= 4096, "%s: %lld rows of %d heads unsupported", fn,
                      (long long)rows, Hq);
   FS_CHECK_SUPPORTED(B <= kMaxRequests, "%s: %d requests > %d", fn, B, kMaxRequests);
@@ -1341,7 +1346,9 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   if (a->T == 0) return FS_OK;
   const int64_t st[] = {a->q_st, a->q_sh, a->o_st, a->o_sh, a->k_sp, a->k_ss, a->k_sh, a->v_sp, a->v_ss, a->v_sh};
   const void* const ptrs[] = {a->q, a->out, a->k_cache, a->v_cache, a->work};
-  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, a->T, st, 10, ptrs, 5)) return rc;
+  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, a->softmax_scale, a->T, st, 10,
+                            ptrs, 5))
+    return rc;
   FS_CHECK_ARG(a->block_table && a->cu_lens && a->seq_lens && a->t_sb >= a->P &&
                    ((uintptr_t)a->block_table | (uintptr_t)a->cu_lens | (uintptr_t)a->seq_lens) % 4 == 0,
                "%s: block_table (row stride %lld of %d), cu_lens and seq_lens must be given, 4-byte aligned", fn,
@@ -1373,8 +1380,8 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   const int64_t st[] = {a->q_sb, a->q_sh, a->q_sl, a->k_sb, a->k_sh, a->k_sl,
                         a->v_sb, a->v_sh, a->v_sl, a->o_sb, a->o_sh, a->o_sl};
   const void* const ptrs[] = {a->q, a->out, a->k, a->v, a->work};
-  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, (int64_t)a->B * a->Lq, st, 12,
-                            ptrs, 5))
+  if (int rc = check_common(fn, a->dtype, a->D, a->Hq, a->Hk, a->B, a->window, a->sinks, a->softmax_scale,
+                            (int64_t)a->B * a->Lq, st, 12, ptrs, 5))
     return rc;
   FS_CHECK_SUPPORTED(a->k_sl >= 0 && a->k_sl < (1 << 23) && a->v_sl >= 0 && a->v_sl < (1 << 23),
                      "%s: row stride unsupported", fn);

@@ -183,6 +183,13 @@ def _window(window, sinks) -> tuple[int, int]:
     return int(window or 0), int(sinks)
 
 
+def _scale(scale, D: int) -> float:
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 <= scale < math.inf:
+        raise ValueError(f"softmax_scale must be finite and not negative, got {scale}")
+    return scale
+
+
 def _attn_dtype(*tensors) -> None:
     dt = tensors[0].dtype
     if dt not in (torch.bfloat16, torch.float16) or any(t.dtype != dt for t in tensors):
@@ -221,6 +228,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _ints(cu_lens, "cu_lens", (B + 1,))
     _ints(seq_lens, "seq_lens", (B,))
     window, sinks = _window(window, sinks)
+    scale = _scale(softmax_scale, D)
     if max_new is not None and int(max_new) < 1:
         raise ValueError(f"max_new must be at least 1, got {max_new}")
     _inference_only("paged_attention", q, k_cache, v_cache)
@@ -240,7 +248,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         block_table=t.data_ptr(), t_sb=t_sb, cu_lens=cu_lens.data_ptr(),
         seq_lens=seq_lens.data_ptr(), dtype=_lib.FS_DTYPE[q.dtype], B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=P, page_size=ps,
         num_pages=pages, max_new=0 if max_new is None else min(int(max_new), T), window=window, sinks=sinks,
-        softmax_scale=1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale))
+        softmax_scale=scale)
     work = torch.empty(_lib.load().fs_paged_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8, device=dev)
     args.work = work.data_ptr()
     _lib.call("fs_paged_attn", args, dev)
@@ -268,6 +276,7 @@ def window_attention(query_states: torch.Tensor, key_states: torch.Tensor, value
     if not (B and Lq and Lk):
         raise ValueError("empty sequence")
     window, sinks = _window(window, sinks)
+    scale = _scale(softmax_scale, D)
     _inference_only("window_attention", q, k, v)
     if out is None:
         out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
@@ -277,7 +286,7 @@ def window_attention(query_states: torch.Tensor, key_states: torch.Tensor, value
         q=q.data_ptr(), q_sb=qs[0], q_sh=qs[1], q_sl=qs[2], k=k.data_ptr(), k_sb=ks[0], k_sh=ks[1], k_sl=ks[2],
         v=v.data_ptr(), v_sb=vs[0], v_sh=vs[1], v_sl=vs[2], out=out.data_ptr(), o_sb=os_[0], o_sl=os_[1], o_sh=os_[2],
         dtype=_lib.FS_DTYPE[q.dtype], B=B, Hq=Hq, Hk=Hk, Lq=Lq, Lk=Lk, D=D, window=window, sinks=sinks,
-        softmax_scale=1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale))
+        softmax_scale=scale)
     work = torch.empty(_lib.load().fs_window_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8, device=dev)
     args.work = work.data_ptr()
     _lib.call("fs_window_attn", args, dev)

@@ -468,7 +468,7 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * at position p:
  *   out = softmax(q . k_s * scale) v over the tokens s <= p with s > p - window
  *         or s < sinks (window == 0: every s <= p),
- * for query head h on KV head h / (Hq / Hk).  A row that sees no token is 0;
+ * for query head h on KV head h / (Hq / Hk); scale finite, not negative.  A row that sees no token is 0;
  * rows past cu_lens[B] are left as they were.  A page outside 0 .. num_pages - 1
  * holds no token.  What stands in slots that no row sees (past a request's end,
  * wholly outside every window) is not used, be it nan; a value of v that is not

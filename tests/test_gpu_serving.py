@@ -145,6 +145,14 @@ def test_paged_attention_scale_and_repeat():
     assert torch.equal(x, b.gpu(softmax_scale=0.2))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-4])
+@pytest.mark.parametrize("lens", [DECODE, CHUNKS], ids=["decode", "chunks"])
+def test_scales_of_zero_and_near(lens, scale):
+    b = Batch(lens, seed=24)
+    b.check(b.gpu(softmax_scale=scale), scale=scale)
+    b.check(b.gpu(softmax_scale=scale, window=30, sinks=20), 30, 20, scale)
+
+
 def test_rows_behind_the_last_request_stay():
     for lens in (DECODE, CHUNKS):
         b = Batch(lens, pad=37, seed=6)
@@ -188,6 +196,26 @@ def test_output_in_the_queries_place_and_a_wide_table(lens):
     k = torch.randn(1, 2, 700, 128, generator=torch.Generator().manual_seed(3)).to(BF).to(DEV)
     want = fa.window_attention(x, k, k, window=90, sinks=4)
     assert torch.equal(fa.window_attention(x, k, k, window=90, sinks=4, out=x.transpose(1, 2)), want)
+
+
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_fewer_tokens_than_rows(max_new):
+    """A length below the number of new tokens: the first rows stand before the first token and are 0."""
+    b = Batch([(0, 9), (0, 70), (0, 1)], seed=25)
+    for take in ((4, 21, 0), (0, 69, 1)):
+        got = fa.paged_attention(b.q.to(DEV), b.kc.to(DEV), b.vc.to(DEV), b.table.to(DEV), b.cu.to(DEV), _i32(list(take)),
+                                 max_new=max_new)
+        for i, (L, (_, n)) in enumerate(zip(take, b.lens)):
+            want, mag = ref.attend(b.q[b.cu[i]:b.cu[i + 1]], b.k[i][:L], b.v[i][:L], L - n)
+            _check_attn(got[b.cu[i]:b.cu[i + 1]], want, mag, 100, BF, (take, i))
+            assert bool((got[b.cu[i]:b.cu[i] + n - L] == 0).all())
+
+
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_more_heads_to_a_group_than_rows_to_a_tile(max_new):
+    b = Batch([(0, 1), (200, 1), (70, 3)], Hq=300, Hk=1, D=64, seed=26)
+    b.check(b.gpu(max_new=max_new))
+    b.check(b.gpu(max_new=max_new, window=20, sinks=17), 20, 17)
 
 
 def test_row_numbers_that_fall_write_nothing():

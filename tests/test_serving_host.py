@@ -48,6 +48,8 @@ PAGED_BAD = [
     (ValueError, "window", dict(window=-3)),
     (ValueError, "sinks", dict(window=4, sinks=-1)),
     (ValueError, "max_new", dict(max_new=0)),
+    (ValueError, "softmax_scale", dict(softmax_scale=-0.1)),
+    (ValueError, "softmax_scale", dict(softmax_scale=math.nan)),
     (ValueError, "out must be", dict(out=torch.zeros(6, 4, 64, dtype=BF))),
     (ValueError, "broadcast", dict(out=torch.zeros(1, 4, 128, dtype=BF).expand(6, 4, 128))),
     (RuntimeError, "no backward", dict(q=torch.zeros(6, 4, 128, dtype=BF, requires_grad=True))),
@@ -66,6 +68,7 @@ def test_window_attention_refuses():
             (ValueError, "on the GPU", (q, k, k), dict(window=4)),
             (ValueError, "window", (q, k, k), dict(window=0)),
             (ValueError, "sinks", (q, k, k), dict(window=4, sinks=-1)),
+            (ValueError, "softmax_scale", (q, k, k), dict(window=4, softmax_scale=-1.0)),
             (TypeError, "bf16 or f16", (q.float(), k.float(), k.float()), dict(window=4)),
             (ValueError, "do not match", (q, k, k[:, :, :5]), dict(window=4)),
             (ValueError, "do not match", (q, k[..., :64], k[..., :64]), dict(window=4)),
@@ -154,7 +157,9 @@ def test_c_abi_refuses_without_a_launch():
                              (-1, "null tensor", dict(work=None)), (-1, "4-byte", dict(cu_lens=18)),
                              (-1, "row stride", dict(t_sb=3)), (-1, "num_pages=0", dict(num_pages=0)),
                              (-2, "rows of", dict(T=1 << 29)), (-2, "67108864 pages", dict(num_pages=1 << 26)),
-                             (-2, "4097 requests", dict(B=4097)), (-2, "slot stride", dict(v_ss=1 << 23))]:
+                             (-2, "4097 requests", dict(B=4097)), (-2, "slot stride", dict(v_ss=1 << 23)),
+                             (-1, "finite", dict(softmax_scale=math.nan)), (-1, "finite", dict(softmax_scale=math.inf)),
+                             (-1, "negative", dict(softmax_scale=-0.1))]:
         got, said = _rc("fs_paged_attn", paged(), **change)
         assert (got, text in said) == (rc, True), (change, got, said)
     assert _rc("fs_paged_attn", paged(), T=0)[0] == 0                     # no token: nothing to do
