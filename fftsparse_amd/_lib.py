@@ -224,19 +224,19 @@ def same_device(*tensors) -> torch.device:
     """The one GPU that every given tensor (None entries skipped) lives on.
     The kernels dereference the tensors' pointers on that GPU, so a host
     tensor, or tensors on two GPUs, raise ValueError before any launch."""
-    dev = None
+    first = index = None
     for t in tensors:
         if t is None:
             continue
         if not t.is_cuda:
             raise ValueError(f"tensors must be on the GPU, got one on {t.device}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    if dev is None:
+        if first is None:
+            first, index = t, t.get_device()
+        elif t.get_device() != index:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    if first is None:
         raise ValueError("no tensor given")
-    return dev
+    return first.device
 
 
 def _raw_stream(index: int) -> int:

@@ -101,7 +101,10 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype, Hk=None, D=None):
     if len(shape) != 4 or not k.numel():
         raise ValueError(f"k_cache must be a [pages, page_size, Hk, D] tensor, got shape {tuple(shape)}")
     want = (shape[0], shape[1], shape[2] if Hk is None else Hk, shape[3] if D is None else D)
-    return want, _written(k, "k_cache", want, dtype), _written(v, "v_cache", want, dtype)
+    ks = _written(k, "k_cache", want, dtype)
+    if v.dtype == dtype and v.shape == shape and v.stride() == k.stride() and not v.data_ptr() & 15:
+        return want, ks, ks                        # laid out as k_cache is
+    return want, ks, _written(v, "v_cache", want, dtype)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -151,8 +154,8 @@ def plan_step(block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch
         raise ValueError(f"page_size {page_size} and num_tokens {num_tokens} out of range for a table of {P} pages")
     dev = _lib.same_device(t, seq_lens, new_lens, free_pages, free_count)
     if out is None:
-        cu_lens, after, positions, count, lacking = torch.empty(
-            2 * B + 3 + num_tokens, dtype=torch.int32, device=dev).split((B + 1, B, num_tokens, 1, 1))
+        cu_lens, after, positions, count, lacking = t.new_empty(2 * B + 3 + num_tokens).split_with_sizes(
+            (B + 1, B, num_tokens, 1, 1))
         out = StepPlan(cu_lens, after, positions, torch.empty(num_tokens, dtype=torch.int64, device=dev), count, lacking)
     else:
         outs = [_ints(out.cu_lens, "out.cu_lens", (B + 1,)), _ints(out.seq_lens, "out.seq_lens", (B,)),
@@ -190,10 +193,10 @@ def _scale(scale, D: int) -> float:
     return scale
 
 
-def _attn_dtype(*tensors) -> None:
-    dt = tensors[0].dtype
-    if dt not in (torch.bfloat16, torch.float16) or any(t.dtype != dt for t in tensors):
-        raise TypeError(f"expected bf16 or f16 tensors of one type, got {[t.dtype for t in tensors]}")
+def _attn_dtype(q, k, v) -> None:
+    dt = q.dtype
+    if (dt != torch.bfloat16 and dt != torch.float16) or k.dtype != dt or v.dtype != dt:
+        raise TypeError(f"expected bf16 or f16 tensors of one type, got {[t.dtype for t in (q, k, v)]}")
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -234,7 +237,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _inference_only("paged_attention", q, k_cache, v_cache)
     if out is None:
         dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens)
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+        out = q.new_empty((T, Hq, D))
         os_ = (Hq * D, D)
     else:
         os_ = _written(out, "out", (T, Hq, D), q.dtype)
@@ -249,7 +252,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         seq_lens=seq_lens.data_ptr(), dtype=_lib.FS_DTYPE[q.dtype], B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=P, page_size=ps,
         num_pages=pages, max_new=0 if max_new is None else min(int(max_new), T), window=window, sinks=sinks,
         softmax_scale=scale)
-    work = torch.empty(_lib.load().fs_paged_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8, device=dev)
+    work = q.new_empty(_lib.load().fs_paged_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8)
     args.work = work.data_ptr()
     _lib.call("fs_paged_attn", args, dev)
     return out
@@ -279,15 +282,18 @@ def window_attention(query_states: torch.Tensor, key_states: torch.Tensor, value
     scale = _scale(softmax_scale, D)
     _inference_only("window_attention", q, k, v)
     if out is None:
-        out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
-    qs, ks, vs, os_ = _strides(q), _strides(k), _strides(v), _written(out, "out", (B, Lq, Hq, D), q.dtype)
+        out = q.new_empty((B, Lq, Hq, D))
+        os_ = (Lq * Hq * D, Hq * D, D)
+    else:
+        os_ = _written(out, "out", (B, Lq, Hq, D), q.dtype)
+    qs, ks, vs = _strides(q), _strides(k), _strides(v)
     dev = _lib.same_device(q, k, v, out)
     args = WindowAttnArgs(
         q=q.data_ptr(), q_sb=qs[0], q_sh=qs[1], q_sl=qs[2], k=k.data_ptr(), k_sb=ks[0], k_sh=ks[1], k_sl=ks[2],
         v=v.data_ptr(), v_sb=vs[0], v_sh=vs[1], v_sl=vs[2], out=out.data_ptr(), o_sb=os_[0], o_sl=os_[1], o_sh=os_[2],
         dtype=_lib.FS_DTYPE[q.dtype], B=B, Hq=Hq, Hk=Hk, Lq=Lq, Lk=Lk, D=D, window=window, sinks=sinks,
         softmax_scale=scale)
-    work = torch.empty(_lib.load().fs_window_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8, device=dev)
+    work = q.new_empty(_lib.load().fs_window_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8)
     args.work = work.data_ptr()
     _lib.call("fs_window_attn", args, dev)
     return out

@@ -91,7 +91,8 @@ def _common(name, q, k, positions, inv_freq):
 def _out(out, name, like):
     """The given output (checked) or a new one, and its strides."""
     if out is None:
-        out = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        T, H, D = like.shape
+        return like.new_empty((T, H, D)), (H * D, D)
     return out, _written(out, name, like.shape, like.dtype)
 
 
