@@ -209,7 +209,7 @@ def cpu_baseline_xattn(q, k, v, args, bs, nnz_total, sel):
 
 
 # The sources each traffic row depends on (fftsparse_amd/csrc, plus the C-ABI header).
-TRAFFIC_SOURCES = {"bsattn": ("attn.hip", "common.h"),
+TRAFFIC_SOURCES = {"bsattn": ("attn.hip", "attn_tile.h", "common.h"),
                    "select": ("pool.hip", "scores.hip", "select.hip", "common.h")}
 # rocprofv3 kernel names summed into each row
 TRAFFIC_KERNELS = {"bsattn": ("bsattn_kernel",),

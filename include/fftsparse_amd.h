@@ -468,17 +468,18 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * at position p:
  *   out = softmax(q . k_s * scale) v over the tokens s <= p with s > p - window
  *         or s < sinks (window == 0: every s <= p),
- * for query head h on KV head h / (Hq / Hk); scale finite, not negative.  A row that sees no token is 0;
- * rows past cu_lens[B] are left as they were.  A page outside 0 .. num_pages - 1
- * holds no token.  What stands in slots that no row sees (past a request's end,
- * wholly outside every window) is not used, be it nan; a value of v that is not
- * finite may reach rows of the same request that do not see its token.  Row
- * numbers that fall (cu_lens[b + 1] < cu_lens[b]) leave every row as it was;
- * lengths and row numbers out of range are taken at the border.  The lengths stay
- * on the device: nothing but B, T and P bounds the work, and max_new (the most
- * new tokens that a request may have, 0: T) only chooses between forms of the
- * kernel.  bf16 / f16, D 64 or 128, page_size a multiple of 16 up to 4096,
- * P * page_size <= 2^26, num_pages < 2^26, B <= 4096.  out may be q itself.
+ * for query head h on KV head h / (Hq / Hk); scale is finite and not negative.  A
+ * row that sees no token is 0; rows past cu_lens[B] are left as they were.  A page
+ * outside 0 .. num_pages - 1 holds no token.  What stands in slots that no row
+ * sees (past a request's end, wholly outside every window) is not used, be it nan;
+ * a value of v that is not finite may reach rows of the same request that do not
+ * see its token.  Row numbers that fall (cu_lens[b + 1] < cu_lens[b]) leave every
+ * row as it was; lengths and row numbers out of range are taken at the border.
+ * The lengths stay on the device: nothing but B, T and P bounds the work, and
+ * max_new (the most new tokens that a request may have, 0: T) only chooses between
+ * forms of the kernel.  bf16 / f16, D 64 or 128, page_size a multiple of 16 up to
+ * 4096, P * page_size <= 2^26, num_pages < 2^26, B <= 4096, k_ss and v_ss
+ * 0 .. 2^23 - 1.  out may be q itself.
  * work: fs_paged_attn_work_bytes(a) bytes of device scratch, which never falls as
  * T, B or max_new grows (nor to max_new = 0).  Calls that overlap on one workspace
  * race. */
@@ -502,7 +503,8 @@ FS_API int fs_paged_attn(const fs_paged_attn_args* a, void* stream);
 /* ---- sliding-window attention with sinks ----------------------------------
  * fs_paged_attn's rule on contiguous tensors: q [B][Hq][Lq][D], k and v
  * [B][Hk][Lk][D] views, query t at position t + Lk - Lq.  Rows that see no
- * token (Lq > Lk) are 0.  B <= 4096, Lk <= 2^26; out may be q itself.
+ * token (Lq > Lk) are 0.  B <= 4096, Lk <= 2^26, k_sl and v_sl 0 .. 2^23 - 1; out
+ * may be q itself.
  * work: fs_window_attn_work_bytes(a) bytes, as above. */
 typedef struct {
   const void* q; int64_t q_sb, q_sh, q_sl;
