@@ -301,11 +301,12 @@ struct Piece {
 };
 
 // How long a call takes, in key tiles' time: N pieces of at most c tiles of the W in all, `slots` at a time; a start
-// per round of pieces and, where sums are joined, a launch and their writing and reading.
-__device__ __forceinline__ float call_time(float N, float c, float W, float slots, float joined) {
-  constexpr float kStart = 1.5f, kJoin = 2.0f, kPiece = 0.014f;
+// per round of pieces and, where sums are joined, a launch, their writing and reading, and a turn for each of the most
+// pieces of a row tile (without that, 16 tokens over 2048 were cut into single tiles: 33 us against 22).
+__device__ __forceinline__ float call_time(float N, float c, float W, float slots, float joined, float most) {
+  constexpr float kStart = 1.5f, kJoin = 1.5f, kPiece = 0.014f, kTurn = 0.3f;
   const float rounds = ceilf(N / slots);
-  return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined > 0.f ? kJoin + joined * kPiece : 0.f);
+  return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined > 0.f ? kJoin + joined * kPiece + most * kTurn : 0.f);
 }
 // The 16 numbers of key tiles per piece that are tried: an i-th part of the longest row tile's, and what gives about i
 // rounds of pieces (U row tiles, of which each may leave a shorter piece).
@@ -1181,7 +1182,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
     }
     n = wave_prefix(n);
     sp = wave_prefix(sp);
-    float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, (float)sp * (float)a.Hk);
+    float t = call_time((float)n * (float)a.Hk, (float)c, W, (float)slots, (float)sp * (float)a.Hk,
+                        (float)parts_of(longest, c));
     if (wave > 0 && (n > max_pieces || (int64_t)sp * a.Hk > max_parts)) t = INFINITY;
     if (lane == 63) cost[wave] = t;
   }
@@ -1251,7 +1253,7 @@ static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
   return w;
 }
 // Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.  At 64 rows few_kernel reads the keys
-// twice: 16 tokens of one request of 2048 20 us against 33, but of 32 requests of 4096 201 against 117.  It counts key
+// twice: 16 tokens of one request of 2048 20 us against 22, but of 32 requests of 4096 201 against 117.  It counts key
 // tiles of row tiles in 32 bits.
 static bool few_rows(int64_t max_new, int G, int64_t T, int B, int Hk, int64_t keys) {
   return max_new * G <= 32 && (T * G / 32 + B) * Hk < (1ll << 30) / (keys / 32 + 2);
