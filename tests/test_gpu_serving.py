@@ -130,6 +130,31 @@ def test_paged_attention_many_requests(max_new):
     b.check(b.gpu(max_new=max_new))
 
 
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_paged_attention_most_requests(max_new):
+    lens = [((7 * i) % 37, 1 if i % 3 else 0) for i in range(4094)] + [(2000, 1), (50, 1)]
+    b = Batch(lens, Hq=2, Hk=1, D=64, seed=27)
+    b.check(b.gpu(max_new=max_new))
+
+
+@pytest.mark.parametrize("window,sinks", [(500, 5), (None, 0)])
+def test_paged_attention_many_row_tiles(window, sinks):
+    """A prompt of more row tiles than the plan of pieces holds in LDS; some of its rows against the oracle."""
+    n, ps = 264_000, 256
+    pages = -(-n // ps)
+    g = torch.Generator().manual_seed(28)
+    q, k, v = (torch.randn(n, h, 64, generator=g).to(BF) for h in (4, 1, 1))
+    table = torch.randperm(pages, generator=g).to(I32)
+    kc, vc = (torch.zeros(pages, ps, 1, 64, dtype=BF) for _ in range(2))
+    for x, c in ((k, kc), (v, vc)):
+        c[table.long()] = torch.cat([x, x.new_zeros(pages * ps - n, 1, 64)]).view(pages, ps, 1, 64)
+    got = fa.paged_attention(q.to(DEV), kc.to(DEV), vc.to(DEV), table[None].to(DEV), _i32([0, n]), _i32([n]), window=window,
+                             sinks=sinks).cpu()
+    for i in (0, 1, 31, 32, 1023, 4999, 131_071, 262_143, 262_144, n - 1) if window else (0, 77, n - 1):
+        want, mag = ref.attend(q[i:i + 1], k[:i + 1], v[:i + 1], i, window, sinks)
+        _check_attn(got[i:i + 1], want, mag, i + 1, BF, i)
+
+
 @pytest.mark.parametrize("lens,max_new", [([(20000, 1)], 1), ([(9000, 20)], None), ([(6000, 100), (40, 1)], None)])
 def test_paged_attention_long(lens, max_new):
     """Long contexts, whose keys are split over workgroups and joined."""
