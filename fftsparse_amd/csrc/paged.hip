@@ -1416,9 +1416,14 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   k.T = a->Lq;
   const bool few = few_rows(*a);
   const Work w = work_of(*a);
-  // Every sequence is as long here: whether splitting keys can pay is known.
+  // Every sequence is as long here, so whether splitting keys pays is known.  In key tiles' time at D = 128: a call without a
+  // plan lasts its longest row tile (slower where two share a CU), one with it its work evenly spread and 21 for the plan,
+  // more pieces' starts and the joining.  Causal, 32 / 8 heads, 1100, 2000: 29.6, 52 us without, 38.9, 61 with; 8 / 2
+  // heads, 900, 1500, 4000: 22.4, 33.7, 78 without, 24.4, 31.9, 58.7 with.
   const int64_t tiles = ((int64_t)a->Lq * (a->Hq / a->Hk) + w.rows - 1) / w.rows * a->B * a->Hk;
-  const int64_t keys = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
-  const bool plan = !few && tiles < kSlotsMany && keys >= 1024;
+  const int64_t most = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
+  const int64_t mean = std::min(most, std::max<int64_t>(a->Lk - a->Lq / 2, most / 2));
+  const bool plan = !few && tiles < kSlotsMany &&
+                    most / 64.0 * (tiles <= kSlotsMany / 2 ? 1.1 : 1.35) > 21.0 + mean / 64.0 * tiles / (kSlotsMany / 2);
   return run<false>(k, a->dtype, a->D, few, plan, w, static_cast<char*>(a->work), a->B, a->Lq, (hipStream_t)stream, fn);
 }
