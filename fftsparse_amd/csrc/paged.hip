@@ -302,9 +302,10 @@ struct Piece {
 
 // How long a call takes, in key tiles' time: N pieces of at most c tiles of the W in all, `slots` at a time; a start
 // per round of pieces and, where sums are joined, a launch, their writing and reading, and a turn for each of the most
-// pieces of a row tile (without that, 16 tokens over 2048 were cut into single tiles: 33 us against 22).
+// pieces of a row tile (without that, 16 tokens over 2048 were cut into single tiles: 33 us against 22; a
+// launch at 1.5 cut a prompt of 700: 35 us against 29, at 9 left a batch of windows whole: 42 against 39).
 __device__ __forceinline__ float call_time(float N, float c, float W, float slots, float joined, float most) {
-  constexpr float kStart = 1.5f, kJoin = 1.5f, kPiece = 0.014f, kTurn = 0.3f;
+  constexpr float kStart = 1.5f, kJoin = 5.0f, kPiece = 0.014f, kTurn = 0.3f;
   const float rounds = ceilf(N / slots);
   return fminf(rounds * c, W / slots + c) + rounds * kStart + (joined > 0.f ? kJoin + joined * kPiece + most * kTurn : 0.f);
 }
