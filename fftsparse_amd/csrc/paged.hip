@@ -1102,8 +1102,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // each.  One workgroup; its lists are read by the attention and the joining kernel.
 template <int M, int TK>
 __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a, int4* pieces, int4* pairs, int4* splits,
-                                                                   int32_t* head, int max_pairs, int max_pieces,
-                                                                   int max_parts, int slots) {
+                                                                   int32_t* head, int max_pieces, int max_parts,
+                                                                   int slots) {
   constexpr int NW = kPlanThreads / 64;
   constexpr int kHeld = 8192;                      // row tiles whose key tiles are kept in LDS
   __shared__ int base[kMaxRequests + 1], tiles[kHeld];
@@ -1231,33 +1231,45 @@ __global__ __launch_bounds__(kPlanThreads) void plan_pieces_kernel(PagedKArgs a,
 
 // ---- host ---------------------------------------------------------------------
 
-// Workspace of a call: head, pairs, pieces, the split pieces' sums.
+// Workspace of a call: the split pieces' sums, and before them, in calls of many_kernel, head, pairs, pieces and splits.
 struct Work {
-  int max_pairs, max_pieces, max_parts, max_splits, rows;
+  int64_t max_pairs, max_pieces, max_splits;
+  int max_parts, rows;
   size_t pairs, pieces, splits, ml, o, bytes;
 };
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-// row tiles of at most `rows` rows of B requests with T tokens in all; few: row tiles of 32
+// row tiles of at most `rows` rows of B requests with T tokens in all; few: row tiles of 32, no lists
 static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
-  Work w;
+  Work w{};
   w.rows = few ? 32 : 128;
-  w.max_pairs = (int)(T * G / w.rows + B);
   w.max_parts = few ? 2 * few_slots(D) : kPartsMany;
-  w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
-  w.max_splits = std::min(w.max_pairs, std::max(w.max_parts / (2 * Hk), 1));
-  w.pairs = 256;
-  w.pieces = w.pairs + align256((size_t)w.max_pairs * 16);
-  w.splits = w.pieces + align256((size_t)w.max_pieces * 16);
-  w.ml = w.splits + align256((size_t)w.max_splits * 16);
+  if (!few) {
+    w.max_pairs = T * G / w.rows + B;
+    w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
+    w.max_splits = std::min<int64_t>(w.max_pairs, std::max(w.max_parts / (2 * Hk), 1));
+    w.pairs = 256;
+    w.pieces = w.pairs + align256((size_t)w.max_pairs * 16);
+    w.splits = w.pieces + align256((size_t)w.max_pieces * 16);
+    w.ml = w.splits + align256((size_t)w.max_splits * 16);
+  }
   w.o = w.ml + align256((size_t)w.max_parts * w.rows * 8);
   w.bytes = w.o + (size_t)w.max_parts * w.rows * D * 4;
   return w;
 }
 // Which kernel: single tokens and few rows of a KV head are bound by the keys' bytes.  At 64 rows few_kernel reads the keys
 // twice: 16 tokens of one request of 2048 20 us against 22, but of 32 requests of 4096 201 against 117.  It counts key
-// tiles of row tiles in 32 bits.
-static bool few_rows(int64_t max_new, int G, int64_t T, int B, int Hk, int64_t keys) {
-  return max_new * G <= 32 && (T * G / 32 + B) * Hk < (1ll << 30) / (keys / 32 + 2);
+// tiles of row tiles (of all KV heads) in 32 bits.
+static bool few_rows(int64_t max_new, int G, int64_t row_tiles, int64_t keys) {
+  return max_new * G <= 32 && row_tiles < (1ll << 30) / (keys / 32 + 2);
+}
+// What a caller is asked for.  It never falls as an argument grows, so a workspace of the largest call serves every other
+// one: the lists are sized as for one KV head, which has the most row tiles and pieces; few_kernel's size is asked for
+// where that is taken with one KV head too (few_rows then holds for any number: at most 32 rows of all heads, and
+// row tiles counted from above), and it is the same for both head dims.  Either kernel's fits into many_kernel's.
+static size_t work_bytes(int64_t max_new, int64_t T, int B, int Hq, int Hk, int D, int64_t keys) {
+  if (few_rows(max_new, Hq, T * Hq / 32 + (int64_t)B * Hk, keys))
+    return std::max(work_of(true, T, B, 1, Hq, 64).bytes, work_of(true, T, B, 1, Hq, 128).bytes);
+  return work_of(false, T, B, 1, Hq, D).bytes;
 }
 
 template <typename T, int D, bool PAGED>
@@ -1280,17 +1292,17 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
     int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
     k.splits = reinterpret_cast<int4*>(work + w.splits);
     k.head = reinterpret_cast<int32_t*>(work);
-    k.max_splits = w.max_splits;
-    grid = (int64_t)w.max_pieces * k.Hk;
+    k.max_splits = (int)w.max_splits;
+    grid = w.max_pieces * k.Hk;
     plan_pieces_kernel<128, 64><<<1, kPlanThreads, 0, s>>>(k, pieces, reinterpret_cast<int4*>(work + w.pairs), k.splits,
-                                                           k.head, w.max_pairs, w.max_pieces, w.max_parts, kSlotsMany);
+                                                           k.head, (int)w.max_pieces, w.max_parts, kSlotsMany);
     if (int rc = fs_host::launch_status(fn)) return rc;
     k.pieces = pieces;
   }
   many_kernel<T, D, PAGED><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    combine_kernel<T, D, 128><<<(unsigned)((int64_t)w.max_splits * k.Hk * 4 * (D / 32)), kJoinThreads, 0, s>>>(k);
+    combine_kernel<T, D, 128><<<(unsigned)(w.max_splits * k.Hk * 4 * (D / 32)), kJoinThreads, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;
@@ -1334,10 +1346,12 @@ static int check_common(const char* fn, int dtype, int D, int Hq, int Hk, int B,
 // the most new tokens of one request
 static int64_t most_new(const fs_paged_attn_args& a) { return a.max_new > 0 && a.max_new < a.T ? a.max_new : a.T; }
 static bool few_rows(const fs_paged_attn_args& a) {
-  return few_rows(most_new(a), a.Hq / a.Hk, a.T, a.B, a.Hk, (int64_t)a.P * a.page_size);
+  const int G = a.Hq / a.Hk;
+  return few_rows(most_new(a), G, ((int64_t)a.T * G / 32 + a.B) * a.Hk, (int64_t)a.P * a.page_size);
 }
 static bool few_rows(const fs_window_attn_args& a) {
-  return few_rows(a.Lq, a.Hq / a.Hk, (int64_t)a.B * a.Lq, a.B, a.Hk, a.Lk);
+  const int G = a.Hq / a.Hk;
+  return few_rows(a.Lq, G, ((int64_t)a.B * a.Lq * G / 32 + a.B) * a.Hk, a.Lk);
 }
 static Work work_of(const fs_paged_attn_args& a) { return work_of(few_rows(a), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D); }
 static Work work_of(const fs_window_attn_args& a) {
@@ -1346,11 +1360,11 @@ static Work work_of(const fs_window_attn_args& a) {
 
 extern "C" size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a) {
   if (!a || a->B <= 0 || a->T <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
-  return work_of(*a).bytes;
+  return work_bytes(most_new(*a), a->T, a->B, a->Hq, a->Hk, a->D, (int64_t)a->P * a->page_size);
 }
 extern "C" size_t fs_window_attn_work_bytes(const fs_window_attn_args* a) {
   if (!a || a->B <= 0 || a->Lq <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
-  return work_of(*a).bytes;
+  return work_bytes(a->Lq, (int64_t)a->B * a->Lq, a->B, a->Hq, a->Hk, a->D, a->Lk);
 }
 
 extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {

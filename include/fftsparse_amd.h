@@ -481,7 +481,9 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * 4096, P * page_size <= 2^26, num_pages < 2^26, B <= 4096, k_ss and v_ss
  * 0 .. 2^23 - 1.  out may be q itself.
  * work: fs_paged_attn_work_bytes(a) bytes of device scratch, which never falls as
- * T, B or max_new grows (nor to max_new = 0).  Calls that overlap on one workspace
+ * any of T, B, Hq, Hk, D, P, page_size and max_new grows (0: T), so one sized for
+ * the largest of each serves every call: about 9 MB where max_new * Hq <= 32, else
+ * 68 MB (D = 64: 35) and T * Hq / 4 bytes.  Calls that overlap on one workspace
  * race. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
@@ -505,7 +507,9 @@ FS_API int fs_paged_attn(const fs_paged_attn_args* a, void* stream);
  * [B][Hk][Lk][D] views, query t at position t + Lk - Lq.  Rows that see no
  * token (Lq > Lk) are 0.  B <= 4096, Lk <= 2^26, k_sl and v_sl 0 .. 2^23 - 1; out
  * may be q itself.
- * work: fs_window_attn_work_bytes(a) bytes, as above. */
+ * work: fs_window_attn_work_bytes(a) bytes, which never falls as any of B, Lq, Lk,
+ * Hq, Hk and D grows: as above with T = B * Lq and max_new = Lq, whether or not
+ * the call cuts its keys into pieces (long prompts do not). */
 typedef struct {
   const void* q; int64_t q_sb, q_sh, q_sl;
   const void* k; int64_t k_sb, k_sh, k_sl;
