@@ -140,3 +140,22 @@ def test_workspaces_hold_what_is_written(cuts, max_new, Hq, Hk, D):
         if n:
             check(got[x], b.q[x], b.k[r], b.v[r], c, None, 0, r)
     assert max_new == 1 or cuts.pop() >= 0
+
+
+@pytest.mark.parametrize("lens", [[(6000, 1), (50, 1)], [(6000, 40), (50, 1)]], ids=["tokens", "chunk"])
+def test_the_largest_values(cuts, lens):
+    """bf16 values up to 2^93, the sums' range at any length: equal weights, and weights that grow along the keys (a row's
+    running maximum then lags behind, and weights up to 2^8 are summed)."""
+    for rise in (0.0, 0.004):
+        b = Batch(lens, ps=64, seed=30)
+        b.q[:] = 1
+        for r, x in enumerate(b.k):
+            x[:] = (rise * torch.arange(len(x)) / 11.3).to(BF)[:, None, None]
+            b.v[r] = b.v[r].clamp(-1, 1) * 2.0 ** 93
+            for i in range(-(-len(x) // 64)):
+                n = min(64, len(x) - 64 * i)
+                b.kc[b.table[r, i], :n], b.vc[b.table[r, i], :n] = x[64 * i:64 * i + n], b.v[r][64 * i:64 * i + n]
+        got = b.gpu()
+        for r, (c, n) in enumerate(b.lens):
+            x = slice(int(b.cu[r]), int(b.cu[r + 1]))
+            check(got[x], b.q[x], b.k[r], b.v[r], c, None, 0, (r, rise))
