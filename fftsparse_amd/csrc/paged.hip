@@ -18,7 +18,10 @@
 // v_mfma_f32_32x32x16, of which a single token uses G of 32 columns (about a tenth of the
 // MFMA rate is taken); V is read transposed from LDS as it is stored.  Measured
 // (bf16, D = 128, 32 / 8 heads): 32 requests of 16384 tokens 5.3 TB/s, 64 of 64 - 8192 4.4 TB/s,
-// one of 131072 4.7 TB/s; a copy of 4 GiB takes 4.9 TB/s on the same card.
+// one of 131072 4.7 TB/s; a copy of 4 GiB takes 4.9 TB/s on the same card, but pool.hip's pass, which only reads as
+// this one does, 6.7: what keeps the last quarter has not been found.  All 106 scalar registers are taken and 72 (D = 64,
+// contiguous) to 102 (D = 128, paged) more are kept in lanes of vector registers; no
+// vector register is spilled.
 //
 // many_kernel (tiles of 128 rows) is bound by MFMA: 4 waves of 32 rows share tiles of 64 keys,
 // two tiles deep: S of the next tile and P V of the last one are interleaved with the
@@ -32,7 +35,9 @@
 //
 // Rounding: scores, maxima, sums and O are in 32 bits; P is rounded to the input type for the
 // second product (its relative error, at most half a step of the type, averages out over the keys as the
-// values' own does), and the row sum adds the rounded P, so that weights add up to one.
+// values' own does), and the row sum adds the rounded P, so that weights add up to one.  Against 64 bits (2-norm)
+// bf16 is off by 1.8e-3 to 2.0e-3 (1.6e-3 to 1.7e-3 with P in 32 bits: the result's own rounding), f16 by 2.2e-4 to 2.8e-4
+// (2.1e-4).  Sums stay below 2^34 of the largest |v| (P up to 2^8, 2^26 keys), so |v| up to 2^93 is safe.
 //
 // Groups of 16 keys are never split by a page (its size is a multiple of 16): a
 // copy of one is addressed by one entry of the table.  A group that not all rows
@@ -303,7 +308,10 @@ struct Piece {
 // How long a call takes, in key tiles' time: N pieces of at most c tiles of the W in all, `slots` at a time; a start
 // per round of pieces and, where sums are joined, a launch, their writing and reading, and a turn for each of the most
 // pieces of a row tile (without that, 16 tokens over 2048 were cut into single tiles: 33 us against 22; a
-// launch at 1.5 cut a prompt of 700: 35 us against 29, at 9 left a batch of windows whole: 42 against 39).
+// launch at 1.5 cut a prompt of 700: 35 us against 29, at 9 left a batch of windows whole: 42 against 39).  One set
+// serves both head dims, though a tile takes about half as long at 64: with all four twice as large there 64 tokens over
+// 8192 took 34.7 us against 37.4, but 16 requests with chunks 71 against 61, windows of them 42.5 against 39.8, 64 tokens over
+// 2048 23.5 against 22.8, and prompts of 300 to 2000 the same within 1%.
 __device__ __forceinline__ float call_time(float N, float c, float W, float slots, float joined, float most) {
   constexpr float kStart = 1.5f, kJoin = 5.0f, kPiece = 0.014f, kTurn = 0.3f;
   const float rounds = ceilf(N / slots);
@@ -1434,7 +1442,9 @@ extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {
   // Every sequence is as long here, so whether splitting keys pays is known.  In key tiles' time at D = 128: a call without a
   // plan lasts its longest row tile (slower where two share a CU), one with it its work evenly spread and 21 for the plan,
   // more pieces' starts and the joining.  Causal, 32 / 8 heads, 1100, 2000: 29.6, 52 us without, 38.9, 61 with; 8 / 2
-  // heads, 900, 1500, 4000: 22.4, 33.7, 78 without, 24.4, 31.9, 58.7 with.
+  // heads, 900, 1500, 4000: 22.4, 33.7, 78 without, 24.4, 31.9, 58.7 with.  At D = 64 the sides meet at the same lengths: 32 / 8
+  // heads, 1100, 2000: 21.3, 37.4 without, 28.5, 45.1 with; 8 / 2 heads, 900, 1500, 4000: 17.3, 25.8, 59.6 without, 19.3, 24.2,
+  // 44.2 with; window of 1500, 1500, 2000, 4000: 25.8, 27.0, 28.2 without, 24.1, 27.2, 36.6 with.
   const int64_t tiles = ((int64_t)a->Lq * (a->Hq / a->Hk) + w.rows - 1) / w.rows * a->B * a->Hk;
   const int64_t most = a->window && a->window < a->Lk ? (int64_t)a->window + std::min(a->sinks, a->Lk) + w.rows : a->Lk;
   const int64_t mean = std::min(most, std::max<int64_t>(a->Lk - a->Lq / 2, most / 2));

@@ -13,7 +13,9 @@
 // 16-byte pieces (both of a pair's pieces where they are apart).  A thread keeps its
 // place in the head and goes from head to head, so that no piece costs a
 // division (found by one, the pieces' places cost more than their bytes in the
-// interleaved layout, where a piece is 16 bytes and not two times 16).
+// interleaved layout, where a piece is 16 bytes and not two times 16).  Few tokens are bound by latency: 48 of them take
+// 5.5 us, the launch and two round trips one after the other, positions and frequencies before the barrier, q, k and
+// v behind it.
 #include <algorithm>
 #include <climits>
 
@@ -56,7 +58,8 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
   }
 }
 
-// V: elements of a piece, 16 bytes where every run of dims allows it, else 1.
+// V: elements of a piece, 16 bytes where every run of dims allows it, else 1.  32768 tokens, 32 / 8 heads of 128: bf16
+// 126 us and f32 249 us (5.3 and 5.4 TB/s); 34 of the dims rotated, by single elements, bf16 421 us (426 interleaved): 1.6 TB/s.
 template <typename T, int V, bool INTER>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
   constexpr bool TWO = !INTER || V == 1;           // a pair's elements are apart: two loads, two stores

@@ -219,7 +219,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     they were (unset in a new tensor).  A page number outside the cache holds no
     token; a row that sees no token is 0.  Slots that no row sees may hold anything;
     a value of v that is not finite may reach rows of its request that do not see
-    it.  ``out`` may be q.  Up to 4096 requests of 2^26 tokens."""
+    it.  Scores, maxima and sums are in 32 bits; the weights are rounded to the input
+    type before the product with v (values up to 2^93).  ``out`` may be q.  Up to 4096
+    requests of 2^26 tokens."""
     q, qs = _rows(q, "q")
     T, Hq, D = q.shape
     _attn_dtype(q, k_cache, v_cache)
@@ -266,8 +268,11 @@ def window_attention(query_states: torch.Tensor, key_states: torch.Tensor, value
     q [B,Hq,Lq,D], k/v [B,Hk,Lk,D] (bf16 / f16, D 64 or 128; strided views) ->
     [B, Lq, Hq, D], as ``block_sparse_attention`` returns it.  Query t is at
     position t + Lk - Lq and sees the last ``window`` tokens up to itself, itself
-    included, and the first ``sinks``; window None: every token up to itself.  The
-    mask is exact to the token.  A query before the first key sees nothing and gives 0."""
+    included, and the first ``sinks``; window None: every token up to itself (dense
+    causal attention; ``block_sparse_attention`` without lists is the faster one for
+    short sequences and for 16384 tokens of few heads).  The mask is exact to the
+    token.  A query before the first key sees nothing and gives 0.  Rounding as in
+    ``paged_attention``."""
     q, k, v = (_check_layout(x) for x in (query_states, key_states, value_states))
     B, Hq, Lq, D = q.shape
     Hk, Lk = k.shape[1], k.shape[2]

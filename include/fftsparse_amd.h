@@ -473,7 +473,8 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * outside 0 .. num_pages - 1 holds no token.  What stands in slots that no row
  * sees (past a request's end, wholly outside every window) is not used, be it nan;
  * a value of v that is not finite may reach rows of the same request that do not
- * see its token.  Row numbers that fall (cu_lens[b + 1] < cu_lens[b]) leave every
+ * see its token.  Scores, maxima and sums are in 32 bits; the weights are rounded to
+ * dtype before the product with v, whose values may be up to 2^93.  Row numbers that fall (cu_lens[b + 1] < cu_lens[b]) leave every
  * row as it was; lengths and row numbers out of range are taken at the border.
  * The lengths stay on the device: nothing but B, T and P bounds the work, and
  * max_new (the most new tokens that a request may have, 0: T) only chooses between
