@@ -49,7 +49,7 @@ def listed():
         # a batch of chats over an 8-bit cache, every length from a few tokens on
         _case("decode8-64", "attend", B=64, Lmin=64, Lmax=8192, ps=16, bits=8),
         # a chunk of a long prompt over an 8-bit cache
-        _case("chunk8-2k", "attend", Lmin=30720, Lmax=30720, Nmin=2048, Nmax=2048, bits=8),
+        _case("chunk8-2k", "attend", Lmin=30000, Lmax=30000, Nmin=2048, Nmax=2048, bits=8),
         # one request with a small tree of drafts
         _case("tree-1", "tree", Nmin=8, Nmax=8),
         # a batch with a tree of 64 tokens each
