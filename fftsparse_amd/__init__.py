@@ -22,14 +22,16 @@ Serving after the prefill, over a paged cache (no counterpart in the reference):
     rope(q, k, positions, inv_freq, ...)            rotary positions (rope_frequencies: plain or scaled)
     rope_cache(q, k, v, positions, slots, ...)      the same, keys and values into the cache
     paged_attention(q, k_cache, v_cache, ...)       new tokens (one or a chunk) over the cache
+    plan_tree, tree_attention, accept_tree, move_kept   drafted tokens as a tree: attention, the path that is kept
     window_attention(q, k, v, window=, sinks=)      sliding window and first tokens, on contiguous K/V
 """
 from .attn import (AttentionCall, BlockSelection, block_sparse_attention, myattn_prefill, rope_pool,  # noqa: F401
                    select_blocks)
 from .paged import StepPlan, paged_attention, plan_step, window_attention  # noqa: F401
 from .rotary import rope, rope_cache, rope_frequencies  # noqa: F401
+from .tree import Accepted, TreePlan, accept_tree, move_kept, plan_tree, tree_attention  # noqa: F401
 from . import fix_mask, flex, xattn  # noqa: F401
 
 __all__ = ["myattn_prefill", "select_blocks", "block_sparse_attention", "rope_pool", "AttentionCall",
            "BlockSelection", "StepPlan", "plan_step", "rope", "rope_cache", "rope_frequencies", "paged_attention",
-           "window_attention", "fix_mask", "flex", "xattn"]
+           "window_attention", "TreePlan", "plan_tree", "tree_attention", "Accepted", "accept_tree", "move_kept", "fix_mask", "flex", "xattn"]

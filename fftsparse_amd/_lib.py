@@ -19,7 +19,7 @@ import torch  # noqa: F401  (must precede the library load, see module docstring
 LIB_PATH = Path(os.environ.get("FFTSPARSE_AMD_LIB") or Path(__file__).resolve().with_name("libfftsparse_amd.so"))
 
 FS_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 
 class PoolArgs(ctypes.Structure):
@@ -137,7 +137,7 @@ class RopeArgs(ctypes.Structure):
                 ("slots", c_void_p),
                 ("k_cache", c_void_p), ("kc_sp", c_int64), ("kc_ss", c_int64), ("kc_sh", c_int64),
                 ("v_cache", c_void_p), ("vc_sp", c_int64), ("vc_ss", c_int64), ("vc_sh", c_int64),
-                ("num_pages", c_int64), ("page_size", c_int)]
+                ("num_pages", c_int64), ("page_size", c_int), ("k_scale", c_void_p), ("v_scale", c_void_p)]
 
 
 class PagedAttnArgs(ctypes.Structure):
@@ -149,7 +149,8 @@ class PagedAttnArgs(ctypes.Structure):
                 ("dtype", c_int), ("B", c_int), ("T", c_int), ("Hq", c_int), ("Hk", c_int), ("D", c_int),
                 ("P", c_int), ("page_size", c_int), ("num_pages", c_int64),
                 ("max_new", c_int), ("window", c_int), ("sinks", c_int), ("softmax_scale", c_float),
-                ("work", c_void_p)]
+                ("work", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("mask", c_void_p), ("mask_words", c_int), ("positions", c_void_p)]
 
 
 class WindowAttnArgs(ctypes.Structure):
@@ -161,14 +162,33 @@ class WindowAttnArgs(ctypes.Structure):
                 ("D", c_int), ("window", c_int), ("sinks", c_int), ("softmax_scale", c_float), ("work", c_void_p)]
 
 
+class TreePlanArgs(ctypes.Structure):
+    _fields_ = [("parents", c_void_p), ("cu_lens", c_void_p), ("seq_lens", c_void_p),
+                ("B", c_int), ("T", c_int), ("words", c_int), ("positions", c_void_p), ("mask", c_void_p)]
+
+
+class TreeAcceptArgs(ctypes.Structure):
+    _fields_ = [("parents", c_void_p), ("tokens", c_void_p), ("chosen", c_void_p), ("cu_lens", c_void_p),
+                ("token_bytes", c_int), ("B", c_int), ("T", c_int), ("most", c_int),
+                ("kept", c_void_p), ("kept_lens", c_void_p), ("dropped", c_void_p), ("next_tokens", c_void_p)]
+
+
+class CacheMoveArgs(ctypes.Structure):
+    _fields_ = [("k_caches", POINTER(c_void_p)), ("k_sp", c_int64), ("k_ss", c_int64), ("k_sh", c_int64),
+                ("v_caches", POINTER(c_void_p)), ("v_sp", c_int64), ("v_ss", c_int64), ("v_sh", c_int64),
+                ("block_table", c_void_p), ("t_sb", c_int64), ("cu_lens", c_void_p), ("seq_lens", c_void_p),
+                ("kept", c_void_p), ("layers", c_int), ("B", c_int), ("T", c_int), ("Hk", c_int), ("D", c_int),
+                ("P", c_int), ("page_size", c_int), ("elem_bytes", c_int), ("num_pages", c_int64)]
+
+
 STRUCTS = [PoolArgs, CorrArgs, StatsArgs, SelectArgs, AttnArgs, ScoresArgs, RopePoolArgs, XattnArgs, FlexArgs,
-           PlanArgs, RopeArgs, PagedAttnArgs, WindowAttnArgs]
+           PlanArgs, RopeArgs, PagedAttnArgs, WindowAttnArgs, TreePlanArgs, TreeAcceptArgs, CacheMoveArgs]
 
 ENTRY_POINTS = ["fs_pool", "fs_rope_pool", "fs_corr_work_bytes", "fs_corr", "fs_stats", "fs_scores_work_bytes",
                 "fs_scores", "fs_scores_noalloc", "fs_select", "fs_bsattn_work_bytes",
                 "fs_bsattn", "fs_bsattn_prepare", "fs_bsattn_run", "fs_xattn_work_bytes", "fs_xattn",
                 "fs_flex_work_bytes", "fs_flex", "fs_plan", "fs_rope", "fs_paged_attn_work_bytes", "fs_paged_attn",
-                "fs_window_attn_work_bytes", "fs_window_attn",
+                "fs_window_attn_work_bytes", "fs_window_attn", "fs_tree_plan", "fs_tree_accept", "fs_cache_move",
                 "fs_last_error", "fs_abi_version", "fs_sizeof_args"]
 
 _lib = None
@@ -207,7 +227,9 @@ def load() -> ctypes.CDLL:
                      ("fs_select", SelectArgs), ("fs_bsattn", AttnArgs), ("fs_bsattn_prepare", AttnArgs),
                      ("fs_bsattn_run", AttnArgs), ("fs_xattn", XattnArgs),
                      ("fs_flex", FlexArgs), ("fs_plan", PlanArgs), ("fs_rope", RopeArgs),
-                     ("fs_paged_attn", PagedAttnArgs), ("fs_window_attn", WindowAttnArgs)]:
+                     ("fs_paged_attn", PagedAttnArgs), ("fs_window_attn", WindowAttnArgs),
+                     ("fs_tree_plan", TreePlanArgs), ("fs_tree_accept", TreeAcceptArgs),
+                     ("fs_cache_move", CacheMoveArgs)]:
         fn = getattr(lib, name)
         fn.restype = c_int
         fn.argtypes = [POINTER(st), c_void_p]

@@ -27,7 +27,7 @@ int launch_status(const char* what) {
 }  // namespace fs_host
 
 extern "C" const char* fs_last_error(void) { return fs_host::g_err; }
-extern "C" int fs_abi_version(void) { return 13; }
+extern "C" int fs_abi_version(void) { return 14; }
 
 extern "C" size_t fs_sizeof_args(int which) {
   switch (which) {
@@ -44,6 +44,9 @@ extern "C" size_t fs_sizeof_args(int which) {
     case 10: return sizeof(fs_rope_args);
     case 11: return sizeof(fs_paged_attn_args);
     case 12: return sizeof(fs_window_attn_args);
+    case 13: return sizeof(fs_tree_plan_args);
+    case 14: return sizeof(fs_tree_accept_args);
+    case 15: return sizeof(fs_cache_move_args);
     default: return 0;
   }
 }

@@ -68,6 +68,16 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   // a copy's lane offsets are 32-bit byte offsets over 16 slots
   FS_CHECK_SUPPORTED(a->k_ss >= 0 && a->k_ss < (1 << 23) && a->v_ss >= 0 && a->v_ss < (1 << 23),
                      "%s: slot stride unsupported", fn);
+  const bool e8 = a->k_scale != nullptr;
+  FS_CHECK_ARG(e8 == (a->v_scale != nullptr) && ((uintptr_t)a->k_scale | (uintptr_t)a->v_scale) % 4 == 0,
+               "%s: k_scale and v_scale come together, 4-byte aligned", fn);
+  if (e8)
+    for (int i = 4; i < 10; ++i) FS_CHECK_ARG(st[i] % 16 == 0, "%s: strides of an 8-bit cache must be multiples of 16 elements", fn);
+  if (a->mask) {
+    FS_CHECK_ARG((uintptr_t)a->mask % 8 == 0 && a->mask_words >= 1 && a->mask_words <= (1 << 20) && (uintptr_t)a->positions % 4 == 0,
+                 "%s: mask of %d words per row, positions must be aligned to their size", fn, a->mask_words);
+    FS_CHECK_ARG(!a->window || a->positions, "%s: a window over a tree needs the rows' positions", fn);
+  }
   PagedKArgs k{};
   k.q = static_cast<const uint16_t*>(a->q);
   k.k = static_cast<const uint16_t*>(a->k_cache);
@@ -78,10 +88,17 @@ extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {
   k.table = a->block_table; k.cu = a->cu_lens; k.lens = a->seq_lens; k.t_sb = a->t_sb; k.num_pages = (int)a->num_pages;
   k.B = a->B; k.T = a->T; k.Hq = a->Hq; k.Hk = a->Hk; k.P = a->P; k.page_size = a->page_size;
   k.window = a->window; k.sinks = a->sinks; k.scale = a->softmax_scale;
+  k.ks = a->k_scale; k.vs = a->v_scale;
+  k.mask = reinterpret_cast<const uint32_t*>(a->mask); k.mask_words = 2 * a->mask_words; k.pos = a->positions;
   const uint32_t groups = a->page_size / 16;       // x / groups for x < 2^22, groups <= 256: mulhi is exact
   k.page_magic = groups > 1 ? (uint32_t)((1ull << 32) / groups + 1) : 0;
   const bool few = few_rows(*a);
-  return run<true, 0>(k, a->dtype, a->D, few, true, work_of(*a), static_cast<char*>(a->work), a->B, a->T, (hipStream_t)stream, fn);
+  const Work w = work_of(*a);
+  char* const work = static_cast<char*>(a->work);
+  const hipStream_t s = (hipStream_t)stream;
+  if (e8) return (a->mask ? run_tree8 : run_paged8)(k, a->dtype, a->D, few, w, work, a->B, a->T, s, fn);
+  if (a->mask) return run_tree(k, a->dtype, a->D, few, w, work, a->B, a->T, s, fn);
+  return run<true, 0>(k, a->dtype, a->D, few, true, w, work, a->B, a->T, s, fn);
 }
 
 extern "C" int fs_window_attn(const fs_window_attn_args* a, void* stream) {

@@ -8,6 +8,10 @@
 // are taken off in 64 bits and the sine and cosine of the rest in 32 (its
 // rounding is 2^-25 of a turn).  The rotation is in 32 bits, rounded once.
 //
+// Into a cache in 8 bits (e4m3, a scale for each KV head) goes the rotated key, and the value, over
+// the scale, held to the largest e4m3 number and rounded once, to nearest even; a
+// nan stays one.  It is not rounded to the input type on the way.
+//
 // One pass over q, k and v.  A workgroup takes a few tokens: their angles, one
 // per (token, pair), go to LDS once and serve every head; then each thread moves
 // 16-byte pieces (both of a pair's pieces where they are apart).  A thread keeps its
@@ -58,9 +62,32 @@ __device__ __forceinline__ void store_piece(T* p, const float* x) {
   }
 }
 
+// V elements, over the scale, to e4m3 (inv: 1 / scale)
+template <int V>
+__device__ __forceinline__ void store_piece8(uint8_t* p, const float* x, float inv) {
+  constexpr float kMost = 448.0f;
+  float y[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    y[i] = x[i] * inv;
+    y[i] = y[i] > kMost ? kMost : y[i] < -kMost ? -kMost : y[i];   // a nan stays
+  }
+  if constexpr (V == 1) {
+    *p = (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[0], 0, false);
+  } else {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
+      w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w[i], true);
+    }
+    __builtin_memcpy(__builtin_assume_aligned(p, V), w, V);
+  }
+}
+
 // V: elements of a piece, 16 bytes where every run of dims allows it, else 1.  32768 tokens, 32 / 8 heads of 128: bf16
 // 126 us and f32 249 us (5.3 and 5.4 TB/s); 34 of the dims rotated, by single elements, bf16 421 us (426 interleaved): 1.6 TB/s.
-template <typename T, int V, bool INTER>
+template <typename T, int V, bool INTER, bool E8>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
   constexpr bool TWO = !INTER || V == 1;           // a pair's elements are apart: two loads, two stores
   const fs_rope_args& a = ka.a;
@@ -123,7 +150,9 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
     const bool turn = c < rot;
     const int d = turn ? (INTER ? c * (V > 1 ? V : 2) : c * V) : 2 * a.half + (c - rot) * V;
     const T* src;
-    T* dst;
+    T* dst = nullptr;
+    uint8_t* dst8 = nullptr;                       // in an 8-bit cache
+    float inv = 1.0f;
     if (h < a.Hq) {
       src = static_cast<const T*>(a.q) + (t0 + t) * a.q_st + h * a.q_sh + d;
       dst = static_cast<T*>(a.q_out) + (t0 + t) * a.qo_st + h * a.qo_sh + d;
@@ -133,15 +162,24 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
       if (a.slots != nullptr) {
         const int64_t at = place[t][0];
         if (at < 0) return;                        // no place in the cache
-        dst = static_cast<T*>(a.k_cache) + at + h * a.kc_sh + d;
+        if constexpr (E8) {
+          dst8 = static_cast<uint8_t*>(a.k_cache) + at + h * a.kc_sh + d;
+          inv = 1.0f / a.k_scale[h];
+        } else {
+          dst = static_cast<T*>(a.k_cache) + at + h * a.kc_sh + d;
+        }
       } else {
         dst = static_cast<T*>(a.k_out) + (t0 + t) * a.ko_st + h * a.ko_sh + d;
       }
     }
+    auto store = [&](int off, const float* x) {
+      if (E8 && dst8 != nullptr) store_piece8<V>(dst8 + off, x, inv);
+      else store_piece<T, V>(dst + off, x);
+    };
     float x1[V], y1[V];
     load_piece<T, V>(src, x1);
     if (!turn) {
-      store_piece<T, V>(dst, x1);
+      store(0, x1);
       return;
     }
     if constexpr (TWO) {
@@ -154,8 +192,8 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
         y1[e] = x1[e] * f.x - x2[e] * f.y;
         y2[e] = x2[e] * f.x + x1[e] * f.y;
       }
-      store_piece<T, V>(dst, y1);
-      store_piece<T, V>(dst + apart, y2);
+      store(0, y1);
+      store(apart, y2);
     } else {
       const float2* w = cs + t * a.half + c * (V / 2);
 #pragma unroll
@@ -164,7 +202,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
         y1[2 * e] = x1[2 * e] * f.x - x1[2 * e + 1] * f.y;
         y1[2 * e + 1] = x1[2 * e + 1] * f.x + x1[2 * e] * f.y;
       }
-      store_piece<T, V>(dst, y1);
+      store(0, y1);
     }
   });
   if (a.v == nullptr) return;
@@ -173,16 +211,17 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeKArgs ka) {
     if (at < 0) return;
     float x[V];
     load_piece<T, V>(static_cast<const T*>(a.v) + (t0 + t) * a.v_st + h * a.v_sh + c * V, x);
-    store_piece<T, V>(static_cast<T*>(a.v_cache) + at + h * a.vc_sh + c * V, x);
+    if constexpr (E8) store_piece8<V>(static_cast<uint8_t*>(a.v_cache) + at + h * a.vc_sh + c * V, x, 1.0f / a.v_scale[h]);
+    else store_piece<T, V>(static_cast<T*>(a.v_cache) + at + h * a.vc_sh + c * V, x);
   });
 }
 
-template <typename T>
+template <typename T, bool E8>
 static int launch_rope(const fs_rope_args& a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const bool wide = a.D % V == 0 && (a.interleaved ? 2 * a.half : a.half) % V == 0;
-  auto f = a.interleaved ? (wide ? rope_kernel<T, V, true> : rope_kernel<T, 1, true>)
-                         : (wide ? rope_kernel<T, V, false> : rope_kernel<T, 1, false>);
+  auto f = a.interleaved ? (wide ? rope_kernel<T, V, true, E8> : rope_kernel<T, 1, true, E8>)
+                         : (wide ? rope_kernel<T, V, false, E8> : rope_kernel<T, 1, false, E8>);
   // Long calls: 2 tokens to a workgroup, 4 where a piece is 16 bytes (32768 tokens, half: 126 us against 131 with 4; 8191
   // interleaved, half of the head: 29.7 against 32.0 with 2).  Few tokens: their heads over several workgroups, so that a
   // thread has one piece to wait for.
@@ -223,10 +262,16 @@ extern "C" int fs_rope(const fs_rope_args* a, void* stream) {
   for (const void* p : ptrs) FS_CHECK_ARG((uintptr_t)p % 16 == 0, "fs_rope: tensors must be 16-byte aligned");
   FS_CHECK_ARG((uintptr_t)a->positions % a->pos_bytes == 0 && (uintptr_t)a->inv_freq % 8 == 0 &&
                    (uintptr_t)a->slots % 8 == 0, "fs_rope: positions, inv_freq and slots must be aligned to their size");
+  const bool e8 = a->k_scale != nullptr;
+  FS_CHECK_ARG(e8 == (a->v_scale != nullptr) && (!e8 || cached) &&
+                   ((uintptr_t)a->k_scale | (uintptr_t)a->v_scale) % 4 == 0,
+               "fs_rope: k_scale and v_scale come together, with slots, 4-byte aligned");
+  if (e8)
+    for (int i = 10; i < 16; ++i) FS_CHECK_ARG(st[i] % 16 == 0, "fs_rope: strides of an 8-bit cache must be multiples of 16 elements");
   const hipStream_t s = (hipStream_t)stream;
   switch (a->dtype) {
-    case FS_DTYPE_BF16: return launch_rope<bf16_t>(*a, s);
-    case FS_DTYPE_F16: return launch_rope<f16_t>(*a, s);
-    default: return launch_rope<float>(*a, s);
+    case FS_DTYPE_BF16: return e8 ? launch_rope<bf16_t, true>(*a, s) : launch_rope<bf16_t, false>(*a, s);
+    case FS_DTYPE_F16: return e8 ? launch_rope<f16_t, true>(*a, s) : launch_rope<f16_t, false>(*a, s);
+    default: return e8 ? launch_rope<float, true>(*a, s) : launch_rope<float, false>(*a, s);
   }
 }

@@ -1,0 +1,242 @@
+// Trees of drafted tokens: their positions and masks, the path that the model's choices keep, and
+// the kept tokens' rows moved to their places in the cache.
+//
+// All three are bound by latency: a batch's tokens are some kilobytes, so what counts is the
+// chain of loads that wait for each other.  One workgroup takes a request (its lengths, then its tokens,
+// side by side), follows parents and children in LDS, and writes.
+#include <algorithm>
+#include <climits>
+
+#include "common.h"
+
+namespace fs {
+
+constexpr int kTreeThreads = 256;
+constexpr int kTreeMost = 1024;                    // tokens of a request that are looked at
+
+// Request b's rows c0 .. c0 + n - 1, within 0 .. T; n <= 0: none.
+struct TreeRows {
+  int c0, n;
+  __device__ __forceinline__ TreeRows(const int32_t* cu, int b, int T) {
+    c0 = min(max(cu[b], 0), T);
+    n = min(max(cu[b + 1], 0), T) - c0;
+  }
+};
+
+// Row t's ancestors are followed one by one; they come in falling order, so the words of its mask do
+// too and each is written once.
+__global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_args a) {
+  __shared__ int par[kTreeMost];
+  const int tid = threadIdx.x, b = blockIdx.x;
+  if (b == a.B) {                                  // rows that no request has
+    for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) {
+      a.positions[t] = -1;
+      for (int w = 0; w < a.words; ++w) a.mask[(int64_t)t * a.words + w] = 0;
+    }
+    return;
+  }
+  const TreeRows r(a.cu_lens, b, a.T);
+  const int64_t first = (int64_t)a.seq_lens[b] - r.n;
+  const int most = min(r.n, 64 * a.words);
+  for (int t = tid; t < most; t += kTreeThreads) par[t] = a.parents[r.c0 + t];
+  __syncthreads();
+  for (int t = tid; t < r.n; t += kTreeThreads) {
+    int64_t* row = a.mask + (int64_t)(r.c0 + t) * a.words;
+    int w = a.words, at = t, depth = 0;
+    uint64_t word = 0;
+    while (t < most) {
+      if (at >> 6 != w) {
+        if (w < a.words) row[w] = (int64_t)word;
+        while (--w > at >> 6) row[w] = 0;
+        word = 0;
+      }
+      word |= 1ull << (at & 63);
+      const int p = par[at];
+      if (p < 0 || p >= at) break;
+      at = p;
+      ++depth;
+    }
+    if (w < a.words) row[w] = (int64_t)word;
+    while (--w >= 0) row[w] = 0;
+    a.positions[r.c0 + t] = t < most ? (int)(first + depth) : -1;
+  }
+}
+
+// Every token that its parent's choice agrees with names itself to the parent, which keeps the lowest; one
+// thread follows those names from the first token on.
+template <typename I>
+__global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accept_args a) {
+  __shared__ int child[kTreeMost], path[kTreeMost];
+  __shared__ int count;
+  const int tid = threadIdx.x, b = blockIdx.x;
+  if (b == a.B) {
+    for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) a.kept[t] = -1;
+    return;
+  }
+  const I *tokens = static_cast<const I*>(a.tokens), *chosen = static_cast<const I*>(a.chosen);
+  const TreeRows r(a.cu_lens, b, a.T);
+  const int most = min(r.n, a.most);
+  for (int t = tid; t < most; t += kTreeThreads) child[t] = INT_MAX;
+  __syncthreads();
+  for (int t = tid; t < most; t += kTreeThreads) {
+    const int p = a.parents[r.c0 + t];
+    if (p < 0 || p >= t) continue;
+    const I x = tokens[r.c0 + t];
+    if (x < 0 || x == chosen[r.c0 + p]) atomicMin(&child[p], t);   // the least of them, in whatever order
+  }
+  __syncthreads();
+  if (tid == 0) {
+    int k = 0;
+    for (int t = 0; t < most; t = child[t]) path[k++] = t;
+    count = k;
+    a.kept_lens[b] = k;
+    a.dropped[b] = k - max(r.n, 0);
+    static_cast<I*>(a.next_tokens)[b] = k ? chosen[r.c0 + path[k - 1]] : (I)-1;
+  }
+  __syncthreads();
+  for (int t = tid; t < r.n; t += kTreeThreads) a.kept[r.c0 + t] = t < count ? path[t] : -1;
+}
+
+constexpr int kMoveLayers = 64;                    // of a launch
+struct MoveKArgs {
+  fs_cache_move_args a;
+  char* caches[2][kMoveLayers];                    // [K, V]
+};
+
+// A workgroup moves one request's rows in one cache.  Rows are read some at a time, all of them before any is
+// written: the place of row i may be that of a row j > i that another thread still has to read.  (Rows of later
+// steps lie behind every place written so far: j >= i.)
+__global__ __launch_bounds__(kTreeThreads) void cache_move_kernel(MoveKArgs ka) {
+  constexpr int HELD = 4;                          // pieces of 16 bytes of a thread
+  const fs_cache_move_args& a = ka.a;
+  __shared__ int64_t from[kTreeMost], to[kTreeMost];   // offsets in elements, -1: stays
+  __shared__ int lo, hi;
+  const int tid = threadIdx.x, b = blockIdx.x, v = blockIdx.y & 1, layer = blockIdx.y >> 1;
+  const int64_t sp = v ? a.v_sp : a.k_sp, ss = v ? a.v_ss : a.k_ss, sh = v ? a.v_sh : a.k_sh;
+  const TreeRows r(a.cu_lens, b, a.T);
+  const int n = min(r.n, kTreeMost);
+  const int64_t first = (int64_t)a.seq_lens[b] - r.n;
+  if (tid == 0) {
+    lo = INT_MAX;
+    hi = -1;
+  }
+  __syncthreads();
+  auto place = [&](int i) -> int64_t {
+    const int64_t s = first + i;
+    if (s < 0 || s >= (int64_t)a.P * a.page_size) return -1;
+    const int pg = (int)s / a.page_size, e = a.block_table[b * a.t_sb + pg];
+    return e >= 0 && e < a.num_pages ? e * sp + ((int)s - pg * a.page_size) * ss : -1;
+  };
+  for (int i = tid; i < n; i += kTreeThreads) {
+    const int j = a.kept[r.c0 + i];
+    int64_t f = -1, t = -1;
+    if (j > i && j < n) {
+      f = place(j);
+      t = place(i);
+      if (f < 0 || t < 0) f = t = -1;
+    }
+    from[i] = f;
+    to[i] = t;
+    if (f >= 0) {
+      atomicMin(&lo, i);
+      atomicMax(&hi, i);
+    }
+  }
+  __syncthreads();
+  char* const base = ka.caches[v][layer];
+  const int per_head = a.D * a.elem_bytes / 16, pieces = a.Hk * per_head;   // 16-byte pieces
+  const int rows = max(HELD * kTreeThreads / pieces, 1);                    // read at a time
+  for (int i0 = lo; i0 <= hi; i0 += rows) {
+    const int items = min(rows, hi + 1 - i0) * pieces;
+    // more pieces than are held (wide rows): columns one part after the other, each in the rows' order
+    for (int c0 = 0; c0 < items; c0 += HELD * kTreeThreads) {
+      uint4 held[HELD];
+      char* dst[HELD];
+#pragma unroll
+      for (int k = 0; k < HELD; ++k) {
+        const int x = c0 + k * kTreeThreads + tid;
+        dst[k] = nullptr;
+        if (x < items) {
+          const int i = x / pieces, c = x - i * pieces, h = c / per_head, d = c - h * per_head;
+          if (from[i0 + i] >= 0) {
+            held[k] = *reinterpret_cast<const uint4*>(base + (from[i0 + i] + h * sh) * a.elem_bytes + d * 16);
+            dst[k] = base + (to[i0 + i] + h * sh) * a.elem_bytes + d * 16;
+          }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < HELD; ++k)
+        if (dst[k] != nullptr) *reinterpret_cast<uint4*>(dst[k]) = held[k];
+    }
+  }
+}
+
+}  // namespace fs
+
+using namespace fs;
+
+static int check_tree(const char* fn, int B, int T) {
+  FS_CHECK_ARG(B >= 1 && T >= 0, "%s: B=%d requests, T=%d rows", fn, B, T);
+  FS_CHECK_SUPPORTED(B <= 65535, "%s: %d requests > 65535", fn, B);
+  return FS_OK;
+}
+
+extern "C" int fs_tree_plan(const fs_tree_plan_args* a, void* stream) {
+  const char* fn = "fs_tree_plan";
+  FS_CHECK_ARG(a != nullptr, "%s: null args", fn);
+  if (int rc = check_tree(fn, a->B, a->T)) return rc;
+  FS_CHECK_ARG(a->words >= 1, "%s: %d words", fn, a->words);
+  FS_CHECK_SUPPORTED(a->words <= kTreeMost / 64, "%s: trees of %d tokens > %d", fn, 64 * a->words, kTreeMost);
+  if (a->T == 0) return FS_OK;
+  FS_CHECK_ARG(a->parents && a->cu_lens && a->seq_lens && a->positions && a->mask, "%s: null tensor pointer", fn);
+  tree_plan_kernel<<<a->B + 1, kTreeThreads, 0, (hipStream_t)stream>>>(*a);
+  return fs_host::launch_status(fn);
+}
+
+extern "C" int fs_tree_accept(const fs_tree_accept_args* a, void* stream) {
+  const char* fn = "fs_tree_accept";
+  FS_CHECK_ARG(a != nullptr, "%s: null args", fn);
+  if (int rc = check_tree(fn, a->B, a->T)) return rc;
+  FS_CHECK_ARG(a->token_bytes == 4 || a->token_bytes == 8, "%s: tokens of %d bytes", fn, a->token_bytes);
+  FS_CHECK_ARG(a->most >= 1, "%s: trees of %d tokens", fn, a->most);
+  FS_CHECK_SUPPORTED(a->most <= kTreeMost, "%s: trees of %d tokens > %d", fn, a->most, kTreeMost);
+  FS_CHECK_ARG(a->cu_lens && a->kept_lens && a->dropped && a->next_tokens &&
+                   (a->T == 0 || (a->parents && a->tokens && a->chosen && a->kept)), "%s: null tensor pointer", fn);
+  if (a->token_bytes == 8) tree_accept_kernel<int64_t><<<a->B + 1, kTreeThreads, 0, (hipStream_t)stream>>>(*a);
+  else tree_accept_kernel<int32_t><<<a->B + 1, kTreeThreads, 0, (hipStream_t)stream>>>(*a);
+  return fs_host::launch_status(fn);
+}
+
+extern "C" int fs_cache_move(const fs_cache_move_args* a, void* stream) {
+  const char* fn = "fs_cache_move";
+  FS_CHECK_ARG(a != nullptr, "%s: null args", fn);
+  if (int rc = check_tree(fn, a->B, a->T)) return rc;
+  FS_CHECK_ARG(a->layers >= 0 && a->Hk >= 1 && a->D >= 1 && a->P >= 1 && a->page_size >= 1 && a->num_pages >= 1,
+               "%s: layers=%d Hk=%d D=%d P=%d page_size=%d num_pages=%lld", fn, a->layers, a->Hk, a->D, a->P, a->page_size,
+               (long long)a->num_pages);
+  FS_CHECK_ARG(a->elem_bytes == 1 || a->elem_bytes == 2 || a->elem_bytes == 4, "%s: elements of %d bytes", fn, a->elem_bytes);
+  FS_CHECK_SUPPORTED((int64_t)a->Hk * a->D <= (1 << 20) && (int64_t)a->D * a->elem_bytes % 16 == 0,
+                     "%s: rows of %d heads of %d unsupported (multiples of 16 bytes)", fn, a->Hk, a->D);
+  FS_CHECK_SUPPORTED((int64_t)a->P * a->page_size <= INT_MAX, "%s: %d pages of %d tokens per request unsupported", fn,
+                     a->P, a->page_size);
+  if (a->T == 0 || a->layers == 0) return FS_OK;
+  const int64_t st[] = {a->k_sp, a->k_ss, a->k_sh, a->v_sp, a->v_ss, a->v_sh};
+  for (int64_t x : st) FS_CHECK_ARG(x * a->elem_bytes % 16 == 0, "%s: strides must be multiples of 16 bytes", fn);
+  FS_CHECK_ARG(a->k_caches && a->v_caches && a->block_table && a->cu_lens && a->seq_lens && a->kept && a->t_sb >= a->P,
+               "%s: null tensor pointer, or row stride %lld of %d", fn, (long long)a->t_sb, a->P);
+  for (int i = 0; i < a->layers; ++i)
+    FS_CHECK_ARG(a->k_caches[i] && a->v_caches[i] && ((uintptr_t)a->k_caches[i] | (uintptr_t)a->v_caches[i]) % 16 == 0,
+                 "%s: caches must be given, 16-byte aligned", fn);
+  for (int l0 = 0; l0 < a->layers; l0 += kMoveLayers) {
+    MoveKArgs k{*a, {}};
+    const int n = std::min(a->layers - l0, kMoveLayers);
+    for (int i = 0; i < n; ++i) {
+      k.caches[0][i] = static_cast<char*>(a->k_caches[l0 + i]);
+      k.caches[1][i] = static_cast<char*>(a->v_caches[l0 + i]);
+    }
+    cache_move_kernel<<<dim3(a->B, 2 * n), kTreeThreads, 0, (hipStream_t)stream>>>(k);
+    if (int rc = fs_host::launch_status(fn)) return rc;
+  }
+  return FS_OK;
+}

@@ -13,6 +13,11 @@ strides that are multiples of 8 elements with d contiguous, e.g. [pages, Hk,
 page_size, D] storage transposed).  Token t of request b is in slot t %
 page_size of page block_table[b, t // page_size].
 
+A cache of ``torch.float8_e4m3fn`` with one scale for each KV head (``k_scale``,
+``v_scale``, float32 [Hk]: a number x stands for x * scale) takes half the place
+and, in decoding, about half the time.  Requests whose new tokens are a tree of
+drafts instead of a chain: ``fftsparse_amd.tree``.
+
 ``window_attention`` is the attention's sliding-window rule on contiguous
 [B, H, L, D] tensors, beside ``block_sparse_attention``.  No counterpart in the
 reference, which serves decoding from the model's own cache.  Inference only:
@@ -31,6 +36,7 @@ from ._lib import PagedAttnArgs, PlanArgs, WindowAttnArgs
 from .attn import _check_layout
 
 _INT32_MAX = 2 ** 31 - 1
+E4M3 = torch.float8_e4m3fn
 
 
 def _inference_only(name: str, *tensors) -> None:
@@ -47,11 +53,16 @@ def _strides(t: torch.Tensor):
 
 
 def _aligned(t: torch.Tensor, st) -> bool:
-    """Whether the kernels can read t as it is: d contiguous, 16-byte rows."""
-    bits = t.data_ptr() >> 1 if st[-1] == 1 else 1
+    """Whether the kernels can read t as it is: d contiguous, 16-byte rows (for elements of 4 bytes: 32)."""
+    if st[-1] != 1:
+        return False
+    if t.dtype == E4M3:
+        bits, m = t.data_ptr(), 15
+    else:
+        bits, m = t.data_ptr() >> 1, 7
     for s in st[:-1]:
         bits |= s
-    return not bits & 7
+    return not bits & m
 
 
 def _rows(t: torch.Tensor, name: str):
@@ -72,8 +83,8 @@ def _written(t: torch.Tensor, name: str, shape, dtype):
     st = _strides(t)
     if not _aligned(t, st) or (0 in st and any(n > 1 and s == 0 for n, s in zip(shape, st))):
         if t.numel():
-            raise ValueError(f"{name} must have d contiguous, strides that are multiples of 8 elements and 16-byte "
-                             f"alignment, and no broadcast dimension, got strides {t.stride()}")
+            raise ValueError(f"{name} must have d contiguous, strides that are multiples of {16 if dtype == E4M3 else 8} "
+                             f"elements and 16-byte alignment, and no broadcast dimension, got strides {t.stride()}")
     return st
 
 
@@ -105,6 +116,21 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype, Hk=None, D=None):
     if v.dtype == dtype and v.shape == shape and v.stride() == k.stride() and not v.data_ptr() & 15:
         return want, ks, ks                        # laid out as k_cache is
     return want, ks, _written(v, "v_cache", want, dtype)
+
+
+def _scales(k_scale, v_scale, dtype, Hk: int) -> bool:
+    """Whether scales come with caches of a type (as they must in 8 bits, and only then)."""
+    if dtype != E4M3:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"k_scale and v_scale go with caches of {E4M3}, got {dtype}")
+        return False
+    if k_scale is None or v_scale is None:
+        raise ValueError(f"caches of {E4M3} need k_scale and v_scale")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        if t.shape != (Hk,) or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous float32 tensor of {Hk} scales, one for each KV head, got "
+                             f"{t.dtype} {tuple(t.shape)}")
+    return True
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -193,8 +219,10 @@ def _scale(scale, D: int) -> float:
     return scale
 
 
-def _attn_dtype(q, k, v) -> None:
+def _attn_dtype(q, k, v, cached: bool = False) -> None:
     dt = q.dtype
+    if cached and k.dtype == v.dtype == E4M3 and (dt == torch.bfloat16 or dt == torch.float16):
+        return
     if (dt != torch.bfloat16 and dt != torch.float16) or k.dtype != dt or v.dtype != dt:
         raise TypeError(f"expected bf16 or f16 tensors of one type, got {[t.dtype for t in (q, k, v)]}")
 
@@ -202,6 +230,7 @@ def _attn_dtype(q, k, v) -> None:
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     cu_lens: torch.Tensor, seq_lens: torch.Tensor, *, max_new: int | None = None,
                     window: int | None = None, sinks: int = 0, softmax_scale: float | None = None,
+                    k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of the new tokens of a batch of requests over their paged caches.
 
@@ -221,11 +250,23 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     a value of v that is not finite may reach rows of its request that do not see
     it.  Scores, maxima and sums are in 32 bits; the weights are rounded to the input
     type before the product with v (values up to 2^93).  ``out`` may be q.  Up to 4096
-    requests of 2^26 tokens."""
+    requests of 2^26 tokens.
+
+    Caches of ``torch.float8_e4m3fn`` need ``k_scale`` and ``v_scale`` (float32 [Hk],
+    positive and finite): a number x of KV head h stands for x * scale[h].  It is
+    taken exactly; queries and weights are not rounded further."""
+    return _attend("paged_attention", q, k_cache, v_cache, block_table, cu_lens, seq_lens, None, None, max_new, window, sinks,
+                   softmax_scale, k_scale, v_scale, out)
+
+
+def _attend(name, q, k_cache, v_cache, block_table, cu_lens, seq_lens, mask, positions, max_new, window, sinks, softmax_scale,
+            k_scale, v_scale, out):
+    """``paged_attention``, and ``tree_attention`` (mask given)."""
     q, qs = _rows(q, "q")
     T, Hq, D = q.shape
-    _attn_dtype(q, k_cache, v_cache)
-    (pages, ps, Hk, _), ks, vs = _caches(k_cache, v_cache, q.dtype, D=D)
+    _attn_dtype(q, k_cache, v_cache, True)
+    (pages, ps, Hk, _), ks, vs = _caches(k_cache, v_cache, k_cache.dtype, D=D)
+    scaled = _scales(k_scale, v_scale, k_cache.dtype, Hk)
     if Hk == 0 or Hq % Hk or Hq == 0:
         raise ValueError(f"query heads {Hq} must be a multiple of key heads {Hk}")
     t = block_table
@@ -236,14 +277,23 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scale = _scale(softmax_scale, D)
     if max_new is not None and int(max_new) < 1:
         raise ValueError(f"max_new must be at least 1, got {max_new}")
-    _inference_only("paged_attention", q, k_cache, v_cache)
+    more = (k_scale, v_scale) if scaled else ()
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != T or not mask.shape[1] or mask.dtype != torch.int64 or not mask.is_contiguous():
+            raise ValueError(f"mask must be a contiguous int64 [{T}, words] tensor, got {mask.dtype} {tuple(mask.shape)}")
+        more += (mask,)
+        if window:
+            if positions is None:
+                raise ValueError("a window over a tree needs the tokens' positions")
+            more += (_ints(positions, "positions", (T,)),)
+    _inference_only(name, q, k_cache, v_cache)
     if out is None:
-        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens)
+        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, *more)
         out = q.new_empty((T, Hq, D))
         os_ = (Hq * D, D)
     else:
         os_ = _written(out, "out", (T, Hq, D), q.dtype)
-        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, out)
+        dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, out, *more)
     if T == 0:
         return out
     args = PagedAttnArgs(
@@ -254,6 +304,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         seq_lens=seq_lens.data_ptr(), dtype=_lib.FS_DTYPE[q.dtype], B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=P, page_size=ps,
         num_pages=pages, max_new=0 if max_new is None else min(int(max_new), T), window=window, sinks=sinks,
         softmax_scale=scale)
+    if scaled:
+        args.k_scale, args.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+    if mask is not None:
+        args.mask, args.mask_words = mask.data_ptr(), mask.shape[1]
+        if window:
+            args.positions = positions.data_ptr()
     work = q.new_empty(_lib.load().fs_paged_attn_work_bytes(ctypes.byref(args)), dtype=torch.uint8)
     args.work = work.data_ptr()
     _lib.call("fs_paged_attn", args, dev)

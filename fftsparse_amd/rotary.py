@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from ._lib import RopeArgs
-from .paged import _caches, _inference_only, _ints, _rows, _written
+from .paged import E4M3, _caches, _inference_only, _ints, _rows, _scales, _written
 
 
 def rope_frequencies(rotary_dim: int, *, base: float = 10000.0, scaling: str | None = None, factor: float = 1.0,
@@ -125,25 +125,32 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
 
 def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                k_cache: torch.Tensor, v_cache: torch.Tensor, inv_freq: torch.Tensor, *, attention_factor: float = 1.0,
-               interleaved: bool = False, q_out: torch.Tensor | None = None) -> torch.Tensor:
+               interleaved: bool = False, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None) -> torch.Tensor:
     """``rope`` of q and k, with the rotated keys and the values v [T, Hk, D] written to ``slots`` (int64 [T], from
     ``plan_step``: page * page_size + slot, all different) of ``k_cache`` / ``v_cache`` [pages, page_size, Hk, D].
     Returns q_rot.  A slot outside the cache (-1: none) is not written; a row with a negative position is left as it
-    was, in the cache too."""
+    was, in the cache too.
+
+    Caches of ``torch.float8_e4m3fn`` need ``k_scale`` and ``v_scale`` (float32 [Hk], positive and finite): x / scale[h] is
+    written, held to -448 .. 448 and rounded once, from 32 bits (nan stays nan)."""
     q, qs, k, ks, inv_freq = _common("rope_cache", q, k, positions, inv_freq)
     v, vs = _rows(v, "v")
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"value {v.dtype} {tuple(v.shape)} must be like key {k.dtype} {tuple(k.shape)}")
     _ints(slots, "slots", (q.shape[0],), (torch.int64,))
-    shape, kc, vc = _caches(k_cache, v_cache, q.dtype, k.shape[1], k.shape[2])
+    shape, kc, vc = _caches(k_cache, v_cache, E4M3 if k_cache.dtype == E4M3 else q.dtype, k.shape[1], k.shape[2])
+    scaled = _scales(k_scale, v_scale, k_cache.dtype, k.shape[1])
     _inference_only("rope_cache", v, k_cache, v_cache)
     q_out, os_ = _out(q_out, "q_out", q)
-    dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out)
+    dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out, k_scale, v_scale)
     if q.shape[0]:
         a = _args(q, qs, k, ks, q_out, os_, positions, inv_freq, attention_factor, interleaved)
         a.v, a.v_st, a.v_sh, a.slots = v.data_ptr(), vs[0], vs[1], slots.data_ptr()
         a.k_cache, a.kc_sp, a.kc_ss, a.kc_sh = k_cache.data_ptr(), kc[0], kc[1], kc[2]
         a.v_cache, a.vc_sp, a.vc_ss, a.vc_sh = v_cache.data_ptr(), vc[0], vc[1], vc[2]
         a.num_pages, a.page_size = shape[0], shape[1]
+        if scaled:
+            a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         _lib.call("fs_rope", a, dev)
     return q_out

@@ -29,7 +29,8 @@
  *                                            Xattention_prefill (:306-406) hands to block_sparse_attn_func
  *   fs_flex      FlexPrefill's selector       attn_src/Flexprefill.py:946-1061 (get_active_blocks), the
  *                                            block index sets its Flexprefill_prefill (:1063-1098) attends
- *   fs_plan, fs_rope, fs_paged_attn, fs_window_attn: no counterpart (serving over a paged cache after the prefill)
+ *   fs_plan, fs_rope, fs_paged_attn, fs_window_attn, fs_tree_plan, fs_tree_accept, fs_cache_move: no
+ *                counterpart (serving over a paged cache after the prefill)
  *   fs_bsattn    block_sparse_attn_func call  my_attn_v7.py:775-786, fix_mask_attn/my_attn.py:196-207
  *                flash_attn_func(causal=True) my_attn_v7.py:509-519 (blk_cnt == NULL: dense causal)
  */
@@ -440,7 +441,11 @@ FS_API int fs_plan(const fs_plan_args* a, void* stream);
  * too); a slot outside 0 .. num_pages * page_size - 1 is not written.
  * positions: int32 or int64 (pos_bytes 4 or 8).  dtype f32, bf16 or f16; D a
  * multiple of 8 up to 512, half <= 128; 16-byte pieces where D and the rotated
- * part allow them (single elements otherwise). */
+ * part allow them (single elements otherwise).
+ * k_scale and v_scale (both, with slots): the caches are in e4m3, and the rotated
+ * key and the value of KV head h are written as x / scale[h], held to -448 .. 448
+ * and rounded once from 32 bits to nearest even (nan stays nan).  Scales are
+ * positive and finite; cache strides multiples of 16 elements. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   const void* k; int64_t k_st, k_sh;
@@ -457,6 +462,8 @@ typedef struct {
   void* v_cache; int64_t vc_sp, vc_ss, vc_sh;
   int64_t num_pages;
   int page_size;
+  const float* k_scale;                  /* [Hk], or NULL: the caches are of dtype */
+  const float* v_scale;
 } fs_rope_args;
 FS_API int fs_rope(const fs_rope_args* a, void* stream);
 
@@ -485,7 +492,17 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * any of T, B, Hq, Hk, D, P, page_size and max_new grows (0: T), so one sized for
  * the largest of each serves every call: about 9 MB where max_new * Hq <= 32, else
  * 68 MB (D = 64: 35) and T * Hq / 4 bytes.  Calls that overlap on one workspace
- * race. */
+ * race.
+ * k_scale and v_scale (both): the caches are in e4m3, and a number x of KV head h
+ * stands for x * scale[h] (positive and finite); cache strides are multiples of 16
+ * elements.  Scores are of q in dtype and the e4m3 numbers, exact in dtype.
+ * mask: the rows of a request are not a chain but a tree, or any other set.  The row
+ * sees the tokens before the request's n new ones, and new token j of its request (the
+ * one at seq_lens[b] - n + j) where bit j % 64 of word j / 64 of its row of the mask
+ * is set, itself included only so.  New tokens past the mask's words are seen by none.
+ * With a window the tokens before the new ones are seen by the row's position
+ * (positions[t], taken within those of the new tokens) as above, the new ones by the
+ * mask alone. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   void* out; int64_t o_st, o_sh;
@@ -499,6 +516,11 @@ typedef struct {
   int max_new, window, sinks;
   float softmax_scale;
   void* work;
+  const float* k_scale;                       /* [Hk], or NULL: the caches are of dtype */
+  const float* v_scale;
+  const int64_t* mask;                        /* [T][mask_words], or NULL: causal */
+  int mask_words;
+  const int32_t* positions;                   /* [T]: with mask and a window */
 } fs_paged_attn_args;
 FS_API size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a);
 FS_API int fs_paged_attn(const fs_paged_attn_args* a, void* stream);
@@ -524,10 +546,70 @@ typedef struct {
 FS_API size_t fs_window_attn_work_bytes(const fs_window_attn_args* a);
 FS_API int fs_window_attn(const fs_window_attn_args* a, void* stream);
 
+/* ---- trees of drafted tokens ------------------------------------------------
+ * The n = cu_lens[b + 1] - cu_lens[b] new tokens of request b are a tree: parents[t]
+ * is the index (0 .. n - 1, within the request) of the token that row t's follows,
+ * below its own; anything else means that it follows the request's tokens before.
+ * fs_tree_plan: positions[t] = seq_lens[b] - n + the number of t's ancestors, and bit
+ * j of mask row t (words of 64) set for t itself and its ancestors.  Rows that no
+ * request has, and a request's tokens from 64 words on, get position -1 and no bit.
+ * words <= 16. */
+typedef struct {
+  const int32_t* parents;                /* [T] */
+  const int32_t* cu_lens;                /* [B + 1] */
+  const int32_t* seq_lens;               /* [B], new tokens included */
+  int B, T, words;
+  int32_t* positions;                    /* [T] */
+  int64_t* mask;                         /* [T][words] */
+} fs_tree_plan_args;
+FS_API int fs_tree_plan(const fs_tree_plan_args* a, void* stream);
+
+/* Which of them are kept.  chosen[t] is the token that the model takes after row t's.
+ * A request's first new token is kept; another one is if its parent is, and its token is
+ * chosen[parent] or negative (given, not drafted), and no sibling before it is.  So the
+ * kept tokens are a path from the first one on.
+ *   kept [T]         row cu_lens[b] + i: the index of request b's i-th kept token, -1 past them;
+ *   kept_lens [B]    how many are kept;
+ *   dropped [B]      kept_lens[b] - n: fs_plan's new_lens, which takes the others back;
+ *   next_tokens [B]  chosen[the last kept one], -1 for a request without new tokens.
+ * Of a request only the first `most` (<= 1024) tokens are looked at; the others are not
+ * kept.  tokens, chosen and next_tokens are int32 or int64 (token_bytes 4 or 8). */
+typedef struct {
+  const int32_t* parents;                /* [T] */
+  const void* tokens;                    /* [T] */
+  const void* chosen;                    /* [T] */
+  const int32_t* cu_lens;                /* [B + 1] */
+  int token_bytes, B, T, most;
+  int32_t* kept;
+  int32_t* kept_lens;
+  int32_t* dropped;
+  void* next_tokens;
+} fs_tree_accept_args;
+FS_API int fs_tree_accept(const fs_tree_accept_args* a, void* stream);
+
+/* The kept tokens' keys and values to where they belong: for every request and i with
+ * j = kept[cu_lens[b] + i] > i (j below n; the j rise with i), the rows of its new token
+ * j in the cache go to the place of its new token i, in each of `layers` pairs of caches
+ * of the same shape and strides (k_caches, v_caches: host arrays of device pointers).
+ * elem_bytes 1, 2 or 4; rows of D * elem_bytes, a multiple of 16 bytes, strides too.
+ * Tokens whose page is none stay.  Of a request only the first 1024 tokens are looked
+ * at. */
+typedef struct {
+  void* const* k_caches; int64_t k_sp, k_ss, k_sh;
+  void* const* v_caches; int64_t v_sp, v_ss, v_sh;
+  const int32_t* block_table; int64_t t_sb;   /* [B][P] */
+  const int32_t* cu_lens;                     /* [B + 1] */
+  const int32_t* seq_lens;                    /* [B], new tokens included */
+  const int32_t* kept;                        /* [T] */
+  int layers, B, T, Hk, D, P, page_size, elem_bytes;
+  int64_t num_pages;
+} fs_cache_move_args;
+FS_API int fs_cache_move(const fs_cache_move_args* a, void* stream);
+
 /* Description of the last failure on this thread ("" if none). */
 FS_API const char* fs_last_error(void);
 /* sizeof the argument struct: 0 pool, 1 corr, 2 stats, 3 select, 4 attn, 5 scores, 6 rope_pool, 7 xattn,
- * 8 flex, 9 plan, 10 rope, 11 paged_attn, 12 window_attn
+ * 8 flex, 9 plan, 10 rope, 11 paged_attn, 12 window_attn, 13 tree_plan, 14 tree_accept, 15 cache_move
  * (lets a foreign-function binding check its struct layout). */
 FS_API size_t fs_sizeof_args(int which);
 /* ABI version of this library (increments on any struct change). */
