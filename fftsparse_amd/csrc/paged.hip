@@ -31,18 +31,21 @@ static bool few_rows(const fs_window_attn_args& a) {
   const int G = a.Hq / a.Hk;
   return few_rows(a.Lq, G, ((int64_t)a.B * a.Lq * G / 32 + a.B) * a.Hk, a.Lk);
 }
-static Work work_of(const fs_paged_attn_args& a) { return work_of(few_rows(a), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D); }
+static int form_of(const fs_paged_attn_args& a) { return (a.k_scale ? k8 : 0) | (a.mask ? kTree : 0); }
+static Work work_of(const fs_paged_attn_args& a) {
+  return work_of(few_rows(a), a.T, a.B, a.Hk, a.Hq / a.Hk, a.D, form_of(a));
+}
 static Work work_of(const fs_window_attn_args& a) {
-  return work_of(few_rows(a), (int64_t)a.B * a.Lq, a.B, a.Hk, a.Hq / a.Hk, a.D);
+  return work_of(few_rows(a), (int64_t)a.B * a.Lq, a.B, a.Hk, a.Hq / a.Hk, a.D, 0);
 }
 
 extern "C" size_t fs_paged_attn_work_bytes(const fs_paged_attn_args* a) {
   if (!a || a->B <= 0 || a->T <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
-  return work_bytes(most_new(*a), a->T, a->B, a->Hq, a->Hk, a->D, (int64_t)a->P * a->page_size);
+  return work_bytes(most_new(*a), a->T, a->B, a->Hq, a->Hk, a->D, (int64_t)a->P * a->page_size, form_of(*a));
 }
 extern "C" size_t fs_window_attn_work_bytes(const fs_window_attn_args* a) {
   if (!a || a->B <= 0 || a->Lq <= 0 || a->Hk <= 0 || a->Hq < a->Hk || a->D <= 0) return 0;
-  return work_bytes(a->Lq, (int64_t)a->B * a->Lq, a->B, a->Hq, a->Hk, a->D, a->Lk);
+  return work_bytes(a->Lq, (int64_t)a->B * a->Lq, a->B, a->Hq, a->Hk, a->D, a->Lk, 0);
 }
 
 extern "C" int fs_paged_attn(const fs_paged_attn_args* a, void* stream) {

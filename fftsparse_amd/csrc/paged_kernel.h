@@ -56,13 +56,14 @@ namespace fs {
 
 constexpr int kFewWaves = 4;                        // of a workgroup of few_kernel (1 or 2, as many in all: 10% slower)
 constexpr int kSlotsMany = 512;                     // workgroups that 256 CUs hold
-constexpr int few_slots(int D) { return 256 * 4 / kFewWaves * (128 / D); }
 constexpr int kPartsMany = 1024;                    // split pieces that the workspace holds
 constexpr int kMaxRequests = 4096;
 constexpr int kPlanThreads = 1024;
 
 // Forms of the kernels (F): the cache in e4m3 with a scale per KV head, the new tokens of a request as a tree.
 constexpr int k8 = 1, kTree = 2;
+
+constexpr int few_slots(int D, int F) { return F & k8 ? 512 : 256 * 4 / kFewWaves * (128 / D); }
 
 struct PagedKArgs {
   const uint16_t* q;
@@ -300,8 +301,15 @@ __device__ __forceinline__ void mask_tree(const PagedKArgs& a, const RowTile& u,
                                           bool v0, bool v1) {
   const int base = u.L - u.n;
   const uint32_t* words = a.mask + (int64_t)p * a.mask_words;
+  // What is loaded is waited for right here: with a load that may still be on its way where this joins the loop, the compiler
+  // waits for all loads, the tiles' copies among them, in every step (16 trees of 64 tokens over 8192: 200 us against 180).
+  constexpr int kLoadsHere = 0x0f70;               // vmcnt(0)
   int lo = 0;                                      // keys below it are out of the window
-  if (a.window) lo = min(min(max(a.pos[p], base), u.L - 1) - a.window + 1, base);
+  if (a.window) {
+    const int at = a.pos[p];
+    __builtin_amdgcn_s_waitcnt(kLoadsHere);
+    lo = min(min(max(at, base), u.L - 1) - a.window + 1, base);
+  }
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     __builtin_amdgcn_sched_barrier(0);             // one group's registers at a time
@@ -310,6 +318,7 @@ __device__ __forceinline__ void mask_tree(const PagedKArgs& a, const RowTile& u,
     if (off > -16) {
       const int w = max(off, 0) >> 5;
       const uint32_t w0 = w < a.mask_words ? words[w] : 0u, w1 = w + 1 < a.mask_words ? words[w + 1] : 0u;
+      __builtin_amdgcn_s_waitcnt(kLoadsHere);
       seen = off < 0 ? (w0 << -off) | ((1u << -off) - 1u) : (uint32_t)((((uint64_t)w1 << 32) | w0) >> (off & 31));
       seen &= k + 16 > u.L ? (1u << max(u.L - k, 0)) - 1u : 0xffffu;
     }
@@ -600,13 +609,12 @@ __device__ __forceinline__ float score_scale(const PagedKArgs& a, int hk) {
 constexpr float kSlack = 8.0f;                     // a row's running max is raised past 2^8 only: few rescales of O
 
 template <typename T, int D, bool PAGED, int NW, int F>
-__global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
+__global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs a) {
   using Ops = MfmaOps<T>;
   using V8 = typename Ops::V8;
   using Copy = GroupCopy<D, PAGED, F>;
   constexpr int TILE = 32 * Copy::ROWB;            // bytes of 32 keys
-  constexpr int SUM_BYTES = D / 32 * 4 * 64 * 16;  // of a wave's sums, which take the V tiles' place
-  constexpr int RING = 2 * TILE + (2 * TILE > SUM_BYTES ? 2 * TILE : SUM_BYTES);   // of a wave: two K tiles, two V tiles
+  constexpr int RING = 4 * TILE;                   // of a wave: two K tiles, two V tiles
   constexpr int NI = 2 * Copy::NI;                 // copies of 32 keys
   __shared__ __attribute__((aligned(1024))) char lds[NW * RING];
   __shared__ float2 ml[NW][64];
@@ -767,14 +775,19 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     // ---- the waves' sums joined through LDS (the V tiles' place), wave w taking dims 32 w, 32 (w + NW) ..; the next piece's
     // first copies go out before
     constexpr int NV = D / 32;
-    constexpr int SUMS = 2 * TILE;                 // of a wave's ring: [D / 32][4][64 lanes] 4 floats
-    static_assert(SUMS + NV * 4 * 64 * 16 <= RING, "the sums take the V tiles' place");
+    constexpr int SUMS = 2 * TILE;                 // of a wave's ring: [NVR][4][64 lanes] 4 floats
+    constexpr int NVR = 2 * TILE / (4 * 64 * 16);  // groups of 32 dims at a time: all, or half of them where tiles hold 8 bits
+    static_assert(NVR >= 1 && NV % NVR == 0, "the sums take the place of two V tiles");
+    auto put = [&](int round) {
 #pragma unroll
-    for (int dt = 0; dt < NV; ++dt)
+      for (int dt = 0; dt < NV; ++dt)
+        if (dt / NVR == round)
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4)
-        reinterpret_cast<float4*>(ring + SUMS)[(dt * 4 + g4) * 64 + lane] =
-            make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+          for (int g4 = 0; g4 < 4; ++g4)
+            reinterpret_cast<float4*>(ring + SUMS)[((dt % NVR) * 4 + g4) * 64 + lane] =
+                make_float4(o[dt][4 * g4], o[dt][4 * g4 + 1], o[dt][4 * g4 + 2], o[dt][4 * g4 + 3]);
+    };
+    put(0);
     ml[wave][lane] = make_float2(m_run, l_run);
     const LaneRow me = sg.me;
     const int slot = sg.slot;
@@ -783,38 +796,51 @@ __global__ __launch_bounds__(64 * NW) void few_kernel(PagedKArgs a) {
     const bool more = pos < end;
     if (more) pos += open(pos);
     __syncthreads();
-    if (me.on) {
-      float m = -INFINITY, l = 0.f, f[NW];
+    float m = -INFINITY, l = 0.f, f[NW];
 #pragma unroll
-      for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w][lane].x);
-      const float mu = m == -INFINITY ? 0.f : m;
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w][lane].x);
+    const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(ml[w][lane].x - mu);
+      l += ml[w][lane].y * f[w];
+      if constexpr (F & k8) f[w] *= vs;
+    }
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    auto join = [&](int dt, int g4) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(ml[w][lane].x - mu);
-        l += ml[w][lane].y * f[w];
-        if constexpr (F & k8) f[w] *= vs;
+        const float4 x = reinterpret_cast<const float4*>(lds + w * RING + SUMS)[((dt % NVR) * 4 + g4) * 64 + lane];
+        acc.x += x.x * f[w];
+        acc.y += x.y * f[w];
+        acc.z += x.z * f[w];
+        acc.w += x.w * f[w];
       }
-      const float inv = l != 0.f ? 1.0f / l : 0.f;
+      if (slot < 0) store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      else reinterpret_cast<float4*>(a.part_o)[(((int64_t)slot * NV + dt) * 4 + g4) * 64 + lane] = acc;
+    };
+    if (me.on) {
+      if constexpr (NVR == NV) {
 #pragma unroll
-      for (int dt = wave; dt < NV; dt += NW)
+        for (int dt = wave; dt < NV; dt += NW)
 #pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-          for (int w = 0; w < NW; ++w) {
-            const float4 x = reinterpret_cast<const float4*>(lds + w * RING + SUMS)[(dt * 4 + g4) * 64 + lane];
-            acc.x += x.x * f[w];
-            acc.y += x.y * f[w];
-            acc.z += x.z * f[w];
-            acc.w += x.w * f[w];
-          }
-          if (slot < 0) store_out<T>(op, dt * 32 + g4 * 8 + hi * 4, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-          else reinterpret_cast<float4*>(a.part_o)[(((int64_t)slot * NV + dt) * 4 + g4) * 64 + lane] = acc;
-        }
+          for (int g4 = 0; g4 < 4; ++g4) join(dt, g4);
+      } else {
+        for (int i = wave; i < NVR * 4; i += NW) join(i >> 2, i & 3);
+      }
       if (slot >= 0 && wave == 0 && hi == 0) {
         a.part_ml[(int64_t)slot * 64 + l32] = m;
         a.part_ml[(int64_t)slot * 64 + 32 + l32] = l;
       }
+    }
+#pragma unroll
+    for (int round = 1; round < NV / NVR; ++round) {
+      __syncthreads();
+      put(round);
+      __syncthreads();
+      if (me.on)
+        for (int i = wave; i < NVR * 4; i += NW) join(round * NVR + (i >> 2), i & 3);
     }
     if (!more) return;
     __syncthreads();                               // the sums are read: V tiles may come
@@ -1381,10 +1407,10 @@ struct Work {
 };
 static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 // row tiles of at most `rows` rows of B requests with T tokens in all; few: row tiles of 32, no lists
-static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D) {
+static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D, int F) {
   Work w{};
   w.rows = few ? 32 : 128;
-  w.max_parts = few ? 2 * few_slots(D) : kPartsMany;
+  w.max_parts = few ? 2 * few_slots(D, F) : kPartsMany;
   if (!few) {
     w.max_pairs = T * G / w.rows + B;
     w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
@@ -1408,10 +1434,10 @@ static bool few_rows(int64_t max_new, int G, int64_t row_tiles, int64_t keys) {
 // one: the lists are sized as for one KV head, which has the most row tiles and pieces; few_kernel's size is asked for
 // where that is taken with one KV head too (few_rows then holds for any number: at most 32 rows of all heads, and
 // row tiles counted from above), and it is the same for both head dims.  Either kernel's fits into many_kernel's.
-static size_t work_bytes(int64_t max_new, int64_t T, int B, int Hq, int Hk, int D, int64_t keys) {
+static size_t work_bytes(int64_t max_new, int64_t T, int B, int Hq, int Hk, int D, int64_t keys, int F) {
   if (few_rows(max_new, Hq, T * Hq / 32 + (int64_t)B * Hk, keys))
-    return std::max(work_of(true, T, B, 1, Hq, 64).bytes, work_of(true, T, B, 1, Hq, 128).bytes);
-  return work_of(false, T, B, 1, Hq, D).bytes;
+    return std::max(work_of(true, T, B, 1, Hq, 64, F).bytes, work_of(true, T, B, 1, Hq, 128, F).bytes);
+  return work_of(false, T, B, 1, Hq, D, F).bytes;
 }
 
 template <typename T, int D, bool PAGED, int F>
@@ -1424,7 +1450,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
     k.part_o = reinterpret_cast<float*>(work + w.o);
   }
   if (few) {
-    k.slots = few_slots(D);
+    k.slots = few_slots(D, F);
     few_kernel<T, D, PAGED, kFewWaves, F><<<k.slots, 64 * kFewWaves, 0, s>>>(k);
     if (int rc = fs_host::launch_status(fn)) return rc;
     combine_kernel<T, D, 32, F><<<(k.slots - 1) * (D / 32), kJoinThreads, 0, s>>>(k);
