@@ -174,8 +174,9 @@ class TreeAcceptArgs(ctypes.Structure):
 
 
 class CacheMoveArgs(ctypes.Structure):
-    _fields_ = [("k_caches", POINTER(c_void_p)), ("k_sp", c_int64), ("k_ss", c_int64), ("k_sh", c_int64),
-                ("v_caches", POINTER(c_void_p)), ("v_sp", c_int64), ("v_ss", c_int64), ("v_sh", c_int64),
+    _fields_ = [("k_caches", POINTER(c_void_p)), ("v_caches", POINTER(c_void_p)),
+                ("k_cache", c_void_p), ("k_sl", c_int64), ("k_sp", c_int64), ("k_ss", c_int64), ("k_sh", c_int64),
+                ("v_cache", c_void_p), ("v_sl", c_int64), ("v_sp", c_int64), ("v_ss", c_int64), ("v_sh", c_int64),
                 ("block_table", c_void_p), ("t_sb", c_int64), ("cu_lens", c_void_p), ("seq_lens", c_void_p),
                 ("kept", c_void_p), ("layers", c_int), ("B", c_int), ("T", c_int), ("Hk", c_int), ("D", c_int),
                 ("P", c_int), ("page_size", c_int), ("elem_bytes", c_int), ("num_pages", c_int64)]

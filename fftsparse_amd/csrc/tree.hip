@@ -100,19 +100,20 @@ __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accep
 constexpr int kMoveLayers = 64;                    // of a launch
 struct MoveKArgs {
   fs_cache_move_args a;
-  char* caches[2][kMoveLayers];                    // [K, V]
+  int caches;                                      // that a workgroup takes
+  char* cache[2 * kMoveLayers];                    // K and V of each layer
 };
 
-// A workgroup moves one request's rows in one cache.  Rows are read some at a time, all of them before any is
-// written: the place of row i may be that of a row j > i that another thread still has to read.  (Rows of later
-// steps lie behind every place written so far: j >= i.)
+// A workgroup moves one request's rows in some of the caches, whose places it looks up once.  The pieces (cache, row, 16
+// bytes) are taken in this order, 1024 at a time, and all of them are read before any is written: the place
+// of row i may be that of a row j > i that another thread still has to read.  Pieces of later steps lie behind
+// every place of their cache that is written by then: row j > i comes from behind j.
 __global__ __launch_bounds__(kTreeThreads) void cache_move_kernel(MoveKArgs ka) {
-  constexpr int HELD = 4;                          // pieces of 16 bytes of a thread
+  constexpr int HELD = 4;                          // pieces of a thread
   const fs_cache_move_args& a = ka.a;
-  __shared__ int64_t from[kTreeMost], to[kTreeMost];   // offsets in elements, -1: stays
+  __shared__ int2 from[kTreeMost], to[kTreeMost];  // page and slot; page -1: stays
   __shared__ int lo, hi;
-  const int tid = threadIdx.x, b = blockIdx.x, v = blockIdx.y & 1, layer = blockIdx.y >> 1;
-  const int64_t sp = v ? a.v_sp : a.k_sp, ss = v ? a.v_ss : a.k_ss, sh = v ? a.v_sh : a.k_sh;
+  const int tid = threadIdx.x, b = blockIdx.x;
   const TreeRows r(a.cu_lens, b, a.T);
   const int n = min(r.n, kTreeMost);
   const int64_t first = (int64_t)a.seq_lens[b] - r.n;
@@ -121,54 +122,56 @@ __global__ __launch_bounds__(kTreeThreads) void cache_move_kernel(MoveKArgs ka) 
     hi = -1;
   }
   __syncthreads();
-  auto place = [&](int i) -> int64_t {
+  auto place = [&](int i) {
     const int64_t s = first + i;
-    if (s < 0 || s >= (int64_t)a.P * a.page_size) return -1;
+    if (s < 0 || s >= (int64_t)a.P * a.page_size) return make_int2(-1, 0);
     const int pg = (int)s / a.page_size, e = a.block_table[b * a.t_sb + pg];
-    return e >= 0 && e < a.num_pages ? e * sp + ((int)s - pg * a.page_size) * ss : -1;
+    return make_int2(e >= 0 && e < a.num_pages ? e : -1, (int)s - pg * a.page_size);
   };
   for (int i = tid; i < n; i += kTreeThreads) {
     const int j = a.kept[r.c0 + i];
-    int64_t f = -1, t = -1;
+    int2 f = make_int2(-1, 0), t = f;
     if (j > i && j < n) {
       f = place(j);
       t = place(i);
-      if (f < 0 || t < 0) f = t = -1;
+      if (f.x < 0 || t.x < 0) f.x = -1;
     }
     from[i] = f;
     to[i] = t;
-    if (f >= 0) {
+    if (f.x >= 0) {
       atomicMin(&lo, i);
       atomicMax(&hi, i);
     }
   }
   __syncthreads();
-  char* const base = ka.caches[v][layer];
-  const int per_head = a.D * a.elem_bytes / 16, pieces = a.Hk * per_head;   // 16-byte pieces
-  const int rows = max(HELD * kTreeThreads / pieces, 1);                    // read at a time
-  for (int i0 = lo; i0 <= hi; i0 += rows) {
-    const int items = min(rows, hi + 1 - i0) * pieces;
-    // more pieces than are held (wide rows): columns one part after the other, each in the rows' order
-    for (int c0 = 0; c0 < items; c0 += HELD * kTreeThreads) {
-      uint4 held[HELD];
-      char* dst[HELD];
+  const int rows = hi + 1 - lo;
+  if (rows <= 0) return;
+  const uint32_t per_head = a.D * a.elem_bytes / 16, pieces = a.Hk * per_head, per_cache = rows * pieces;
+  const int c0 = blockIdx.y * ka.caches, caches = min(ka.caches, 2 * a.layers - c0);
+  // below 2^32: 8 caches of 1024 rows of 2^18 pieces
+  for (uint32_t x0 = 0; x0 < caches * per_cache; x0 += HELD * kTreeThreads) {
+    uint4 held[HELD];
+    char* dst[HELD];
 #pragma unroll
-      for (int k = 0; k < HELD; ++k) {
-        const int x = c0 + k * kTreeThreads + tid;
-        dst[k] = nullptr;
-        if (x < items) {
-          const int i = x / pieces, c = x - i * pieces, h = c / per_head, d = c - h * per_head;
-          if (from[i0 + i] >= 0) {
-            held[k] = *reinterpret_cast<const uint4*>(base + (from[i0 + i] + h * sh) * a.elem_bytes + d * 16);
-            dst[k] = base + (to[i0 + i] + h * sh) * a.elem_bytes + d * 16;
-          }
+    for (int k = 0; k < HELD; ++k) {
+      const uint32_t x = x0 + k * kTreeThreads + tid;
+      dst[k] = nullptr;
+      if (x < caches * per_cache) {
+        const uint32_t c = x / per_cache, y = x - c * per_cache, i = y / pieces, z = y - i * pieces, h = z / per_head;
+        const int2 f = from[lo + i], t = to[lo + i];
+        if (f.x >= 0) {
+          const bool v = (c0 + c) & 1;
+          const int64_t sp = v ? a.v_sp : a.k_sp, ss = v ? a.v_ss : a.k_ss;
+          char* at = ka.cache[c0 + c] + h * (v ? a.v_sh : a.k_sh) * a.elem_bytes + (z - h * per_head) * 16;
+          held[k] = *reinterpret_cast<const uint4*>(at + (f.x * sp + f.y * ss) * a.elem_bytes);
+          dst[k] = at + (t.x * sp + t.y * ss) * a.elem_bytes;
         }
       }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < HELD; ++k)
-        if (dst[k] != nullptr) *reinterpret_cast<uint4*>(dst[k]) = held[k];
     }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < HELD; ++k)
+      if (dst[k] != nullptr) *reinterpret_cast<uint4*>(dst[k]) = held[k];
   }
 }
 
@@ -221,21 +224,27 @@ extern "C" int fs_cache_move(const fs_cache_move_args* a, void* stream) {
   FS_CHECK_SUPPORTED((int64_t)a->P * a->page_size <= INT_MAX, "%s: %d pages of %d tokens per request unsupported", fn,
                      a->P, a->page_size);
   if (a->T == 0 || a->layers == 0) return FS_OK;
-  const int64_t st[] = {a->k_sp, a->k_ss, a->k_sh, a->v_sp, a->v_ss, a->v_sh};
+  const bool arrays = a->k_caches != nullptr;
+  const int64_t st[] = {a->k_sp, a->k_ss, a->k_sh, a->v_sp, a->v_ss, a->v_sh, arrays ? 0 : a->k_sl, arrays ? 0 : a->v_sl};
   for (int64_t x : st) FS_CHECK_ARG(x * a->elem_bytes % 16 == 0, "%s: strides must be multiples of 16 bytes", fn);
-  FS_CHECK_ARG(a->k_caches && a->v_caches && a->block_table && a->cu_lens && a->seq_lens && a->kept && a->t_sb >= a->P,
+  FS_CHECK_ARG(arrays == (a->v_caches != nullptr) && a->block_table && a->cu_lens && a->seq_lens && a->kept && a->t_sb >= a->P,
                "%s: null tensor pointer, or row stride %lld of %d", fn, (long long)a->t_sb, a->P);
+  auto cache = [&](bool v, int i) {
+    return arrays ? static_cast<char*>((v ? a->v_caches : a->k_caches)[i])
+                  : static_cast<char*>(v ? a->v_cache : a->k_cache) + i * (v ? a->v_sl : a->k_sl) * a->elem_bytes;
+  };
+  FS_CHECK_ARG(arrays || (a->k_cache && a->v_cache), "%s: caches must be given, 16-byte aligned", fn);
   for (int i = 0; i < a->layers; ++i)
-    FS_CHECK_ARG(a->k_caches[i] && a->v_caches[i] && ((uintptr_t)a->k_caches[i] | (uintptr_t)a->v_caches[i]) % 16 == 0,
+    FS_CHECK_ARG(cache(false, i) && cache(true, i) && ((uintptr_t)cache(false, i) | (uintptr_t)cache(true, i)) % 16 == 0,
                  "%s: caches must be given, 16-byte aligned", fn);
   for (int l0 = 0; l0 < a->layers; l0 += kMoveLayers) {
-    MoveKArgs k{*a, {}};
+    MoveKArgs k{*a, 1, {}};
     const int n = std::min(a->layers - l0, kMoveLayers);
-    for (int i = 0; i < n; ++i) {
-      k.caches[0][i] = static_cast<char*>(a->k_caches[l0 + i]);
-      k.caches[1][i] = static_cast<char*>(a->v_caches[l0 + i]);
-    }
-    cache_move_kernel<<<dim3(a->B, 2 * n), kTreeThreads, 0, (hipStream_t)stream>>>(k);
+    for (int i = 0; i < 2 * n; ++i) k.cache[i] = cache(i & 1, l0 + i / 2);
+    k.a.layers = n;
+    // few requests: a cache each; else as many as leave two workgroups per CU (64 requests, 32 layers: 9.6 us either way)
+    k.caches = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)a->B * 2 * n / 512));
+    cache_move_kernel<<<dim3(a->B, (2 * n + k.caches - 1) / k.caches), kTreeThreads, 0, (hipStream_t)stream>>>(k);
     if (int rc = fs_host::launch_status(fn)) return rc;
   }
   return FS_OK;

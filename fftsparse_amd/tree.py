@@ -75,7 +75,7 @@ def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tens
     words = -(-_most(max_new) // 64)
     dev = _lib.same_device(parents, cu_lens, seq_lens)
     if out is None:
-        out = TreePlan(parents.new_empty(T), torch.empty((T, words), dtype=torch.int64, device=dev))
+        out = TreePlan(parents.new_empty(T), parents.new_empty((T, words), dtype=torch.int64))
     else:
         _lib.same_device(parents, _ints(out.positions, "out.positions", (T,)),
                          _ints(out.mask, "out.mask", (T, words), (torch.int64,)))
@@ -149,29 +149,32 @@ _CACHE_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3
 
 
 def _layers(caches, name: str, shape, dtype):
-    """The caches' addresses, their strides and the tensors: one [pages, page_size, Hk, D] cache, several in a tensor
-    [layers, ...], or a sequence of the first."""
+    """The caches of one layer [pages, page_size, Hk, D], of several in a tensor [layers, ...], or in a sequence of the
+    first: their number, addresses (None: apart by a stride), address of the first, strides (layer, page, slot, head) in
+    elements, and the tensors."""
     if isinstance(caches, torch.Tensor):
-        if caches.dim() == 5:
-            if not caches.shape[0]:
-                raise ValueError(f"{name} holds no layer")
-            st = _written(caches[0], name, shape, dtype)
-            step, first = caches.stride(0) * caches.element_size(), caches.data_ptr()
-            if caches.shape[0] > 1 and (step == 0 or step % 16):
-                raise ValueError(f"{name}: the layers must be apart by multiples of 16 bytes, got stride {caches.stride(0)}")
-            return [first + i * step for i in range(caches.shape[0])], st, (caches,)
-        caches = (caches,)
+        if caches.dim() == len(shape):
+            return 1, None, caches.data_ptr(), (0, *_written(caches, name, shape, dtype)), (caches,)
+        n, st, whole = caches.shape[0], caches.stride(), caches.shape[1:]
+        if whole != shape or caches.dtype != dtype:
+            raise ValueError(f"{name} must be a [layers, {', '.join(map(str, shape))}] {dtype} tensor, got {caches.dtype} "
+                             f"{tuple(caches.shape)}")
+        per = 16 // caches.element_size()
+        if st[4] != 1 and shape[3] > 1 or caches.data_ptr() & 15 or any(
+                m > 1 and (s % per or s == 0) for s, m in zip(st[:4], caches.shape)):
+            raise ValueError(f"{name} must have d contiguous, the other strides multiples of 16 bytes, 16-byte alignment and no "
+                             f"broadcast dimension, got strides {st}")
+        return n, None, caches.data_ptr(), [s if m > 1 else 0 for s, m in zip(st[:4], caches.shape)], (caches,)
     if not len(caches):
         raise ValueError(f"{name} holds no layer")
     st = _written(caches[0], name, shape, dtype)
-    like = caches[0].stride()
-    ptrs = []
+    like, ptrs = caches[0].stride(), []
     for t in caches:
         p = t.data_ptr()
         if t.dtype != dtype or t.shape != shape or t.stride() != like or p & 15:
             raise ValueError(f"{name}: the layers' caches must be of one shape, type and layout, 16-byte aligned")
         ptrs.append(p)
-    return ptrs, st, caches
+    return len(ptrs), ptrs, 0, (0, *st), caches
 
 
 def move_kept(k_cache: torch.Tensor | Sequence[torch.Tensor], v_cache: torch.Tensor | Sequence[torch.Tensor],
@@ -187,16 +190,16 @@ def move_kept(k_cache: torch.Tensor | Sequence[torch.Tensor], v_cache: torch.Ten
     launch.  Tokens without a page stay as they are; of a request the first 1024 are
     looked at."""
     one = k_cache if isinstance(k_cache, torch.Tensor) else k_cache[0] if len(k_cache) else None
-    if one is None or one.dim() < 4 or not one.numel():
+    if one is None or one.dim() not in (4, 5) or (one.dim() == 5 and one is not k_cache) or not one.numel():
         raise ValueError("k_cache must be [pages, page_size, Hk, D] or [layers, pages, page_size, Hk, D], or a sequence of the first")
     shape, dtype = one.shape[-4:], one.dtype
     if dtype not in _CACHE_DTYPES:
         raise TypeError(f"unsupported cache type {dtype}")
     pages, ps, Hk, D = shape
-    kp, ks, kt = _layers(k_cache, "k_cache", shape, dtype)
-    vp, vs, vt = _layers(v_cache, "v_cache", shape, dtype)
-    if len(kp) != len(vp):
-        raise ValueError(f"{len(kp)} layers of keys and {len(vp)} of values")
+    n, kp, k0, ks, kt = _layers(k_cache, "k_cache", shape, dtype)
+    m, vp, v0, vs, vt = _layers(v_cache, "v_cache", shape, dtype)
+    if n != m or (kp is None) != (vp is None):
+        raise ValueError(f"{n} layers of keys and {m} of values, or not in one form")
     B, P, t_sb = _table(block_table)
     _ints(cu_lens, "cu_lens", (B + 1,))
     _ints(seq_lens, "seq_lens", (B,))
@@ -205,10 +208,12 @@ def move_kept(k_cache: torch.Tensor | Sequence[torch.Tensor], v_cache: torch.Ten
     dev = _lib.same_device(block_table, cu_lens, seq_lens, kept, *kt, *vt)
     if not T:
         return
-    n = len(kp)
-    array = _lib.c_void_p * n
-    _lib.call("fs_cache_move", CacheMoveArgs(
-        k_caches=array(*kp), k_sp=ks[0], k_ss=ks[1], k_sh=ks[2], v_caches=array(*vp), v_sp=vs[0], v_ss=vs[1], v_sh=vs[2],
+    args = CacheMoveArgs(
+        k_cache=k0, k_sl=ks[0], k_sp=ks[1], k_ss=ks[2], k_sh=ks[3], v_cache=v0, v_sl=vs[0], v_sp=vs[1], v_ss=vs[2], v_sh=vs[3],
         block_table=block_table.data_ptr(), t_sb=t_sb, cu_lens=cu_lens.data_ptr(), seq_lens=seq_lens.data_ptr(),
         kept=kept.data_ptr(), layers=n, B=B, T=T, Hk=Hk, D=D, P=P, page_size=ps, elem_bytes=one.element_size(),
-        num_pages=pages), dev)
+        num_pages=pages)
+    if kp is not None:
+        array = _lib.c_void_p * n
+        args.k_caches, args.v_caches = array(*kp), array(*vp)
+    _lib.call("fs_cache_move", args, dev)

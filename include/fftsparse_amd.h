@@ -590,13 +590,16 @@ FS_API int fs_tree_accept(const fs_tree_accept_args* a, void* stream);
 /* The kept tokens' keys and values to where they belong: for every request and i with
  * j = kept[cu_lens[b] + i] > i (j below n; the j rise with i), the rows of its new token
  * j in the cache go to the place of its new token i, in each of `layers` pairs of caches
- * of the same shape and strides (k_caches, v_caches: host arrays of device pointers).
+ * of the same shape and strides: k_caches and v_caches, host arrays of device pointers, or,
+ * where these are NULL, k_cache + i * k_sl and v_cache + i * v_sl (elements) for layer i.
  * elem_bytes 1, 2 or 4; rows of D * elem_bytes, a multiple of 16 bytes, strides too.
  * Tokens whose page is none stay.  Of a request only the first 1024 tokens are looked
  * at. */
 typedef struct {
-  void* const* k_caches; int64_t k_sp, k_ss, k_sh;
-  void* const* v_caches; int64_t v_sp, v_ss, v_sh;
+  void* const* k_caches;                      /* [layers], or NULL */
+  void* const* v_caches;
+  void* k_cache; int64_t k_sl, k_sp, k_ss, k_sh;
+  void* v_cache; int64_t v_sl, v_sp, v_ss, v_sh;
   const int32_t* block_table; int64_t t_sb;   /* [B][P] */
   const int32_t* cu_lens;                     /* [B + 1] */
   const int32_t* seq_lens;                    /* [B], new tokens included */

@@ -115,6 +115,11 @@ def test_move_kept_refuses():
             (ValueError, "on the GPU", torch.stack([c, c]), torch.stack([c, c]), {}),
             (ValueError, "k_cache must be", c[0], c, {}), (ValueError, "k_cache must be", [], [], {}),
             (ValueError, "no layer", [c], [], {}), (ValueError, "layers of keys", [c, c], [c], {}),
+            (ValueError, "layers of keys", [c], c, {}), (ValueError, "layers of keys", torch.stack([c, c]), c, {}),
+            (ValueError, "v_cache", torch.stack([c, c]), torch.stack([c, c]).half(), {}),
+            (ValueError, "v_cache", c, torch.stack([c, c])[..., :64], {}),
+            (ValueError, "broadcast", torch.stack([c, c]), c[None].expand(2, *c.shape), {}),
+            (ValueError, "k_cache must be", [torch.stack([c, c])], [torch.stack([c, c])], {}),
             (ValueError, "one shape", [c, other], [c, c], {}), (ValueError, "one shape", [c, c.half()], [c, c], {}),
             (ValueError, "v_cache", c, c[..., :64], {}), (ValueError, "v_cache", c, c.half(), {}),
             (TypeError, "unsupported", c.double(), c.double(), {}),
@@ -177,7 +182,10 @@ def test_c_abi_refuses_without_a_launch():
         return _lib.CacheMoveArgs(k_caches=ptrs, v_caches=ptrs, block_table=16, t_sb=4, cu_lens=16, seq_lens=16, kept=16,
                                   layers=2, B=2, T=3, Hk=2, D=128, P=4, page_size=16, elem_bytes=2, num_pages=8)
     for rc, text, change in [(-1, "of 3 bytes", dict(elem_bytes=3)), (-2, "heads of 4", dict(D=4)), (-1, "layers=-1", dict(layers=-1)),
-                             (-1, "16-byte", dict(k_caches=odd)), (-1, "multiples of 16 bytes", dict(v_ss=4)),
+                             (-1, "16-byte", dict(k_caches=odd)), (-1, "null tensor", dict(v_caches=None)),
+                             (-1, "caches must be given", dict(k_caches=None, v_caches=None)),
+                             (-1, "16-byte", dict(k_caches=None, v_caches=None, k_cache=8, v_cache=16)),
+                             (-1, "multiples of 16 bytes", dict(k_caches=None, v_caches=None, k_cache=16, v_cache=16, v_sl=4)), (-1, "multiples of 16 bytes", dict(v_ss=4)),
                              (-1, "row stride 3", dict(t_sb=3)), (-1, "null tensor", dict(kept=None)),
                              (-2, "per request", dict(P=1 << 28, t_sb=1 << 28))]:
         got, said = _rc("fs_cache_move", move(), **change)
