@@ -63,7 +63,12 @@ constexpr int kPlanThreads = 1024;
 // Forms of the kernels (F): the cache in e4m3 with a scale per KV head, the new tokens of a request as a tree.
 constexpr int k8 = 1, kTree = 2;
 
+// Workgroups of few_kernel: as many as its LDS and registers let the GPU hold (8-bit tiles are half as large: two to a CU).
 constexpr int few_slots(int D, int F) { return F & k8 ? 512 : 256 * 4 / kFewWaves * (128 / D); }
+// KV heads that a workgroup's waves share out (where Hk is a multiple of it): at 8 bits and head dim 64 a cache line
+// holds two heads' rows of a token, and one head alone uses half of it (64 requests of up to 4096, 28 / 4 heads: 36 us, 44 with one
+// head; at head dim 128 two heads gain 3% on long contexts and lose 10 to 20% on short ones: 48 requests of 600 26.5, 23.8).
+constexpr int few_heads(int D, int F) { return F & k8 && D == 64 ? 2 : 1; }
 
 struct PagedKArgs {
   const uint16_t* q;
@@ -494,7 +499,7 @@ __device__ __forceinline__ int small_quotient(int n, int d) {
 // lane l adds the tiles of a group of requests, in a second one the lanes take one request each of the group that is
 // looked for (one request per lane up to 64: the second step is the first).  It is kept short: a wave takes 4 cycles per
 // instruction and its first copies wait for it.
-template <int M, int TK, int F>
+template <int M, int TK, int HP, int F>
 struct Ranges {
   struct Request {
     Lengths x;
@@ -533,7 +538,7 @@ struct Ranges {
     const int upto = wave_prefix(tiles);
     before = upto - tiles;
     W1 = __builtin_amdgcn_readlane(upto, 63);
-    W = W1 * a.Hk;
+    W = W1 * (a.Hk / HP);
     const int sh = 31 - __builtin_clz(groups);
     per = max((W + groups - 1) >> sh, 1);          // at least 2 or 4: one request of 1000 tokens 13.8, 17.2 us, not 12.2
   }
@@ -608,8 +613,9 @@ __device__ __forceinline__ float score_scale(const PagedKArgs& a, int hk) {
 }
 constexpr float kSlack = 8.0f;                     // a row's running max is raised past 2^8 only: few rescales of O
 
-template <typename T, int D, bool PAGED, int NW, int F>
-__global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs a) {
+template <typename T, int D, bool PAGED, int KW, int HP, int F>
+__global__ __launch_bounds__(64 * KW * HP, F & k8 ? 2 : 1) void few_kernel(PagedKArgs a) {
+  constexpr int NW = KW * HP;
   using Ops = MfmaOps<T>;
   using V8 = typename Ops::V8;
   using Copy = GroupCopy<D, PAGED, F>;
@@ -622,7 +628,8 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   char* ring = lds + wave * RING;
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
-  const Ranges<32, 32 * NW, F> ranges(a, gridDim.x);
+  const int kw = HP == 1 ? wave : wave % KW, hp = HP == 1 ? 0 : wave / KW;   // this wave's share of a tile's keys, and its head
+  const Ranges<32, 32 * KW, HP, F> ranges(a, gridDim.x);
   const int first = blockIdx.x * ranges.per, end = min(first + ranges.per, ranges.W);
   if (first >= end) return;
 
@@ -639,7 +646,7 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
     int e[2], slot[2];
   } x0, x1, x2;
   // this wave's two groups of keys of each of the piece's tiles: the first one's place among those visited
-  auto group_of = [&](int i) { return (sg.begin + i) * (2 * NW) + 2 * wave; };
+  auto group_of = [&](int i) { return (sg.begin + i) * (2 * KW) + 2 * kw; };
   auto load_ent = [&](int i) {
     Ent x{{-1, -1}, {0, 0}};
 #pragma unroll
@@ -669,11 +676,11 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
   auto open = [&](int pos) {
     const auto at = ranges.find(pos);
     const int count = min(at.start + at.nt, end) - pos;
-    sg.hk = at.hk;
+    sg.hk = at.hk * HP + hp;
     sg.b = at.b;
     sg.begin = pos - at.start;
-    sg.slot = count == at.nt ? -1 : 2 * blockIdx.x + (pos != first);   // a range's first piece or, not starting with it, its last
-    sg.u = row_tile<32, 32 * NW, F>(a, at.x, at.rt);
+    sg.slot = count == at.nt ? -1 : (2 * blockIdx.x + (pos != first)) * HP + hp;   // a range's first piece or, not starting with it, its last
+    sg.u = row_tile<32, 32 * KW, F>(a, at.x, at.rt);
     sg.me = lane_row<F>(a, sg.u, l32);
     sg.cnt = min(count, sg.u.nt - sg.begin);
     if (sg.cnt > 0 && sg.u.key_of(group_of(sg.cnt - 1)) >= sg.u.kend) --sg.cnt;   // the last tile ends before this wave's keys
@@ -772,7 +779,7 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
       x1 = x2;
       x2 = x3;
     }
-    // ---- the waves' sums joined through LDS (the V tiles' place), wave w taking dims 32 w, 32 (w + NW) ..; the next piece's
+    // ---- the sums of a head's waves joined through LDS (the V tiles' place), wave w taking dims 32 w, 32 (w + NW) ..; the next piece's
     // first copies go out before
     constexpr int NV = D / 32;
     constexpr int SUMS = 2 * TILE;                 // of a wave's ring: [NVR][4][64 lanes] 4 floats
@@ -796,22 +803,23 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
     const bool more = pos < end;
     if (more) pos += open(pos);
     __syncthreads();
-    float m = -INFINITY, l = 0.f, f[NW];
+    float m = -INFINITY, l = 0.f, f[KW];
+    const int w0 = hp * KW;                        // the head's first wave
 #pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w][lane].x);
+    for (int w = 0; w < KW; ++w) m = fmaxf(m, ml[w0 + w][lane].x);
     const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      f[w] = __builtin_amdgcn_exp2f(ml[w][lane].x - mu);
-      l += ml[w][lane].y * f[w];
+    for (int w = 0; w < KW; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(ml[w0 + w][lane].x - mu);
+      l += ml[w0 + w][lane].y * f[w];
       if constexpr (F & k8) f[w] *= vs;
     }
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     auto join = [&](int dt, int g4) {
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float4 x = reinterpret_cast<const float4*>(lds + w * RING + SUMS)[((dt % NVR) * 4 + g4) * 64 + lane];
+      for (int w = 0; w < KW; ++w) {
+        const float4 x = reinterpret_cast<const float4*>(lds + (w0 + w) * RING + SUMS)[((dt % NVR) * 4 + g4) * 64 + lane];
         acc.x += x.x * f[w];
         acc.y += x.y * f[w];
         acc.z += x.z * f[w];
@@ -823,13 +831,13 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
     if (me.on) {
       if constexpr (NVR == NV) {
 #pragma unroll
-        for (int dt = wave; dt < NV; dt += NW)
+        for (int dt = kw; dt < NV; dt += KW)
 #pragma unroll
           for (int g4 = 0; g4 < 4; ++g4) join(dt, g4);
       } else {
-        for (int i = wave; i < NVR * 4; i += NW) join(i >> 2, i & 3);
+        for (int i = kw; i < NVR * 4; i += KW) join(i >> 2, i & 3);
       }
-      if (slot >= 0 && wave == 0 && hi == 0) {
+      if (slot >= 0 && kw == 0 && hi == 0) {
         a.part_ml[(int64_t)slot * 64 + l32] = m;
         a.part_ml[(int64_t)slot * 64 + 32 + l32] = l;
       }
@@ -840,7 +848,7 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
       put(round);
       __syncthreads();
       if (me.on)
-        for (int i = wave; i < NVR * 4; i += NW) join(round * NVR + (i >> 2), i & 3);
+        for (int i = kw; i < NVR * 4; i += KW) join(round * NVR + (i >> 2), i & 3);
     }
     if (!more) return;
     __syncthreads();                               // the sums are read: V tiles may come
@@ -851,28 +859,29 @@ __global__ __launch_bounds__(64 * NW, F & k8 ? 2 : 1) void few_kernel(PagedKArgs
 // piece (J as many threads as there are for an item), then the J sums are added in LDS; always in the same
 // order.  Wave 0 looks up what the workgroup joins (mostly nothing).
 constexpr int kJoinThreads = 256;
-template <typename T, int D, int M, int F>
+template <typename T, int D, int M, int HP, int F>
 __global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
   constexpr int QW = M / 32, NV = D / 32, NT = kJoinThreads, AHEAD = M == 32 ? 8 : 16;
   constexpr bool FEW = M == 32;
   __shared__ float4 part[NT];
   __shared__ float2 ml[NT];
   __shared__ int job[10];                          // pieces, first slot, second slot, KV head, request, row tile, lengths
-  const int tid = threadIdx.x, dt = blockIdx.x % NV, qq = blockIdx.x / NV % QW, w = blockIdx.x / (NV * QW);
+  const int tid = threadIdx.x, dt = blockIdx.x % NV, qq = blockIdx.x / NV % QW;
+  const int hp = blockIdx.x / (NV * QW) % HP, w = blockIdx.x / (NV * QW * HP);
   if (tid < 64) {
     int np = 0;
     if constexpr (FEW) {
       // the row tile that the end of range w cuts, if it is the first that does
-      const Ranges<M, 32 * kFewWaves, F> ranges(a, a.slots);
+      const Ranges<M, 32 * kFewWaves / HP, HP, F> ranges(a, a.slots);
       const int cut = (w + 1) * ranges.per;
       if (cut < ranges.W) {
         const auto at = ranges.find(cut);
         if (at.start < cut && at.start >= w * ranges.per) {
           np = small_quotient(at.start + at.nt - 1, ranges.per) - w + 1;
           if (tid == 0) {
-            job[1] = 2 * w + (at.start != w * ranges.per);
-            job[2] = 2 * (w + 1);                  // the others are their ranges' first pieces
-            job[3] = at.hk;
+            job[1] = (2 * w + (at.start != w * ranges.per)) * HP + hp;
+            job[2] = 2 * (w + 1) * HP + hp;        // the others are their ranges' first pieces
+            job[3] = at.hk * HP + hp;
             job[4] = at.b;
             job[5] = at.rt;
             job[6] = at.x.row0;
@@ -913,7 +922,7 @@ __global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
   const int rows = min(u.nrows - qq * 32, 32);
   if (rows <= 0) return;
   const int items = rows * 8, J = NT / items;      // an item: row, and 4 dims: 32 dt + 4 c ..
-  auto slot_of = [&](int j) { return (int64_t)(j == 0 ? s0 : s1 + (j - 1) * (FEW ? 2 : QW)); };
+  auto slot_of = [&](int j) { return (int64_t)(j == 0 ? s0 : s1 + (j - 1) * (FEW ? 2 * HP : QW)); };
   const int jg = tid / items, it = tid - jg * items;
   const int c = it / rows, r = it - c * rows;
   float m = -INFINITY, l = 0.f;
@@ -1410,7 +1419,7 @@ static size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 static Work work_of(bool few, int64_t T, int B, int Hk, int G, int D, int F) {
   Work w{};
   w.rows = few ? 32 : 128;
-  w.max_parts = few ? 2 * few_slots(D, F) : kPartsMany;
+  w.max_parts = few ? 2 * few_slots(D, F) * few_heads(D, F) : kPartsMany;
   if (!few) {
     w.max_pairs = T * G / w.rows + B;
     w.max_pieces = w.max_pairs + (w.max_parts + Hk - 1) / Hk;
@@ -1440,6 +1449,16 @@ static size_t work_bytes(int64_t max_new, int64_t T, int B, int Hq, int Hk, int 
   return work_of(false, T, B, 1, Hq, D, F).bytes;
 }
 
+template <typename T, int D, bool PAGED, int HP, int F>
+static int launch_few(PagedKArgs k, hipStream_t s, const char* fn) {
+  constexpr int NW = kFewWaves;
+  k.slots = few_slots(D, F);
+  few_kernel<T, D, PAGED, NW / HP, HP, F><<<k.slots, 64 * NW, 0, s>>>(k);
+  if (int rc = fs_host::launch_status(fn)) return rc;
+  combine_kernel<T, D, 32, HP, F><<<(k.slots - 1) * HP * (D / 32), kJoinThreads, 0, s>>>(k);
+  return fs_host::launch_status(fn);
+}
+
 template <typename T, int D, bool PAGED, int F>
 static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, int B, int Lq, hipStream_t s, const char* fn) {
   const int64_t rows = (int64_t)Lq * k.G;
@@ -1450,11 +1469,10 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
     k.part_o = reinterpret_cast<float*>(work + w.o);
   }
   if (few) {
-    k.slots = few_slots(D, F);
-    few_kernel<T, D, PAGED, kFewWaves, F><<<k.slots, 64 * kFewWaves, 0, s>>>(k);
-    if (int rc = fs_host::launch_status(fn)) return rc;
-    combine_kernel<T, D, 32, F><<<(k.slots - 1) * (D / 32), kJoinThreads, 0, s>>>(k);
-    return fs_host::launch_status(fn);
+    constexpr int HP = few_heads(D, F);
+    if constexpr (HP > 1)
+      if (k.Hk % HP == 0) return launch_few<T, D, PAGED, HP, F>(k, s, fn);
+    return launch_few<T, D, PAGED, 1, F>(k, s, fn);
   }
   if (plan) {
     int4* pieces = reinterpret_cast<int4*>(work + w.pieces);
@@ -1470,7 +1488,7 @@ static int launch(PagedKArgs k, bool few, bool plan, const Work& w, char* work, 
   many_kernel<T, D, PAGED, F><<<(unsigned)((grid + 7) / 8 * 8), 256, 0, s>>>(k);
   if (int rc = fs_host::launch_status(fn)) return rc;
   if (plan) {
-    combine_kernel<T, D, 128, F><<<(unsigned)(w.max_splits * k.Hk * 4 * (D / 32)), kJoinThreads, 0, s>>>(k);
+    combine_kernel<T, D, 128, 1, F><<<(unsigned)(w.max_splits * k.Hk * 4 * (D / 32)), kJoinThreads, 0, s>>>(k);
     return fs_host::launch_status(fn);
   }
   return FS_OK;

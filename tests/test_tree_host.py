@@ -199,7 +199,7 @@ def test_the_forms_spill_no_vector_registers(tmp_path, name):
     spills = {}
     for meta in asm.split("  - .agpr_count:")[1:]:
         spills[re.search(r"\.name: +(\S+)", meta)[1]] = int(re.search(r"\.vgpr_spill_count: +(\d+)", meta)[1])
-    assert sum("many_kernel" in n for n in spills) == 4 and sum("few_kernel" in n for n in spills) == 4
+    assert sum("many_kernel" in n for n in spills) == 4 and sum("few_kernel" in n for n in spills) == (6 if "8" in name else 4)
     assert {n: s for n, s in spills.items() if s} == {}
 
 
