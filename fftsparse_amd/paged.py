@@ -138,6 +138,13 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
     return p, p + t.numel() * t.element_size()
 
 
+def _apart(outs, ins, what: str) -> None:
+    """Refuses outputs that share storage with what is read while they are written."""
+    read = [_span(x) for x in ins]
+    if any(lo < end and start < hi for lo, hi in map(_span, outs) for start, end in read):
+        raise ValueError(f"out shares storage with an input: {what}")
+
+
 @dataclass
 class StepPlan:
     """What ``plan_step`` forms on the GPU for one step."""
@@ -286,7 +293,7 @@ def _attend(name, q, k_cache, v_cache, block_table, cu_lens, seq_lens, mask, pos
             if positions is None:
                 raise ValueError("a window over a tree needs the tokens' positions")
             more += (_ints(positions, "positions", (T,)),)
-    _inference_only(name, q, k_cache, v_cache)
+    _inference_only(name, q, k_cache, v_cache, *more)
     if out is None:
         dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, *more)
         out = q.new_empty((T, Hq, D))

@@ -141,7 +141,7 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     _ints(slots, "slots", (q.shape[0],), (torch.int64,))
     shape, kc, vc = _caches(k_cache, v_cache, E4M3 if k_cache.dtype == E4M3 else q.dtype, k.shape[1], k.shape[2])
     scaled = _scales(k_scale, v_scale, k_cache.dtype, k.shape[1])
-    _inference_only("rope_cache", v, k_cache, v_cache)
+    _inference_only("rope_cache", v, k_cache, v_cache, *((k_scale, v_scale) if scaled else ()))
     q_out, os_ = _out(q_out, "q_out", q)
     dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out, k_scale, v_scale)
     if q.shape[0]:

@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import CacheMoveArgs, TreeAcceptArgs, TreePlanArgs
-from .paged import _attend, _inference_only, _ints, _table, _written
+from .paged import _apart, _attend, _inference_only, _ints, _table, _written
 
 MOST = 1024                    # tokens of a request's tree
 
@@ -68,7 +68,8 @@ def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tens
     the token it follows, and one; it sees its ancestors and itself.  A parent that is
     not an index below the token's own counts as none.  ``max_new``: at least the most
     new tokens that one request has, up to 1024; a request's tokens past it (rounded up to
-    64) get position -1 and an empty mask.  ``out``: a former result to write into."""
+    64) get position -1 and an empty mask.  ``out``: a former result to write into, whose tensors are not this
+    call's inputs."""
     T = _tokens_by_row(parents, "parents")
     B = _rows_of(cu_lens)
     _ints(seq_lens, "seq_lens", (B,))
@@ -79,6 +80,7 @@ def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tens
     else:
         _lib.same_device(parents, _ints(out.positions, "out.positions", (T,)),
                          _ints(out.mask, "out.mask", (T, words), (torch.int64,)))
+        _apart((out.positions, out.mask), (parents, cu_lens, seq_lens), "they are read while it is written")
     if T:
         _lib.call("fs_tree_plan", TreePlanArgs(
             parents=parents.data_ptr(), cu_lens=cu_lens.data_ptr(), seq_lens=seq_lens.data_ptr(), B=B, T=T, words=words,
@@ -100,7 +102,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     tokens before the new ones are restricted to the last ``window`` up to the row's
     position (``positions`` int32 [T], taken within those of the request's new tokens) and the
     first ``sinks``; among the new ones the mask alone decides.  A row that sees no
-    token is 0.  Everything else as in ``paged_attention``, 8-bit caches too."""
+    token is 0.  Everything else as in ``paged_attention``, 8-bit caches too: the new
+    tokens' keys and values are in the cache, all of them (a value that is not finite may
+    reach rows of its request whose mask leaves it out)."""
     return _attend("tree_attention", q, k_cache, v_cache, block_table, cu_lens, seq_lens, mask, positions, max_new, window,
                    sinks, softmax_scale, k_scale, v_scale, out)
 
@@ -123,7 +127,7 @@ def accept_tree(parents: torch.Tensor, tokens: torch.Tensor, chosen: torch.Tenso
     request's first new token is kept; another one if its parent is and the parent's
     chosen token is this one (or the token is negative: given, not drafted), the
     lowest of several such.  ``max_new`` as in ``plan_tree``; a request's tokens past it are
-    not kept.  ``out``: a former result to write into."""
+    not kept.  ``out``: a former result to write into, whose tensors are not this call's inputs."""
     T = _tokens_by_row(parents, "parents")
     B = _rows_of(cu_lens)
     kinds = (torch.int32, torch.int64)
@@ -138,6 +142,8 @@ def accept_tree(parents: torch.Tensor, tokens: torch.Tensor, chosen: torch.Tenso
         _lib.same_device(parents, _ints(out.kept, "out.kept", (T,)), _ints(out.kept_lens, "out.kept_lens", (B,)),
                          _ints(out.dropped, "out.dropped", (B,)),
                          _ints(out.next_tokens, "out.next_tokens", (B,), (chosen.dtype,)))
+        _apart((out.kept, out.kept_lens, out.dropped, out.next_tokens), (parents, tokens, chosen, cu_lens),
+               "they are read while it is written")
     _lib.call("fs_tree_accept", TreeAcceptArgs(
         parents=parents.data_ptr(), tokens=tokens.data_ptr(), chosen=chosen.data_ptr(), cu_lens=cu_lens.data_ptr(),
         token_bytes=tokens.element_size(), B=B, T=T, most=most, kept=out.kept.data_ptr(), kept_lens=out.kept_lens.data_ptr(),

@@ -219,3 +219,45 @@ def test_half_steps_of_e4m3():
     x = torch.tensor([1.0, 1.9, 2.0, 0.5, 448.0, 300.0, 2.0 ** -6, 2.0 ** -7, 0.0, 500.0], dtype=torch.float64)
     assert tree.e4m3_half_step(x).tolist() == [2.0 ** -4, 2.0 ** -4, 2.0 ** -3, 2.0 ** -5, 16.0, 16.0, 2.0 ** -10, 2.0 ** -10,
                                                2.0 ** -10, 16.0]
+
+
+def _bytes(T=64, B=8, Hq=32, Hk=8, D=128, P=64, max_new=0, eight=True, tree=False):
+    a = _lib.PagedAttnArgs(dtype=1, B=B, T=T, Hq=Hq, Hk=Hk, D=D, P=P, page_size=64, max_new=max_new)
+    if eight:
+        a.k_scale = a.v_scale = 16
+    if tree:
+        a.mask, a.mask_words = 16, 1
+    return _lib.load().fs_paged_attn_work_bytes(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("eight", [False, True])
+def test_workspaces_of_the_forms_never_fall(eight, tree):
+    """One sized for the largest call of a form serves every smaller one of it, and 8-bit calls' serve 16-bit ones'."""
+    kw = dict(eight=eight, tree=tree)
+    for B in (1, 64, 4096):
+        for m in (0, 1, 8, 64):
+            n = [_bytes(T, B, max_new=m, **kw) for T in (1, 2, 8, 64, 1000, 4096, 100000)]
+            assert n == sorted(n) and n[0] > 0
+    for T in (1, 64, 5000):
+        for D in (64, 128):
+            n = [_bytes(T, 16, D=D, max_new=m, **kw) for m in [*range(1, 200), 0]]
+            assert n == sorted(n)
+        n = [_bytes(T, 16, P=1 << p, max_new=1, **kw) for p in range(20)]
+        assert n == sorted(n)
+        for m in (1, 64):
+            assert _bytes(T, 16, D=64, max_new=m, **kw) <= _bytes(T, 16, D=128, max_new=m, **kw)
+            heads = [(1, 1), (4, 1), (8, 1), (8, 2), (32, 2), (32, 8), (64, 8), (64, 64)]
+            n = [_bytes(T, 16, q, k, max_new=m, **kw) for q, k in heads]
+            assert n == sorted(n)
+            assert _bytes(T, 16, max_new=m, eight=True, tree=tree) >= _bytes(T, 16, max_new=m, eight=False, tree=tree)
+
+
+def test_scales_and_outputs_that_are_refused():
+    with pytest.raises(RuntimeError, match="no backward"):
+        fa.paged_attention(**_eight(k_scale=torch.ones(2, requires_grad=True)))
+    q, k = torch.zeros(6, 4, 128, dtype=BF), torch.zeros(6, 2, 128, dtype=BF)
+    c8 = torch.zeros(4, 16, 2, 128, dtype=torch.uint8).view(E4M3)
+    with pytest.raises(RuntimeError, match="no backward"):
+        fa.rope_cache(q, k, k, torch.zeros(6, dtype=I32), torch.zeros(6, dtype=I64), c8, c8, torch.ones(64, dtype=torch.float64),
+                      k_scale=torch.ones(2), v_scale=torch.ones(2, requires_grad=True))
