@@ -3,7 +3,10 @@
 //
 // All three are bound by latency: a batch's tokens are some kilobytes, so what counts is the
 // chain of loads that wait for each other.  One workgroup takes a request (its lengths, then its tokens,
-// side by side), follows parents and children in LDS, and writes.
+// side by side).  Lines of parents and of children are followed in LDS, one by one at first, as far as trees go, and then by
+// doubling: each round every token takes over what the token that it points to has, and that token's pointer, so a
+// line of d takes log2 d rounds.  (One by one alone, a line of 1024 took 386 us for the masks and 55 for the path, 37
+// and 12 so; by doubling alone trees of 16 took 4.2 and 4.5 us, 3.4 and 2.6 so.)
 #include <algorithm>
 #include <climits>
 
@@ -23,10 +26,15 @@ struct TreeRows {
   }
 };
 
-// Row t's ancestors are followed one by one; they come in falling order, so the words of its mask do
-// too and each is written once.
+constexpr int kSteps = 16;                         // one by one
+
+// rows[w][t]: word w of token t's mask.  After k rounds it holds t and its ancestors less than 16 2^k away, and up[t] is the one
+// 16 2^k away.  Ancestors come in falling order, so the steps write each word once.  In a round a row may take over one that has grown in the same round already: what it gets beyond is ancestors
+// as well.
 __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_args a) {
-  __shared__ int par[kTreeMost];
+  extern __shared__ uint64_t rows[];
+  const int cap = 64 * a.words;                    // tokens of a tree
+  int* par = reinterpret_cast<int*>(rows + (size_t)a.words * cap);
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {                                  // rows that no request has
     for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) {
@@ -37,37 +45,77 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_ar
   }
   const TreeRows r(a.cu_lens, b, a.T);
   const int64_t first = (int64_t)a.seq_lens[b] - r.n;
-  const int most = min(r.n, 64 * a.words);
+  const int most = min(r.n, cap);
   for (int t = tid; t < most; t += kTreeThreads) par[t] = a.parents[r.c0 + t];
   __syncthreads();
-  for (int t = tid; t < r.n; t += kTreeThreads) {
-    int64_t* row = a.mask + (int64_t)(r.c0 + t) * a.words;
-    int w = a.words, at = t, depth = 0;
+  constexpr int PER = kTreeMost / kTreeThreads;
+  int up[PER];
+  bool more = false;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = tid + i * kTreeThreads;
+    up[i] = -1;
+    if (t >= most) continue;
+    int at = t, w = a.words;
     uint64_t word = 0;
-    while (t < most) {
+    for (int s = 0; s < kSteps && at >= 0; ++s) {
       if (at >> 6 != w) {
-        if (w < a.words) row[w] = (int64_t)word;
-        while (--w > at >> 6) row[w] = 0;
+        if (w < a.words) rows[w * cap + t] = word;
+        while (--w > at >> 6) rows[w * cap + t] = 0;
         word = 0;
       }
       word |= 1ull << (at & 63);
       const int p = par[at];
-      if (p < 0 || p >= at) break;
-      at = p;
-      ++depth;
+      at = p < at ? p : -1;                        // a parent below 0, or not below the token: none
     }
-    if (w < a.words) row[w] = (int64_t)word;
-    while (--w >= 0) row[w] = 0;
+    rows[w * cap + t] = word;
+    while (--w >= 0) rows[w * cap + t] = 0;
+    up[i] = max(at, -1);
+    more |= at >= 0;
+  }
+  if (__syncthreads_or(more)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (tid + i * kTreeThreads < most) par[tid + i * kTreeThreads] = up[i];   // now: the token that it is followed to
+  }
+  while (__syncthreads_or(more)) {
+    int next[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int t = tid + i * kTreeThreads, p = t < most ? par[t] : -1;
+      next[i] = -1;
+      if (p < 0) continue;
+      for (int w = 0; w <= p >> 6; ++w) rows[w * cap + t] |= rows[w * cap + p];
+      next[i] = par[p];
+    }
+    __syncthreads();
+    more = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int t = tid + i * kTreeThreads;
+      if (t < most) par[t] = next[i];
+      more |= next[i] >= 0;
+    }
+  }
+  for (int t = tid; t < r.n; t += kTreeThreads) {
+    int depth = -1;
+    for (int w = 0; w < a.words; ++w) {
+      const uint64_t x = t < most ? rows[w * cap + t] : 0;
+      a.mask[(int64_t)(r.c0 + t) * a.words + w] = (int64_t)x;
+      depth += __popcll(x);
+    }
     a.positions[r.c0 + t] = t < most ? (int)(first + depth) : -1;
   }
 }
 
-// Every token that its parent's choice agrees with names itself to the parent, which keeps the lowest; one
-// thread follows those names from the first token on.
+// Every token that its parent's choice agrees with names itself to the parent, which keeps the lowest (`next`).  The tokens
+// that the first one comes to, if it is a long path, are marked; on a path the numbers rise, so a token's place on it is the number of marks below.
 template <typename I>
 __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accept_args a) {
-  __shared__ int child[kTreeMost], path[kTreeMost];
-  __shared__ int count;
+  constexpr int PER = kTreeMost / kTreeThreads, NW = kTreeThreads / 64;
+  __shared__ int next[kTreeMost];
+  __shared__ uint8_t marked[kTreeMost];
+  __shared__ int marks[PER][NW], path[kSteps], steps, last;
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {
     for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) a.kept[t] = -1;
@@ -76,25 +124,72 @@ __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accep
   const I *tokens = static_cast<const I*>(a.tokens), *chosen = static_cast<const I*>(a.chosen);
   const TreeRows r(a.cu_lens, b, a.T);
   const int most = min(r.n, a.most);
-  for (int t = tid; t < most; t += kTreeThreads) child[t] = INT_MAX;
+  if (tid == 0) last = 0;
+  for (int t = tid; t < most; t += kTreeThreads) {
+    next[t] = INT_MAX;
+    marked[t] = t == 0;
+  }
   __syncthreads();
   for (int t = tid; t < most; t += kTreeThreads) {
     const int p = a.parents[r.c0 + t];
     if (p < 0 || p >= t) continue;
     const I x = tokens[r.c0 + t];
-    if (x < 0 || x == chosen[r.c0 + p]) atomicMin(&child[p], t);   // the least of them, in whatever order
+    if (x < 0 || x == chosen[r.c0 + p]) atomicMin(&next[p], t);   // the least of them, in whatever order
   }
   __syncthreads();
   if (tid == 0) {
-    int k = 0;
-    for (int t = 0; t < most; t = child[t]) path[k++] = t;
-    count = k;
-    a.kept_lens[b] = k;
-    a.dropped[b] = k - max(r.n, 0);
-    static_cast<I*>(a.next_tokens)[b] = k ? chosen[r.c0 + path[k - 1]] : (I)-1;
+    int k = 0, t = 0;
+    for (; t < most && k < kSteps; t = next[t]) path[k++] = t;
+    steps = t < most ? -1 : k;                     // -1: it goes on
+    if (t >= most) {
+      a.kept_lens[b] = k;
+      a.dropped[b] = k - max(r.n, 0);
+      static_cast<I*>(a.next_tokens)[b] = k ? chosen[r.c0 + path[k - 1]] : (I)-1;
+    }
   }
   __syncthreads();
-  for (int t = tid; t < r.n; t += kTreeThreads) a.kept[r.c0 + t] = t < count ? path[t] : -1;
+  if (steps >= 0) {
+    for (int t = tid; t < r.n; t += kTreeThreads) a.kept[r.c0 + t] = t < steps ? path[t] : -1;
+    return;
+  }
+  // After k rounds the first 2^k tokens of the path are marked and next[t] is 2^k on.
+  while (next[0] < most) {
+    int on[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int t = tid + i * kTreeThreads, n = t < most ? next[t] : INT_MAX;
+      on[i] = n < most ? next[n] : INT_MAX;
+      if (n < most && marked[t]) marked[n] = 1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (tid + i * kTreeThreads < most) next[tid + i * kTreeThreads] = on[i];
+    __syncthreads();
+  }
+  uint64_t who[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int t = tid + i * kTreeThreads;
+    who[i] = __ballot(t < most && marked[t]);
+    if ((tid & 63) == 0) marks[i][tid >> 6] = (int)__popcll(who[i]);
+  }
+  __syncthreads();
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    for (int w = 0; w < NW; ++w) {
+      if (w == tid >> 6 && who[i] >> (tid & 63) & 1) a.kept[r.c0 + count + rank_below(who[i])] = tid + i * kTreeThreads;
+      count += marks[i][w];
+      if (w == tid >> 6 && marks[i][w] && (tid & 63) == 0) atomicMax(&last, i * kTreeThreads + w * 64 + 63 - (int)__builtin_clzll(who[i]));
+    }
+  for (int t = count + tid; t < r.n; t += kTreeThreads) a.kept[r.c0 + t] = -1;
+  __syncthreads();
+  if (tid == 0) {
+    a.kept_lens[b] = count;
+    a.dropped[b] = count - max(r.n, 0);
+    static_cast<I*>(a.next_tokens)[b] = count ? chosen[r.c0 + last] : (I)-1;
+  }
 }
 
 constexpr int kMoveLayers = 64;                    // of a launch
@@ -193,7 +288,9 @@ extern "C" int fs_tree_plan(const fs_tree_plan_args* a, void* stream) {
   FS_CHECK_SUPPORTED(a->words <= kTreeMost / 64, "%s: trees of %d tokens > %d", fn, 64 * a->words, kTreeMost);
   if (a->T == 0) return FS_OK;
   FS_CHECK_ARG(a->parents && a->cu_lens && a->seq_lens && a->positions && a->mask, "%s: null tensor pointer", fn);
-  tree_plan_kernel<<<a->B + 1, kTreeThreads, 0, (hipStream_t)stream>>>(*a);
+  const size_t bytes = (size_t)a->words * 64 * (a->words * sizeof(uint64_t) + sizeof(int));   // 132 KiB at most
+  if (int rc = fs_host::allow_dynamic_lds(tree_plan_kernel, bytes, fn)) return rc;
+  tree_plan_kernel<<<a->B + 1, kTreeThreads, bytes, (hipStream_t)stream>>>(*a);
   return fs_host::launch_status(fn);
 }
 
