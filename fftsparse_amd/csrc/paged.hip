@@ -1,3 +1,4 @@
+// Entry points of paged and window attention, and the kernels' form over 16-bit keys and values without trees.
 #include "paged_kernel.h"
 
 using namespace fs;

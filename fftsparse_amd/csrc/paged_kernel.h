@@ -44,6 +44,18 @@
 // of the tile may read as a whole (the end of the request, the window's edge, a
 // page that is none) is copied row by row, zeros in place of the rows that no row
 // of the tile sees: nothing stands there that could spoil a sum.
+//
+// 8-bit pages (k8): tiles stay e4m3 in LDS, half as large, and operands are widened to the input type, which holds every e4m3
+// number, as they are read (the transposing read of V by bytes).  A key's scale goes into the scores' factor, a value's
+// into the sums at the end.  Two workgroups of few_kernel share a CU, so that as many bytes are on their way as in 16 bits.  Measured
+// (bf16, D = 128, 32 / 8 heads): 64 requests of 64 - 8192 tokens 62 us (103 in 16 bits), 64 of 4096 119 to 124 us, 4.3 to 4.5 TB/s
+// (112 us, 4.8 TB/s, from pages that keep a head's rows together: pieces of 128 bytes of a token's 1024 cost the rest); a
+// chunk of 2048 tokens over 30000 1080 us, 0.99 PFLOP/s.  Widening each group once into 16-bit tiles, a quarter of the
+// conversions, was no faster (1072 us, trees at D = 64 5% slower): the conversions are not what bounds it.
+//
+// Trees (kTree): rows of a request see its context and the new tokens that their masks name, so all row tiles of a request
+// have the same keys and only the last tiles are looked up.  Otherwise as a chain, and as fast (16 requests of 8192 with 64
+// new tokens each 183 us, chains 181; 0.75 PFLOP/s: the keys come from HBM for two row tiles, not from L2 for many).
 #pragma once
 #include <algorithm>
 #include <cmath>

@@ -445,7 +445,7 @@ FS_API int fs_plan(const fs_plan_args* a, void* stream);
  * k_scale and v_scale (both, with slots): the caches are in e4m3, and the rotated
  * key and the value of KV head h are written as x / scale[h], held to -448 .. 448
  * and rounded once from 32 bits to nearest even (nan stays nan).  Scales are
- * positive and finite; cache strides multiples of 16 elements. */
+ * positive, finite and not subnormal; cache strides multiples of 16 elements. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   const void* k; int64_t k_st, k_sh;
@@ -495,14 +495,15 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * race.
  * k_scale and v_scale (both): the caches are in e4m3, and a number x of KV head h
  * stands for x * scale[h] (positive and finite); cache strides are multiples of 16
- * elements.  Scores are of q in dtype and the e4m3 numbers, exact in dtype.
+ * elements.  Scores are of q in dtype and the e4m3 numbers, exact in dtype.  The
+ * workspace is about 17 MB where it is 9 above.
  * mask: the rows of a request are not a chain but a tree, or any other set.  The row
  * sees the tokens before the request's n new ones, and new token j of its request (the
  * one at seq_lens[b] - n + j) where bit j % 64 of word j / 64 of its row of the mask
  * is set, itself included only so.  New tokens past the mask's words are seen by none.
  * With a window the tokens before the new ones are seen by the row's position
  * (positions[t], taken within those of the new tokens) as above, the new ones by the
- * mask alone. */
+ * mask alone.  All new tokens' keys and values are read. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   void* out; int64_t o_st, o_sh;
