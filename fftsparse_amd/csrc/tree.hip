@@ -29,15 +29,15 @@ struct TreeRows {
 constexpr int kSteps = 16;                         // one by one
 
 // rows[w][t]: word w of token t's mask.  After k rounds it holds t and its ancestors less than 16 2^k away, and up[t] is the one
-// 16 2^k away.  Ancestors come in falling order, so the steps write each word once.  In a round a row may take over one that has grown in the same round already: what it gets beyond is ancestors
-// as well.
+// 16 2^k away.  Ancestors come in falling order, so the steps write each word once.  In a round a row may take over one that
+// has grown in the same round already: what it gets beyond is ancestors as well.
 __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_args a) {
   extern __shared__ uint64_t rows[];
   const int cap = 64 * a.words;                    // tokens of a tree
   int* par = reinterpret_cast<int*>(rows + (size_t)a.words * cap);
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {                                  // rows that no request has
-    for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) {
+    for (int t = min(max(a.cu_lens[a.B], 0), a.T) + tid; t < a.T; t += kTreeThreads) {
       a.positions[t] = -1;
       for (int w = 0; w < a.words; ++w) a.mask[(int64_t)t * a.words + w] = 0;
     }
@@ -109,7 +109,8 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_ar
 }
 
 // Every token that its parent's choice agrees with names itself to the parent, which keeps the lowest (`next`).  The tokens
-// that the first one comes to, if it is a long path, are marked; on a path the numbers rise, so a token's place on it is the number of marks below.
+// that the first one comes to, if it is a long path, are marked; on a path the numbers rise, so a token's place on it is
+// the number of marks below.
 template <typename I>
 __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accept_args a) {
   constexpr int PER = kTreeMost / kTreeThreads, NW = kTreeThreads / 64;
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accep
   __shared__ int marks[PER][NW], path[kSteps], steps, last;
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {
-    for (int t = max(a.cu_lens[a.B], 0) + tid; t < a.T; t += kTreeThreads) a.kept[t] = -1;
+    for (int t = min(max(a.cu_lens[a.B], 0), a.T) + tid; t < a.T; t += kTreeThreads) a.kept[t] = -1;
     return;
   }
   const I *tokens = static_cast<const I*>(a.tokens), *chosen = static_cast<const I*>(a.chosen);

@@ -132,7 +132,7 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     Returns q_rot.  A slot outside the cache (-1: none) is not written; a row with a negative position is left as it
     was, in the cache too.
 
-    Caches of ``torch.float8_e4m3fn`` need ``k_scale`` and ``v_scale`` (float32 [Hk], positive, finite, not subnormal): x / scale[h] is
+    Caches of ``torch.float8_e4m3fn`` need ``k_scale`` and ``v_scale`` (float32 [Hk], 2^-126 to 2^126): x / scale[h] is
     written, held to -448 .. 448 and rounded once, from 32 bits (nan stays nan)."""
     q, qs, k, ks, inv_freq = _common("rope_cache", q, k, positions, inv_freq)
     v, vs = _rows(v, "v")

@@ -211,3 +211,28 @@ def test_the_largest_trees(bits):
     tokens = torch.arange(b.T, device=DEV)
     a = fa.accept_tree(_i32(parents), tokens, tokens + 1, cu, max_new=1024)
     assert a.kept_lens.tolist() == [1024, 700] and a.kept.tolist() == [*range(1024), *range(700)]
+
+
+@pytest.mark.parametrize("last", [2 ** 31 - 1, -(2 ** 31)])
+def test_row_numbers_at_the_ends_of_their_range(last):
+    """A last row number far out of range is taken as the number of rows, or as 0, and nothing outside the outputs is written."""
+    T, B = 70, 1
+    parents = torch.arange(-1, T - 1, dtype=I32, device=DEV)
+    cu = torch.tensor([0, last], dtype=I32, device=DEV)
+    n = T if last > 0 else 0
+    held = torch.full((3 * T,), 7, dtype=I32, device=DEV)
+    masks = torch.full((3 * T, 2), 7, dtype=torch.int64, device=DEV)
+    fa.plan_tree(parents, cu, _i32([n]), max_new=128, out=fa.TreePlan(held[T:2 * T], masks[T:2 * T]))
+    torch.cuda.synchronize()
+    assert held[T:2 * T].tolist() == (list(range(T)) if n else [-1] * T)
+    want = [[(1 << min(t + 1, 63)) - 1 | (-(1 << 63) if t > 62 else 0), (1 << max(t - 63, 0)) - 1] for t in range(T)]
+    assert masks[T:2 * T].tolist() == (want if n else [[0, 0]] * T)
+    tokens = torch.ones(T, dtype=I32, device=DEV)
+    kept = torch.full((3 * T,), 7, dtype=I32, device=DEV)
+    small = torch.zeros(2, B, dtype=I32, device=DEV)
+    acc = fa.accept_tree(parents, tokens, tokens, cu, max_new=128,
+                         out=fa.Accepted(kept[T:2 * T], small[0], small[1], tokens.new_empty(B)))
+    assert kept[T:2 * T].tolist() == (list(range(T)) if n else [-1] * T)
+    assert acc.kept_lens.tolist() == [n] and acc.dropped.tolist() == [0]
+    for x in (held, kept, masks):
+        assert bool((x[:T] == 7).all()) and bool((x[2 * T:] == 7).all())
