@@ -50,7 +50,7 @@
 // into the sums at the end.  Two workgroups of few_kernel share a CU, so that as many bytes are on their way as in 16 bits.  Measured
 // (bf16, D = 128, 32 / 8 heads): 64 requests of 64 - 8192 tokens 62 us (103 in 16 bits), 64 of 4096 119 to 124 us, 4.3 to 4.5 TB/s
 // (112 us, 4.8 TB/s, from pages that keep a head's rows together: pieces of 128 bytes of a token's 1024 cost the rest); a
-// chunk of 2048 tokens over 30000 1080 us, 0.99 PFLOP/s.  Widening each group once into 16-bit tiles, a quarter of the
+// chunk of 2048 tokens over 30000 1080 - 1104 us, 0.95 PFLOP/s.  Widening each group once into 16-bit tiles, a quarter of the
 // conversions, was no faster (1072 us, trees at D = 64 5% slower): the conversions are not what bounds it.
 //
 // Trees (kTree): rows of a request see its context and the new tokens that their masks name, so all row tiles of a request
