@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import CacheMoveArgs, TreeAcceptArgs, TreePlanArgs
-from .paged import _apart, _attend, _inference_only, _ints, _table, _written
+from .paged import _apart, _attend, _inference_only, _ints, _strides, _table, _written
 
 MOST = 1024                    # tokens of a request's tree
 
@@ -161,16 +161,16 @@ def _layers(caches, name: str, shape, dtype):
     if isinstance(caches, torch.Tensor):
         if caches.dim() == len(shape):
             return 1, None, caches.data_ptr(), (0, *_written(caches, name, shape, dtype)), (caches,)
-        n, st, whole = caches.shape[0], caches.stride(), caches.shape[1:]
-        if whole != shape or caches.dtype != dtype:
+        whole, st, size = caches.shape, _strides(caches), caches.element_size()
+        if whole[1:] != shape or caches.dtype != dtype:
             raise ValueError(f"{name} must be a [layers, {', '.join(map(str, shape))}] {dtype} tensor, got {caches.dtype} "
-                             f"{tuple(caches.shape)}")
-        per = 16 // caches.element_size()
-        if st[4] != 1 and shape[3] > 1 or caches.data_ptr() & 15 or any(
-                m > 1 and (s % per or s == 0) for s, m in zip(st[:4], caches.shape)):
+                             f"{tuple(whole)}")
+        p, (s0, s1, s2, s3, sd) = caches.data_ptr(), st
+        if (sd != 1 and shape[3] > 1) or (p | (s0 | s1 | s2 | s3) * size) & 15 or (
+                0 in st and any(m > 1 and s == 0 for s, m in zip(st, whole))):
             raise ValueError(f"{name} must have d contiguous, the other strides multiples of 16 bytes, 16-byte alignment and no "
-                             f"broadcast dimension, got strides {st}")
-        return n, None, caches.data_ptr(), [s if m > 1 else 0 for s, m in zip(st[:4], caches.shape)], (caches,)
+                             f"broadcast dimension, got strides {caches.stride()}")
+        return whole[0], None, p, st, (caches,)
     if not len(caches):
         raise ValueError(f"{name} holds no layer")
     st = _written(caches[0], name, shape, dtype)
@@ -203,7 +203,11 @@ def move_kept(k_cache: torch.Tensor | Sequence[torch.Tensor], v_cache: torch.Ten
         raise TypeError(f"unsupported cache type {dtype}")
     pages, ps, Hk, D = shape
     n, kp, k0, ks, kt = _layers(k_cache, "k_cache", shape, dtype)
-    m, vp, v0, vs, vt = _layers(v_cache, "v_cache", shape, dtype)
+    if (isinstance(v_cache, torch.Tensor) and one is k_cache and v_cache.dtype == dtype and v_cache.shape == k_cache.shape
+            and v_cache.stride() == k_cache.stride() and not v_cache.data_ptr() & 15):
+        m, vp, v0, vs, vt = n, None, v_cache.data_ptr(), ks, (v_cache,)    # laid out as k_cache is
+    else:
+        m, vp, v0, vs, vt = _layers(v_cache, "v_cache", shape, dtype)
     if n != m or (kp is None) != (vp is None):
         raise ValueError(f"{n} layers of keys and {m} of values, or not in one form")
     B, P, t_sb = _table(block_table)
