@@ -50,8 +50,8 @@
 // into the sums at the end.  Two workgroups of few_kernel share a CU, so that as many bytes are on their way as in 16 bits.  Measured
 // (bf16, D = 128, 32 / 8 heads): 64 requests of 64 - 8192 tokens 62 us (103 in 16 bits), 64 of 4096 119 to 124 us, 4.3 to 4.5 TB/s
 // (112 us, 4.8 TB/s, from pages that keep a head's rows together: pieces of 128 bytes of a token's 1024 cost the rest); a
-// chunk of 2048 tokens over 30000 1080 - 1104 us, 0.95 PFLOP/s.  Widening each group once into 16-bit tiles, a quarter of the
-// conversions, was no faster (1072 us, trees at D = 64 5% slower): the conversions are not what bounds it.
+// chunk of 2048 tokens over 30000 980 us, 1.06 PFLOP/s, as over 16-bit pages.  Widening each group once into 16-bit tiles, a
+// quarter of the conversions, took 1072 us (trees at D = 64 5% slower).
 //
 // Trees (kTree): rows of a request see its context and the new tokens that their masks name, so all row tiles of a request
 // have the same keys and only the last tiles are looked up.  Otherwise as a chain, and as fast (16 requests of 8192 with 64
@@ -1185,15 +1185,33 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       rs = exps(s_cur, p_cur, (m_run == -INFINITY ? 0.f : m_run) - kBias<T>);
     }
     if constexpr (decltype(hasS)::value && decltype(hasPV)::value && decltype(hasE)::value) {
-      // one MFMA, then three VALU instructions, operand reads eight MFMAs ahead (6: 1.9% slower, 10: 65%; VPM 4: 0.5%)
-      constexpr int NS = 2 * (D / 16), NM = NS + 4 * (D / 32), LA = 8, VPM = 3;
-      __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
+      constexpr int NS = 2 * (D / 16), NM = NS + 4 * (D / 32), LA = 8;
+      if constexpr (!((F & k8) && (D == 128 || !(F & kTree)))) {
+        // one MFMA, then three VALU instructions, operand reads eight MFMAs ahead (6: 1.9% slower, 10: 65%; VPM 4: 0.5%)
+        constexpr int VPM = 3;
+        __builtin_amdgcn_sched_group_barrier(0x100, LA, 0);
 #pragma unroll
-      for (int i = 0; i < NM; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (i + LA < NS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        else if (i + LA < NM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
+        for (int i = 0; i < NM; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i + LA < NS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          else if (i + LA < NM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, VPM, 0);
+        }
+      } else {
+        // From e4m3 an operand takes four conversions (128 of the step's 296 VALU instructions at D = 128), so as many go
+        // before the first MFMA, and after each the next operand's and one more (of S) or two (of P V) of the softmax's; a read of
+        // keys serves two MFMAs.  In the order above, which has no place for them, 2048 tokens over 30000 took 1047 us and not 929 (D =
+        // 64, 28 / 4 heads: 673 and 602); with 4 or 6 in place of 5 1020 to 1054, with 5, 7, 9 in place of the second 6 1 to 3%
+        // more, with 3 or 8 before the first 13% and 4%.  Trees at D = 64 stay with it: 16 of 64 over 8192 112 us and not 123.
+        __builtin_amdgcn_sched_group_barrier(0x100, LA / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i + LA < NS ? ((i + LA) & 3) < 2 : i + LA < NM) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          if (i < NS) __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+          else __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);
+        }
       }
     }
     if constexpr (decltype(hasE)::value) {
