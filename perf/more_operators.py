@@ -220,7 +220,8 @@ def prepare(case, seed):
         tokens = torch.randint(1, 128000, (T,), generator=g, device=DEV)
         first = torch.tensor([0] + new).cumsum(0).tolist()
         like = torch.tensor([first[b] + t if t >= 0 else -1 for b, x in enumerate(liked) for t in x], device=DEV)
-        return dict(s, tokens=tokens, chosen=torch.where(like >= 0, tokens[like.clamp(min=0)], 0))
+        return dict(s, tokens=tokens, chosen=torch.where(like >= 0, tokens[like.clamp(min=0)], 0), k_layers=list(kc),
+                    v_layers=list(vc))
     if case["op"] == "store":
         qkv = randn(T, (Hq + 2 * Hk) * D).to(dt)           # the views of one projection
         q, k, v = (x.view(T, -1, D) for x in qkv.split([Hq * D, Hk * D, Hk * D], dim=1))
@@ -257,7 +258,7 @@ def _own(s):
         return dict(q=q, kc=s["kc"], vc=s["vc"])
     if c["op"] == "verify":
         a = fa.accept_tree(s["parents"], s["tokens"], s["chosen"], s["cu"], max_new=s["N"])
-        fa.move_kept(s["kc"], s["vc"], s["table"], s["cu"], s["lens"], a.kept)
+        fa.move_kept(s["k_layers"], s["v_layers"], s["table"], s["cu"], s["lens"], a.kept)
         return dict(kept=a.kept, count=a.kept_lens, dropped=a.dropped, next=a.next_tokens, kc=s["kc"], vc=s["vc"])
     w = dict(max_new=s["N"], window=c["window"] or None, sinks=c["sinks"], **scales)
     if c["op"] == "attend":
