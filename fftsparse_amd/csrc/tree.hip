@@ -9,6 +9,9 @@
 // and 12 so; by doubling alone trees of 16 took 4.2 and 4.5 us, 3.4 and 2.6 so.)
 #include <algorithm>
 #include <climits>
+#include <new>
+#include <utility>
+#include <vector>
 
 #include "common.h"
 
@@ -275,6 +278,95 @@ __global__ __launch_bounds__(kTreeThreads) void cache_move_kernel(MoveKArgs ka) 
 
 using namespace fs;
 
+// Part of an offset into the caches: lo to hi times `step` bytes.
+struct Term {
+  int64_t step, lo, hi;
+};
+// Whether some sum of the terms from t to `end`, the largest steps first, is less than `row` bytes from d: two caches d
+// apart then have bytes in common, where the terms are what can lie between two of their rows.  Steps that hold all
+// smaller ones (every layout that is a view of a dense tensor) leave one or two numbers to try for each; `tries`
+// bounds the others (0: not known, taken as shared).
+static bool shares(const Term* t, const Term* end, int64_t d, int64_t row, int& tries) {
+  int64_t lo = 1 - row, hi = row - 1;              // what the terms after t reach
+  if (t == end) return d >= lo && d <= hi;
+  for (const Term* x = t + 1; x < end; ++x) {
+    lo += x->step * x->lo;
+    hi += x->step * x->hi;
+  }
+  auto down = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+  const int64_t from = std::max(t->lo, -down(hi - d, t->step)), to = std::min(t->hi, down(d - lo, t->step));
+  for (int64_t c = from; c <= to; ++c)
+    if (--tries < 0 || shares(t + 1, end, d - c * t->step, row, tries)) return true;
+  return false;
+}
+// Whether the caches of a move have bytes in common.  Each is moved by workgroups of its own, so one that is named twice would be
+// moved twice, in any order.
+static bool caches_share(const fs_cache_move_args& a, const std::vector<std::pair<int64_t, bool>>& at) {
+  const int64_t e = a.elem_bytes, row = a.D * e;
+  const int64_t n[] = {a.layers, std::min<int64_t>(a.num_pages, INT_MAX), a.page_size, a.Hk};   // a table's numbers are below
+  const int64_t st[2][4] = {{at.empty() ? a.k_sl * e : 0, a.k_sp * e, a.k_ss * e, a.k_sh * e},
+                            {at.empty() ? a.v_sl * e : 0, a.v_sp * e, a.v_ss * e, a.v_sh * e}};
+  // cache y of kind vy lies d bytes behind cache x of kind vx; layers: from another layer on (0: any)
+  auto pair = [&](bool vx, bool vy, int64_t d, int layers) {
+    Term t[8];
+    int m = 0;
+    auto add = [&](int64_t step, int64_t lo, int64_t hi) {
+      if (step < 0) {
+        step = -step;
+        std::swap(lo, hi);
+        lo = -lo;
+        hi = -hi;
+      }
+      if (step == 0 || (lo == 0 && hi == 0)) return;
+      for (int i = 0; i < m; ++i)
+        if (t[i].step == step) {
+          t[i].lo += lo;
+          t[i].hi += hi;
+          return;
+        }
+      t[m++] = {step, lo, hi};
+    };
+    for (int i = 0; i < 4; ++i) {
+      if (i == 0 && layers) {
+        add(st[vx][0], layers, n[0] - 1);
+        continue;
+      }
+      add(st[vx][i], 0, n[i] - 1);
+      add(st[vy][i], 1 - n[i], 0);
+    }
+    std::sort(t, t + m, [](const Term& x, const Term& y) { return x.step > y.step; });
+    int tries = 1 << 16;
+    return shares(t, t + m, d, row, tries);
+  };
+  if (at.empty())
+    return (a.layers > 1 && (pair(false, false, 0, 1) || pair(true, true, 0, 1))) ||
+           pair(false, true, (int64_t)((uintptr_t)a.v_cache - (uintptr_t)a.k_cache), 0);
+  int64_t size[2], inner[2];                       // bytes from a cache's first to its last, and from a page's
+  bool mixed = false;
+  for (int v = 0; v < 2; ++v) {
+    inner[v] = row;
+    for (int i = 2; i < 4; ++i) inner[v] += st[v][i] * (n[i] - 1);
+    size[v] = inner[v] + st[v][1] * (n[1] - 1);
+    for (int i = 1; i < 4; ++i) mixed |= st[v][i] < 0;
+  }
+  const bool back = mixed;                         // some run backwards: every two are looked at
+  for (size_t i = 0; i + 1 < at.size(); ++i) mixed |= at[i].first + size[at[i].second] > at[i + 1].first;
+  if (!mixed) return false;
+  // pages of several caches side by side: each has a place of its own within a step from page to page
+  if (!back && st[0][1] == st[1][1] && st[0][1] > 0) {
+    std::vector<std::pair<int64_t, bool>> in(at);
+    for (auto& x : in) x.first %= st[0][1];
+    std::sort(in.begin(), in.end());
+    bool apart = in.back().first + inner[in.back().second] <= in[0].first + st[0][1];
+    for (size_t i = 0; i + 1 < in.size(); ++i) apart &= in[i].first + inner[in[i].second] <= in[i + 1].first;
+    if (apart) return false;
+  }
+  for (size_t i = 0; i < at.size(); ++i)
+    for (size_t j = i + 1; j < at.size() && (back || at[j].first < at[i].first + std::max(size[0], size[1])); ++j)
+      if (pair(at[i].second, at[j].second, at[j].first - at[i].first, 0)) return true;
+  return false;
+}
+
 static int check_tree(const char* fn, int B, int T) {
   FS_CHECK_ARG(B >= 1 && T >= 0, "%s: B=%d requests, T=%d rows", fn, B, T);
   FS_CHECK_SUPPORTED(B <= 65535, "%s: %d requests > 65535", fn, B);
@@ -335,6 +427,17 @@ extern "C" int fs_cache_move(const fs_cache_move_args* a, void* stream) {
   for (int i = 0; i < a->layers; ++i)
     FS_CHECK_ARG(cache(false, i) && cache(true, i) && ((uintptr_t)cache(false, i) | (uintptr_t)cache(true, i)) % 16 == 0,
                  "%s: caches must be given, 16-byte aligned", fn);
+  bool share = false;
+  try {
+    std::vector<std::pair<int64_t, bool>> at;      // address, whether of values; in order
+    for (int i = 0; arrays && i < a->layers; ++i)
+      for (bool v : {false, true}) at.emplace_back((int64_t)(uintptr_t)cache(v, i), v);
+    std::sort(at.begin(), at.end());
+    share = caches_share(*a, at);
+  } catch (const std::bad_alloc&) {
+    FS_CHECK_SUPPORTED(false, "%s: no host memory to look over %d layers", fn, a->layers);
+  }
+  FS_CHECK_ARG(!share, "%s: caches share storage; each is moved once: name it once", fn);
   for (int l0 = 0; l0 < a->layers; l0 += kMoveLayers) {
     MoveKArgs k{*a, 1, {}};
     const int n = std::min(a->layers - l0, kMoveLayers);

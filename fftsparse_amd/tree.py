@@ -191,7 +191,9 @@ def move_kept(k_cache: torch.Tensor | Sequence[torch.Tensor], v_cache: torch.Ten
     ``k_cache`` / ``v_cache``: one layer's caches [pages, page_size, Hk, D], those of
     several layers in one tensor [layers, pages, page_size, Hk, D], or a sequence of the
     first (all of one layout; bf16, f16, f32 or ``torch.float8_e4m3fn``; rows of a
-    multiple of 16 bytes).  ``seq_lens`` int32 [B]: new tokens included, as for the step's
+    multiple of 16 bytes).  Each cache is moved by itself, so all of them have to be apart:
+    one that several layers read is named once (caches that share storage are refused; views of
+    one storage that lie between each other's rows are apart).  ``seq_lens`` int32 [B]: new tokens included, as for the step's
     attention; ``kept`` int32 [T] from ``accept_tree``.  Up to 64 layers go in one
     launch.  Tokens without a page stay as they are; of a request the first 1024 are
     looked at."""

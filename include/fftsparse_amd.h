@@ -594,6 +594,7 @@ FS_API int fs_tree_accept(const fs_tree_accept_args* a, void* stream);
  * of the same shape and strides: k_caches and v_caches, host arrays of device pointers, or,
  * where these are NULL, k_cache + i * k_sl and v_cache + i * v_sl (elements) for layer i.
  * elem_bytes 1, 2 or 4; rows of D * elem_bytes, a multiple of 16 bytes, strides too.
+ * The caches must have no byte in common, of another layer or of keys and values (checked on the host: each is moved once).
  * Tokens whose page is none stay.  Of a request only the first 1024 tokens are looked
  * at. */
 typedef struct {

@@ -1,0 +1,66 @@
+"""Calls of the tree operators on the GPU that the documentation allows beside the usual ones, and some that it refuses."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fftsparse_amd as fa
+from tests.test_gpu_tree import BF, DEV, E4M3, I32, _i32, _moved
+
+pytestmark = pytest.mark.gpu
+
+LAYERS, PAGES, PS, HK, D = 3, 5, 16, 2, 64
+TABLE = [[3, 0, -1], [4, 1, 2]]
+CU, LENS, KEPT = [0, 12, 32], [30, 40], [0, 2, 3, 7, 11, *[-1] * 7, 0, 1, 4, 9, 10, 18, 19, *[-1] * 13]
+
+
+def _views(form, dtype):
+    """One storage and the layers' keys and values in it, [PAGES, PS, HK, D] each."""
+    n = 2 * LAYERS * PAGES * PS * HK * D * torch.empty(0, dtype=dtype).element_size()
+    raw = torch.randint(0, 256, (n,), generator=torch.Generator().manual_seed(1), dtype=torch.uint8).to(DEV)
+    x = raw.view(dtype)
+    if form == "pages hold all layers":
+        x = x.view(PAGES, LAYERS, 2, PS, HK, D)
+        return raw, [x[:, i, 0] for i in range(LAYERS)], [x[:, i, 1] for i in range(LAYERS)]
+    if form == "tokens hold keys and values":
+        x = x.view(LAYERS, PAGES, PS, 2, HK, D)
+        return raw, x[:, :, :, 0], x[:, :, :, 1]
+    if form == "heads hold keys and values":
+        x = x.view(LAYERS, PAGES, PS, HK, 2, D)
+        return raw, [*x[..., 0, :]], [*x[..., 1, :]]
+    if form == "values by heads":                          # of each page, behind the keys by tokens
+        x = x.view(LAYERS, PAGES, 2, PS * HK * D)
+        return (raw, [*x[:, :, 0].view(LAYERS, PAGES, PS, HK, D)],
+                [*x[:, :, 1].view(LAYERS, PAGES, HK, PS, D).transpose(2, 3)])
+    x = x.view(2 * LAYERS, PAGES, PS, HK, D)               # keys and values in turn
+    return raw, [*x[::2]], [*x[1::2]]
+
+
+@pytest.mark.parametrize("dtype", [BF, E4M3])
+@pytest.mark.parametrize("form", ["pages hold all layers", "tokens hold keys and values", "heads hold keys and values",
+                                  "values by heads", "in turn"])
+def test_move_kept_in_caches_of_one_storage(form, dtype):
+    """Caches that lie between each other's rows are apart: each is moved as if it were alone."""
+    raw, k, v = _views(form, dtype)
+    before = [[t.view(torch.uint8).cpu()[None] if t.is_contiguous() else t.contiguous().view(torch.uint8).cpu()[None] for t in c]
+              for c in (k, v)]
+    table = torch.tensor(TABLE, dtype=I32)
+    fa.move_kept(k, v, table.to(DEV), _i32(CU), _i32(LENS), _i32(KEPT))
+    for c, old in zip((k, v), before):
+        for t, x in zip(c, old):
+            assert torch.equal(t.contiguous().view(torch.uint8).cpu()[None], _moved(x, table, CU, LENS, KEPT, PS))
+
+
+def test_move_kept_refuses_caches_that_share_storage():
+    """A cache that is named twice, in whatever form: refused, and nothing is moved."""
+    table = torch.tensor(TABLE, dtype=I32).to(DEV)
+    raw, k, v = _views("in turn", BF)
+    before = raw.clone()
+    whole = raw.view(BF).view(2 * LAYERS, PAGES, PS, HK, D)
+    for a, b in [([k[0], k[0]], v[:2]), (k[:2], [v[1], v[1]]), ([k[0], k[1], k[0]], [v[0], v[1], v[0]]), (k, k), (k[0], k[0]),
+                 (whole[:3], whole[2:5]), (whole[:3], whole[:3]), (whole[0], whole.view(-1, PS, HK, D)[2:7]),
+                 ([k[0]], [k[0].view(PAGES, HK, PS, D).transpose(1, 2)])]:
+        with pytest.raises(ValueError, match="share storage"):
+            fa.move_kept(a, b, table, _i32(CU), _i32(LENS), _i32(KEPT))
+    torch.cuda.synchronize()
+    assert torch.equal(raw, before)

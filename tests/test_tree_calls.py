@@ -1,0 +1,51 @@
+"""CPU tests of calls of the tree operators that cannot be taken: refused before any launch, at the C ABI and in Python."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from fftsparse_amd import _lib
+from tests.test_serving_host import _rc
+
+PAGE = 16 * 2 * 128 * 2                                    # bytes of a page of 16 tokens, 2 heads of 128, 16 bits
+SIZE = 8 * PAGE                                            # of a cache
+AT = 1 << 30
+
+
+def _move(k, v, **kw):
+    """A move in caches at the given addresses (lists: a sequence of layers; numbers: layers by a stride)."""
+    args = dict(block_table=16, t_sb=4, cu_lens=16, seq_lens=16, kept=16, layers=2, B=2, T=3, Hk=2, D=128, P=4, page_size=16,
+                elem_bytes=2, num_pages=8, k_sp=4096, k_ss=256, k_sh=128, v_sp=4096, v_ss=256, v_sh=128)
+    if isinstance(k, list):
+        arrays = [(ctypes.c_void_p * len(x))(*x) for x in (k, v)]
+        args.update(k_caches=arrays[0], v_caches=arrays[1], layers=len(k))
+    else:
+        args.update(k_cache=k, v_cache=v, k_sl=SIZE // 2, v_sl=SIZE // 2)
+    return _lib.CacheMoveArgs(**{**args, **kw})
+
+
+@pytest.mark.parametrize("k,v,kw", [
+    ([AT, AT], [AT + SIZE, AT + 2 * SIZE], {}),                                        # layers of one cache of keys
+    ([AT, AT + SIZE], [AT + 2 * SIZE, AT + 2 * SIZE], {}),                             # and of values
+    ([AT, AT + SIZE, AT], [AT + 2 * SIZE, AT + 3 * SIZE, AT + 2 * SIZE], {}),          # both, not side by side
+    ([AT], [AT], {}),                                                                  # keys and values in one
+    ([AT + SIZE, AT], [AT + 2 * SIZE, AT + SIZE], {}),
+    ([AT, AT + SIZE // 2], [AT + 2 * SIZE, AT + 3 * SIZE], {}),                        # caches that overlap by half
+    ([AT], [AT + 7 * PAGE], {}),                                                       # by a page
+    ([AT], [AT + SIZE - 256], {}),                                                     # by the last token's last head
+    ([AT], [AT + 256], {}),
+    ([AT], [AT + SIZE - 256], dict(v_ss=128, v_sh=16 * 128)),                          # of different layouts
+    ([AT + i * 100 * SIZE for i in range(70)] + [AT], [AT + (i * 100 + 1) * SIZE for i in range(71)], {}),   # two launches
+    (AT, AT, {}),
+    (AT, AT + SIZE, {}),                                                               # the values are the second layer's keys
+    (AT, AT + 2 * SIZE, dict(k_sl=0)),                                                 # layers by a stride that is none,
+    (AT, AT + 2 * SIZE, dict(v_sl=0)),
+    (AT, AT + 4 * SIZE, dict(k_sl=2048)),                                              # or too short
+    (AT, AT + 4 * SIZE, dict(v_sl=4096 * 7)),
+    (AT, AT + 256, dict(k_sp=8192, k_ss=512, k_sh=128, v_sp=8192, v_ss=512, v_sh=128, k_sl=SIZE, v_sl=SIZE)),
+])
+def test_caches_of_a_move_that_share_storage_are_refused(k, v, kw):
+    """Each cache is moved by workgroups of its own: one that is named twice would be moved twice."""
+    got, said = _rc("fs_cache_move", _move(k, v, **kw))
+    assert (got, "share storage" in said) == (-1, True), (got, said)
