@@ -19,7 +19,7 @@ import torch  # noqa: F401  (must precede the library load, see module docstring
 LIB_PATH = Path(os.environ.get("FFTSPARSE_AMD_LIB") or Path(__file__).resolve().with_name("libfftsparse_amd.so"))
 
 FS_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 
 class PoolArgs(ctypes.Structure):
@@ -164,7 +164,8 @@ class WindowAttnArgs(ctypes.Structure):
 
 class TreePlanArgs(ctypes.Structure):
     _fields_ = [("parents", c_void_p), ("cu_lens", c_void_p), ("seq_lens", c_void_p),
-                ("B", c_int), ("T", c_int), ("words", c_int), ("positions", c_void_p), ("mask", c_void_p)]
+                ("B", c_int), ("T", c_int), ("words", c_int), ("window", c_int), ("sinks", c_int),
+                ("positions", c_void_p), ("mask", c_void_p)]
 
 
 class TreeAcceptArgs(ctypes.Structure):

@@ -27,7 +27,7 @@ int launch_status(const char* what) {
 }  // namespace fs_host
 
 extern "C" const char* fs_last_error(void) { return fs_host::g_err; }
-extern "C" int fs_abi_version(void) { return 14; }
+extern "C" int fs_abi_version(void) { return 15; }
 
 extern "C" size_t fs_sizeof_args(int which) {
   switch (which) {

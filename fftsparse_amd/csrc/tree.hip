@@ -31,9 +31,24 @@ struct TreeRows {
 
 constexpr int kSteps = 16;                         // one by one
 
+// The k lowest of x's set bits (k below 1: none).
+__device__ __forceinline__ uint64_t low_bits(uint64_t x, int k) {
+  if (k >= (int)__popcll(x)) return x;
+  int at = 0;                                      // the place of the bit after them
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) {
+    const int c = (int)__popcll(x >> at & ((1ull << s) - 1));
+    at += c <= k ? s : 0;
+    k -= c <= k ? c : 0;
+  }
+  return x & ((1ull << at) - 1);
+}
+
 // rows[w][t]: word w of token t's mask.  After k rounds it holds t and its ancestors less than 16 2^k away, and up[t] is the one
 // 16 2^k away.  Ancestors come in falling order, so the steps write each word once.  In a round a row may take over one that
 // has grown in the same round already: what it gets beyond is ancestors as well.
+// A parent's number is below its child's, so a row's bits stand in the order of the positions: a window leaves the row's highest
+// bits, and the first tokens its lowest.
 __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_args a) {
   extern __shared__ uint64_t rows[];
   const int cap = 64 * a.words;                    // tokens of a tree
@@ -102,10 +117,22 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_ar
   }
   for (int t = tid; t < r.n; t += kTreeThreads) {
     int depth = -1;
-    for (int w = 0; w < a.words; ++w) {
-      const uint64_t x = t < most ? rows[w * cap + t] : 0;
-      a.mask[(int64_t)(r.c0 + t) * a.words + w] = (int64_t)x;
-      depth += __popcll(x);
+    if (a.window == 0) {
+      for (int w = 0; w < a.words; ++w) {
+        const uint64_t x = t < most ? rows[w * cap + t] : 0;
+        a.mask[(int64_t)(r.c0 + t) * a.words + w] = (int64_t)x;
+        depth += __popcll(x);
+      }
+    } else {
+      for (int w = 0; w < a.words; ++w) depth += t < most ? __popcll(rows[w * cap + t]) : 0;
+      int from = (int)min(max(a.sinks - first, (int64_t)0), (int64_t)kTreeMost);   // bits of the first tokens,
+      int to = max(depth + 1 - a.window, 0);       // and below the window
+      for (int w = 0; w < a.words; ++w) {
+        const uint64_t x = t < most ? rows[w * cap + t] : 0;
+        a.mask[(int64_t)(r.c0 + t) * a.words + w] = (int64_t)(x & ~(low_bits(x, to) & ~low_bits(x, from)));
+        from -= __popcll(x);
+        to -= __popcll(x);
+      }
     }
     a.positions[r.c0 + t] = t < most ? (int)(first + depth) : -1;
   }
@@ -378,6 +405,7 @@ extern "C" int fs_tree_plan(const fs_tree_plan_args* a, void* stream) {
   FS_CHECK_ARG(a != nullptr, "%s: null args", fn);
   if (int rc = check_tree(fn, a->B, a->T)) return rc;
   FS_CHECK_ARG(a->words >= 1, "%s: %d words", fn, a->words);
+  FS_CHECK_ARG(a->window >= 0 && a->sinks >= 0, "%s: window %d and sinks %d must not be negative", fn, a->window, a->sinks);
   FS_CHECK_SUPPORTED(a->words <= kTreeMost / 64, "%s: trees of %d tokens > %d", fn, 64 * a->words, kTreeMost);
   if (a->T == 0) return FS_OK;
   FS_CHECK_ARG(a->parents && a->cu_lens && a->seq_lens && a->positions && a->mask, "%s: null tensor pointer", fn);

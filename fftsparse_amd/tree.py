@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import CacheMoveArgs, TreeAcceptArgs, TreePlanArgs
-from .paged import _apart, _attend, _inference_only, _ints, _strides, _table, _written
+from .paged import _apart, _attend, _inference_only, _ints, _strides, _table, _window, _written
 
 MOST = 1024                    # tokens of a request's tree
 
@@ -60,7 +60,7 @@ class TreePlan:
 
 
 def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tensor, *, max_new: int,
-              out: TreePlan | None = None) -> TreePlan:
+              window: int | None = None, sinks: int = 0, out: TreePlan | None = None) -> TreePlan:
     """Positions of the new tokens of a batch of trees, and the masks that ``tree_attention`` reads (one launch).
 
     ``parents`` int32 [T]; ``cu_lens`` int32 [B + 1] and ``seq_lens`` int32 [B] as
@@ -68,12 +68,18 @@ def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tens
     the token it follows, and one; it sees its ancestors and itself.  A parent that is
     not an index below the token's own counts as none.  ``max_new``: at least the most
     new tokens that one request has, up to 1024; a request's tokens past it (rounded up to
-    64) get position -1 and an empty mask.  ``out``: a former result to write into, whose tensors are not this
-    call's inputs."""
+    64) get position -1 and an empty mask.
+
+    For attention under a ``window`` (and ``sinks``) give the same here: a token then sees
+    of its ancestors those less than ``window`` positions before it and those at the first
+    ``sinks`` positions, as if it had been decoded after them one by one.  Without it a token
+    sees all of its ancestors, which is the same for trees no deeper than the window.
+    ``out``: a former result to write into, whose tensors are not this call's inputs."""
     T = _tokens_by_row(parents, "parents")
     B = _rows_of(cu_lens)
     _ints(seq_lens, "seq_lens", (B,))
     words = -(-_most(max_new) // 64)
+    window, sinks = _window(window, sinks)
     dev = _lib.same_device(parents, cu_lens, seq_lens)
     if out is None:
         out = TreePlan(parents.new_empty(T), parents.new_empty((T, words), dtype=torch.int64))
@@ -84,7 +90,7 @@ def plan_tree(parents: torch.Tensor, cu_lens: torch.Tensor, seq_lens: torch.Tens
     if T:
         _lib.call("fs_tree_plan", TreePlanArgs(
             parents=parents.data_ptr(), cu_lens=cu_lens.data_ptr(), seq_lens=seq_lens.data_ptr(), B=B, T=T, words=words,
-            positions=out.positions.data_ptr(), mask=out.mask.data_ptr()), dev)
+            window=window, sinks=sinks, positions=out.positions.data_ptr(), mask=out.mask.data_ptr()), dev)
     return out
 
 
@@ -101,7 +107,8 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     other set; new tokens past the words are seen by none).  With ``window`` the
     tokens before the new ones are restricted to the last ``window`` up to the row's
     position (``positions`` int32 [T], taken within those of the request's new tokens) and the
-    first ``sinks``; among the new ones the mask alone decides.  A row that sees no
+    first ``sinks``; among the new ones the mask alone decides: form it with
+    ``plan_tree(..., window=, sinks=)`` of the same numbers where trees are deeper than the window.  A row that sees no
     token is 0.  Everything else as in ``paged_attention``, 8-bit caches too: the new
     tokens' keys and values are in the cache, all of them (a value that is not finite may
     reach rows of its request whose mask leaves it out)."""

@@ -503,7 +503,7 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * is set, itself included only so.  New tokens past the mask's words are seen by none.
  * With a window the tokens before the new ones are seen by the row's position
  * (positions[t], taken within those of the new tokens) as above, the new ones by the
- * mask alone.  All new tokens' keys and values are read. */
+ * mask alone (fs_tree_plan forms it under the same window).  All new tokens' keys and values are read. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   void* out; int64_t o_st, o_sh;
@@ -554,12 +554,13 @@ FS_API int fs_window_attn(const fs_window_attn_args* a, void* stream);
  * fs_tree_plan: positions[t] = seq_lens[b] - n + the number of t's ancestors, and bit
  * j of mask row t (words of 64) set for t itself and its ancestors.  Rows that no
  * request has, and a request's tokens from 64 words on, get position -1 and no bit.
- * words <= 16. */
+ * words <= 16.  window (0: none): ancestors `window` or more positions before t get no bit, if their position is not below
+ * `sinks`: the rule of a window by positions, as attention has it for the tokens before the new ones. */
 typedef struct {
   const int32_t* parents;                /* [T] */
   const int32_t* cu_lens;                /* [B + 1] */
   const int32_t* seq_lens;               /* [B], new tokens included */
-  int B, T, words;
+  int B, T, words, window, sinks;
   int32_t* positions;                    /* [T] */
   int64_t* mask;                         /* [T][words] */
 } fs_tree_plan_args;

@@ -17,8 +17,8 @@ def lines(parents):
     return out
 
 
-def plan(parents, cu, seq_lens, words):
-    """positions [T], mask [T][words] of unsigned 64-bit numbers."""
+def plan(parents, cu, seq_lens, words, window=None, sinks=0):
+    """positions [T], mask [T][words] of unsigned 64-bit numbers; under a window without the ancestors that it hides."""
     T = len(parents)
     pos, mask = [-1] * T, [[0] * words for _ in range(T)]
     for b, L in enumerate(seq_lens):
@@ -26,7 +26,11 @@ def plan(parents, cu, seq_lens, words):
         own = lines(parents[c0:c1])
         for t, line in enumerate(own[:64 * words]):
             pos[c0 + t] = L - (c1 - c0) + len(line) - 1
+            base = L - (c1 - c0)
             for j in line:
+                at = base + len(own[j]) - 1
+                if window and at <= pos[c0 + t] - window and at >= sinks:
+                    continue
                 mask[c0 + t][j // 64] |= 1 << (j % 64)
     return pos, mask
 

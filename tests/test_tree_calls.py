@@ -4,9 +4,12 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
+import fftsparse_amd as fa
 from fftsparse_amd import _lib
-from tests.test_serving_host import _rc
+from oracle import paged, tree
+from tests.test_serving_host import I32, _rc
 
 PAGE = 16 * 2 * 128 * 2                                    # bytes of a page of 16 tokens, 2 heads of 128, 16 bits
 SIZE = 8 * PAGE                                            # of a cache
@@ -49,3 +52,27 @@ def test_caches_of_a_move_that_share_storage_are_refused(k, v, kw):
     """Each cache is moved by workgroups of its own: one that is named twice would be moved twice."""
     got, said = _rc("fs_cache_move", _move(k, v, **kw))
     assert (got, "share storage" in said) == (-1, True), (got, said)
+
+
+def test_plan_tree_refuses_windows():
+    p, cu, lens = torch.zeros(6, dtype=I32), torch.zeros(4, dtype=I32), torch.zeros(3, dtype=I32)
+    for text, kw in [("on the GPU", dict(window=5, sinks=2)), ("on the GPU", dict(window=2 ** 31 - 1, sinks=2 ** 31 - 1)),
+                     ("window", dict(window=0)), ("window", dict(window=2 ** 31)), ("sinks", dict(window=5, sinks=-1))]:
+        with pytest.raises(ValueError, match=text):
+            fa.plan_tree(p, cu, lens, max_new=4, **kw)
+    args = _lib.TreePlanArgs(parents=16, cu_lens=16, seq_lens=16, B=2, T=3, words=1, positions=16, mask=16)
+    for change in (dict(window=-1), dict(window=1, sinks=-1)):
+        got, said = _rc("fs_tree_plan", args, **change)
+        assert (got, "must not be negative" in said) == (-1, True), said
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (3, 0), (3, 22), (5, 23), (4, 100), (8, 0), (25, 2), (None, 0)])
+def test_the_oracle_of_a_chain_is_that_of_paged_attention_under_any_window(window, sinks):
+    """Windows shorter than the chain too: the new tokens that it hides are hidden."""
+    g = torch.Generator().manual_seed(0)
+    q, k, v = torch.randn(9, 4, 16, generator=g), *(torch.randn(30, 2, 16, generator=g) for _ in range(2))
+    pos, mask = tree.plan([-1, *range(8)], [0, 9], [30], 1, window, sinks)
+    sees = torch.tensor([[m[0] >> j & 1 for j in range(9)] for m in mask], dtype=torch.bool)
+    a = tree.attend(q, k, v, 9, sees, window, sinks, pos=pos)[0]
+    b = paged.attend(q, k, v, 21, window, sinks)[0]
+    assert torch.allclose(a, b, atol=1e-12)
