@@ -134,15 +134,21 @@ def _scales(k_scale, v_scale, dtype, Hk: int) -> bool:
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
-    p = t.data_ptr()
-    return p, p + t.numel() * t.element_size()
+    """From a tensor's first byte to behind its last one."""
+    p, n = t.data_ptr(), t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum((m - 1) * s for m, s in zip(t.shape, t.stride()))
+    return p, p + n * t.element_size()
 
 
 def _apart(outs, ins, what: str) -> None:
-    """Refuses outputs that share storage with what is read while they are written."""
-    read = [_span(x) for x in ins]
-    if any(lo < end and start < hi for lo, hi in map(_span, outs) for start, end in read):
+    """Refuses outputs that share storage with each other, or with what is read while they are written."""
+    read, written = [_span(x) for x in ins], [_span(x) for x in outs]
+    if any(lo < end and start < hi for lo, hi in written for start, end in read):
         raise ValueError(f"out shares storage with an input: {what}")
+    written.sort()
+    if any(hi > start for (_, hi), (start, _) in zip(written, written[1:])):
+        raise ValueError("out's tensors share storage with each other")
 
 
 @dataclass
@@ -301,6 +307,8 @@ def _attend(name, q, k_cache, v_cache, block_table, cu_lens, seq_lens, mask, pos
     else:
         os_ = _written(out, "out", (T, Hq, D), q.dtype)
         dev = _lib.same_device(q, k_cache, v_cache, t, cu_lens, seq_lens, out, *more)
+        if more:
+            _apart((out,), more, "masks, positions and scales are read until the last row is written")
     if T == 0:
         return out
     args = PagedAttnArgs(

@@ -9,7 +9,8 @@ import torch
 import fftsparse_amd as fa
 from fftsparse_amd import _lib
 from oracle import paged, tree
-from tests.test_serving_host import I32, _rc
+from tests.test_serving_host import BF, I32, _paged, _rc
+from tests.test_tree_host import _eight
 
 PAGE = 16 * 2 * 128 * 2                                    # bytes of a page of 16 tokens, 2 heads of 128, 16 bits
 SIZE = 8 * PAGE                                            # of a cache
@@ -76,3 +77,41 @@ def test_the_oracle_of_a_chain_is_that_of_paged_attention_under_any_window(windo
     a = tree.attend(q, k, v, 9, sees, window, sinks, pos=pos)[0]
     b = paged.attend(q, k, v, 21, window, sinks)[0]
     assert torch.allclose(a, b, atol=1e-12)
+
+
+def test_outputs_that_share_storage_are_refused(monkeypatch):
+    """With each other, or with what the kernels still read when they are written (the check that these tensors are on a GPU is
+    left out, so that the next one is reached; nothing is launched)."""
+    monkeypatch.setattr(_lib, "same_device", lambda *tensors: tensors[0].device)
+    monkeypatch.setattr(_lib, "call", lambda name, *rest: pytest.fail(f"{name} was launched"))
+    p, cu, lens, x = torch.zeros(6, dtype=I32), torch.zeros(4, dtype=I32), torch.zeros(3, dtype=I32), torch.zeros(6, dtype=torch.int64)
+    buf = torch.zeros(64, dtype=torch.int64)
+    half = buf.view(I32)
+    for out, text in [(fa.TreePlan(half[5:11], buf[:6].view(6, 1)), "each other"), (fa.TreePlan(half[:6], buf[:6].view(6, 1)), "each other"),
+                      (fa.TreePlan(p, buf[:6].view(6, 1)), "an input")]:
+        with pytest.raises(ValueError, match=text):
+            fa.plan_tree(p, cu, lens, max_new=4, out=out)
+    small = torch.zeros(3, dtype=I32)
+    for out, text in [(fa.Accepted(half[:6], small, small, buf[20:23]), "each other"),
+                      (fa.Accepted(half[:6], half[5:8], small, buf[20:23]), "each other"),
+                      (fa.Accepted(half[:6], small, half[42:45], buf[20:23]), "each other"),
+                      (fa.Accepted(half[:6], small, half[8:11], x[:3]), "an input")]:
+        with pytest.raises(ValueError, match=text):
+            fa.accept_tree(p, x, x.clone(), cu, max_new=4, out=out)
+    a = _paged()
+    rows = torch.zeros(4096 + 6 * 2048, dtype=torch.uint8)                  # out's rows in 8 bytes of each 2048
+    out = rows.view(BF)[:6 * 1024].view(6, 1024)[:, :512].view(6, 4, 128)
+    inside = rows[1024:1024 + 48].view(torch.int64).view(6, 1)              # behind a row, within the tensor's span
+    for kw in [dict(mask=torch.zeros(6 * 128, dtype=torch.int64)), dict(mask=inside),
+               dict(mask=torch.zeros(6, 1, dtype=torch.int64), window=3, positions=rows[2048:2048 + 24].view(I32))]:
+        if kw["mask"].dim() == 1:
+            whole = kw["mask"]
+            kw["mask"], o = whole[:6].view(6, 1), whole.view(BF)[:6 * 512].view(6, 4, 128)
+        else:
+            o = out
+        with pytest.raises(ValueError, match="an input"):
+            fa.tree_attention(**a, **kw, out=o)
+    e = _eight()
+    scale = torch.zeros(6 * 256)
+    with pytest.raises(ValueError, match="an input"):
+        fa.paged_attention(**{**e, "k_scale": scale[:2]}, out=scale.view(BF)[:6 * 512].view(6, 4, 128))
