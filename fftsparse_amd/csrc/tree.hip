@@ -29,6 +29,14 @@ struct TreeRows {
   }
 };
 
+// f of the rows behind the last request's, and before the first one's (a batch's later requests taken alone).
+template <typename F>
+__device__ __forceinline__ void rows_of_none(const int32_t* cu, int B, int T, F f) {
+  const int c0 = min(max(cu[0], 0), T), c1 = min(max(cu[B], 0), T);
+  for (int t = threadIdx.x; t < c0; t += kTreeThreads) f(t);
+  for (int t = max(c0, c1) + (int)threadIdx.x; t < T; t += kTreeThreads) f(t);
+}
+
 constexpr int kSteps = 16;                         // one by one
 
 // The k lowest of x's set bits (k below 1: none).
@@ -55,10 +63,10 @@ __global__ __launch_bounds__(kTreeThreads) void tree_plan_kernel(fs_tree_plan_ar
   int* par = reinterpret_cast<int*>(rows + (size_t)a.words * cap);
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {                                  // rows that no request has
-    for (int t = min(max(a.cu_lens[a.B], 0), a.T) + tid; t < a.T; t += kTreeThreads) {
+    rows_of_none(a.cu_lens, a.B, a.T, [&](int t) {
       a.positions[t] = -1;
       for (int w = 0; w < a.words; ++w) a.mask[(int64_t)t * a.words + w] = 0;
-    }
+    });
     return;
   }
   const TreeRows r(a.cu_lens, b, a.T);
@@ -149,7 +157,7 @@ __global__ __launch_bounds__(kTreeThreads) void tree_accept_kernel(fs_tree_accep
   __shared__ int marks[PER][NW], path[kSteps], steps, last;
   const int tid = threadIdx.x, b = blockIdx.x;
   if (b == a.B) {
-    for (int t = min(max(a.cu_lens[a.B], 0), a.T) + tid; t < a.T; t += kTreeThreads) a.kept[t] = -1;
+    rows_of_none(a.cu_lens, a.B, a.T, [&](int t) { a.kept[t] = -1; });
     return;
   }
   const I *tokens = static_cast<const I*>(a.tokens), *chosen = static_cast<const I*>(a.chosen);

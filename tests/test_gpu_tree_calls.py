@@ -5,7 +5,8 @@ import pytest
 import torch
 
 import fftsparse_amd as fa
-from tests.test_gpu_tree import BF, DEV, E4M3, I32, _i32, _moved
+from oracle import tree as ref
+from tests.test_gpu_tree import BF, DEV, E4M3, I32, Batch, _i32, _moved
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +65,30 @@ def test_move_kept_refuses_caches_that_share_storage():
             fa.move_kept(a, b, table, _i32(CU), _i32(LENS), _i32(KEPT))
     torch.cuda.synchronize()
     assert torch.equal(raw, before)
+
+
+@pytest.mark.parametrize("first,last", [(0, 6), (2, 6), (3, 5), (5, 6), (0, 1)])
+def test_requests_of_the_middle_of_a_batch(first, last):
+    """Row numbers that begin behind the first rows and end before the last ones: rows of no request have position -1, no bit
+    and nothing kept, and attention leaves them as they were."""
+    b = Batch([(5, 8), (62, 3), (0, 70), (64, 1), (99, 8), (30, 4)], kind="random", seed=3)
+    parents = [p for t in b.trees for p in t]
+    cu, lens = _i32(b.cu)[first:last + 1], _i32(b.total)[first:last]
+    rows = slice(b.cu[first], b.cu[last])
+    out = fa.TreePlan(torch.full((b.T,), 7, dtype=I32, device=DEV), torch.full((b.T, 2), 7, dtype=torch.int64, device=DEV))
+    fa.plan_tree(_i32(parents), cu, lens, max_new=70, out=out)
+    pos, mask = [-1] * b.T, torch.zeros(b.T, 2, dtype=torch.int64)
+    pos[rows], mask[rows] = b.pos[rows], b.mask[rows]
+    assert out.positions.tolist() == pos and torch.equal(out.mask.cpu(), mask)
+    tokens = torch.ones(b.T, dtype=I32, device=DEV)
+    want = ref.accept(parents, [1] * b.T, [1] * b.T, b.cu, 70)
+    acc = fa.Accepted(torch.full((b.T,), 7, dtype=I32, device=DEV), *(torch.full((last - first,), 7, dtype=I32, device=DEV) for _ in range(3)))
+    fa.accept_tree(_i32(parents), tokens, tokens, cu, max_new=70, out=acc)
+    kept = [-1] * b.T
+    kept[rows] = want[0][rows]
+    assert acc.kept.tolist() == kept and acc.kept_lens.tolist() == want[1][first:last]
+    got = torch.full(b.q.shape, 7.0, dtype=BF, device=DEV)
+    fa.tree_attention(b.q.to(DEV), *b.dev_caches(), b.table.to(DEV)[first:last], cu, lens, out.mask, out=got)
+    assert bool((got[:rows.start] == 7.0).all()) and bool((got[rows.stop:] == 7.0).all())
+    got[:rows.start], got[rows.stop:] = (b.gpu()[x] for x in (slice(0, rows.start), slice(rows.stop, None)))
+    b.check(got)
