@@ -10,7 +10,8 @@
 //
 // Into a cache in 8 bits (e4m3, a scale for each KV head) goes the rotated key, and the value, over
 // the scale, held to the largest e4m3 number and rounded once, to nearest even; a
-// nan stays one.  It is not rounded to the input type on the way.
+// nan stays one.  It is not rounded to the input type on the way.  Scales are 2^-126 to 2^126, whose reciprocals are normal
+// numbers; the quotient is a product with one, off by up to 2^-22, so one that near a middle may go to either side.
 //
 // One pass over q, k and v.  A workgroup takes a few tokens: their angles, one
 // per (token, pair), go to LDS once and serve every head; then each thread moves

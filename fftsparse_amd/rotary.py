@@ -133,7 +133,9 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     was, in the cache too.
 
     Caches of ``torch.float8_e4m3fn`` need ``k_scale`` and ``v_scale`` (float32 [Hk], 2^-126 to 2^126): x / scale[h] is
-    written, held to -448 .. 448 and rounded once, from 32 bits (nan stays nan)."""
+    written, held to -448 .. 448 and rounded once, from 32 bits (nan stays nan); the quotient there, a product with the
+    scale's reciprocal, is off by up to 2^-22 of itself.  f16 queries are then rounded from 32 bits too, and may differ from
+    ``rope``'s in the last place."""
     q, qs, k, ks, inv_freq = _common("rope_cache", q, k, positions, inv_freq)
     v, vs = _rows(v, "v")
     if v.shape != k.shape or v.dtype != k.dtype:

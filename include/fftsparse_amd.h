@@ -444,8 +444,9 @@ FS_API int fs_plan(const fs_plan_args* a, void* stream);
  * part allow them (single elements otherwise).
  * k_scale and v_scale (both, with slots): the caches are in e4m3, and the rotated
  * key and the value of KV head h are written as x / scale[h], held to -448 .. 448
- * and rounded once from 32 bits to nearest even (nan stays nan).  Scales are
- * positive, finite and not subnormal; cache strides multiples of 16 elements. */
+ * and rounded once from 32 bits to nearest even (nan stays nan); the quotient in 32
+ * bits, a product with the scale's reciprocal, is off by up to 2^-22 of itself.  Scales are
+ * 2^-126 to 2^126; cache strides multiples of 16 elements. */
 typedef struct {
   const void* q; int64_t q_st, q_sh;
   const void* k; int64_t k_st, k_sh;
@@ -494,7 +495,7 @@ FS_API int fs_rope(const fs_rope_args* a, void* stream);
  * 68 MB (D = 64: 35) and T * Hq / 4 bytes.  Calls that overlap on one workspace
  * race.
  * k_scale and v_scale (both): the caches are in e4m3, and a number x of KV head h
- * stands for x * scale[h] (positive and finite); cache strides are multiples of 16
+ * stands for x * scale[h] (positive and finite, values up to 2^93); cache strides are multiples of 16
  * elements.  Scores are of q in dtype and the e4m3 numbers, exact in dtype.  The
  * workspace is about 17 MB where it is 9 above.
  * mask: the rows of a request are not a chain but a tree, or any other set.  The row

@@ -92,3 +92,29 @@ def test_requests_of_the_middle_of_a_batch(first, last):
     assert bool((got[:rows.start] == 7.0).all()) and bool((got[rows.stop:] == 7.0).all())
     got[:rows.start], got[rows.stop:] = (b.gpu()[x] for x in (slice(0, rows.start), slice(rows.stop, None)))
     b.check(got)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 1.5 * 2.0 ** -126, 2.0 ** -60, 2.0 ** 60, 1.75 * 2.0 ** 125, 2.0 ** 126])
+def test_scales_at_the_ends_of_their_range(scale):
+    """x / scale in e4m3, exact where the scale is a power of two, else within half a step and the quotient's 2^-22; attention
+    reads the numbers times the scale (results below 2^-126 in steps of 2^-133)."""
+    T, D = 20, 64
+    g = torch.Generator().manual_seed(6)
+    v = (torch.randn(T, 1, D, generator=g).double() * 1.9 * scale).float().clamp(-3e38, 3e38)
+    kc, vc = (torch.zeros(2, 16, 1, D, dtype=torch.uint8, device=DEV).view(E4M3) for _ in range(2))
+    one, s = torch.ones(1, device=DEV), torch.tensor([scale], device=DEV)
+    pos, zero = torch.arange(T, dtype=I32, device=DEV), torch.zeros(T, 1, D, device=DEV)
+    fa.rope_cache(zero, zero, v.to(DEV), pos, pos.long(), kc, vc, torch.ones(32, dtype=torch.float64, device=DEV),
+                  k_scale=one, v_scale=s)
+    y, got = v[:, 0].double() / scale, vc.view(32, D)[:T].cpu().float().double()
+    assert bool(((got - y).abs() <= ref.e4m3_half_step(y) + y.abs() * 2.0 ** -22).all())
+    if scale == 2.0 ** torch.tensor(scale).log2().round().item():
+        assert torch.equal(got, y.float().to(E4M3).double())
+    if scale > 2.0 ** 84:                                  # attention takes values up to 2^93
+        return
+    # every key alike: the mean of the values up to each token, in 32 bits but for the weights and the result (bf16)
+    q = torch.ones(T, 1, D, dtype=BF, device=DEV)
+    out = fa.paged_attention(q, kc, vc, _i32([[0, 1]]), _i32([0, T]), _i32([T]), k_scale=one, v_scale=s).double().cpu()[:, 0]
+    want = (got.cumsum(0) / torch.arange(1, T + 1)[:, None]) * scale
+    mag = (got.abs().cumsum(0) / torch.arange(1, T + 1)[:, None]) * scale
+    assert bool(((out - want).abs() <= 3 * 2.0 ** -8 * mag + 2.0 ** -133).all())
