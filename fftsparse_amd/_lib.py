@@ -252,12 +252,12 @@ def same_device(*tensors) -> torch.device:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError(f"tensors must be on the GPU, got one on {t.device}")
-        if first is None:
+        if t.get_device() != index:                        # -1: on the host
+            if not t.is_cuda:
+                raise ValueError(f"tensors must be on the GPU, got one on {t.device}")
+            if first is not None:
+                raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
             first, index = t, t.get_device()
-        elif t.get_device() != index:
-            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
     if first is None:
         raise ValueError("no tensor given")
     return first.device

@@ -52,17 +52,13 @@ def _strides(t: torch.Tensor):
     return [s if n > 1 else 0 for n, s in zip(shape, st)] if 1 in shape else st
 
 
-def _aligned(t: torch.Tensor, st) -> bool:
-    """Whether the kernels can read t as it is: d contiguous, 16-byte rows (for elements of 4 bytes: 32)."""
-    if st[-1] != 1:
-        return False
-    if t.dtype == E4M3:
-        bits, m = t.data_ptr(), 15
-    else:
-        bits, m = t.data_ptr() >> 1, 7
+def _aligned(t: torch.Tensor, st, eight: bool = False) -> bool:
+    """Whether the kernels can read t as it is: d contiguous, 16-byte rows (for elements of 4 bytes: 32); eight: elements of
+    one byte."""
+    bits = (t.data_ptr() if eight else t.data_ptr() >> 1) if st[-1] == 1 else 1
     for s in st[:-1]:
         bits |= s
-    return not bits & m
+    return not bits & (15 if eight else 7)
 
 
 def _rows(t: torch.Tensor, name: str):
@@ -81,9 +77,9 @@ def _written(t: torch.Tensor, name: str, shape, dtype):
     if t.shape != shape or t.dtype != dtype:
         raise ValueError(f"{name} must be a {list(shape)} {dtype} tensor, got {t.dtype} {tuple(t.shape)}")
     st = _strides(t)
-    if not _aligned(t, st) or (0 in st and any(n > 1 and s == 0 for n, s in zip(shape, st))):
+    if not _aligned(t, st, dtype is E4M3) or (0 in st and any(n > 1 and s == 0 for n, s in zip(shape, st))):
         if t.numel():
-            raise ValueError(f"{name} must have d contiguous, strides that are multiples of {16 if dtype == E4M3 else 8} "
+            raise ValueError(f"{name} must have d contiguous, strides that are multiples of {16 if dtype is E4M3 else 8} "
                              f"elements and 16-byte alignment, and no broadcast dimension, got strides {t.stride()}")
     return st
 
@@ -97,10 +93,11 @@ def _ints(t: torch.Tensor, name: str, shape, dtypes=(torch.int32,)) -> torch.Ten
 
 def _table(t: torch.Tensor):
     """[B, P] block table -> B, P, row stride."""
-    if t.dim() != 2 or t.dtype != torch.int32 or not t.numel() or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape = t.shape
+    if len(shape) != 2 or t.dtype != torch.int32 or 0 in shape or (shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"block_table must be an int32 [requests, pages] tensor with contiguous rows, got {t.dtype} "
-                         f"{tuple(t.shape)}")
-    B, P = t.shape
+                         f"{tuple(shape)}")
+    B, P = shape
     if B > 1 and t.stride(0) < P:
         raise ValueError("block_table's rows overlap")
     return B, P, t.stride(0) if B > 1 else P
@@ -118,19 +115,16 @@ def _caches(k: torch.Tensor, v: torch.Tensor, dtype, Hk=None, D=None):
     return want, ks, _written(v, "v_cache", want, dtype)
 
 
-def _scales(k_scale, v_scale, dtype, Hk: int) -> bool:
-    """Whether scales come with caches of a type (as they must in 8 bits, and only then)."""
-    if dtype != E4M3:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError(f"k_scale and v_scale go with caches of {E4M3}, got {dtype}")
-        return False
+def _scales(k_scale, v_scale, dtype, Hk: int) -> None:
+    """Scales come with caches in 8 bits, and only then."""
+    if dtype is not E4M3:
+        raise ValueError(f"k_scale and v_scale go with caches of {E4M3}, got {dtype}")
     if k_scale is None or v_scale is None:
         raise ValueError(f"caches of {E4M3} need k_scale and v_scale")
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
         if t.shape != (Hk,) or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous float32 tensor of {Hk} scales, one for each KV head, got "
                              f"{t.dtype} {tuple(t.shape)}")
-    return True
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -232,10 +226,8 @@ def _scale(scale, D: int) -> float:
     return scale
 
 
-def _attn_dtype(q, k, v, cached: bool = False) -> None:
+def _attn_dtype(q, k, v) -> None:
     dt = q.dtype
-    if cached and k.dtype == v.dtype == E4M3 and (dt == torch.bfloat16 or dt == torch.float16):
-        return
     if (dt != torch.bfloat16 and dt != torch.float16) or k.dtype != dt or v.dtype != dt:
         raise TypeError(f"expected bf16 or f16 tensors of one type, got {[t.dtype for t in (q, k, v)]}")
 
@@ -277,9 +269,13 @@ def _attend(name, q, k_cache, v_cache, block_table, cu_lens, seq_lens, mask, pos
     """``paged_attention``, and ``tree_attention`` (mask given)."""
     q, qs = _rows(q, "q")
     T, Hq, D = q.shape
-    _attn_dtype(q, k_cache, v_cache, True)
-    (pages, ps, Hk, _), ks, vs = _caches(k_cache, v_cache, k_cache.dtype, D=D)
-    scaled = _scales(k_scale, v_scale, k_cache.dtype, Hk)
+    dt = k_cache.dtype
+    if dt is not E4M3 or v_cache.dtype is not E4M3 or q.dtype not in (torch.bfloat16, torch.float16):
+        _attn_dtype(q, k_cache, v_cache)
+    (pages, ps, Hk, _), ks, vs = _caches(k_cache, v_cache, dt, D=D)
+    scaled = dt is E4M3 or k_scale is not None or v_scale is not None
+    if scaled:
+        _scales(k_scale, v_scale, dt, Hk)
     if Hk == 0 or Hq % Hk or Hq == 0:
         raise ValueError(f"query heads {Hq} must be a multiple of key heads {Hk}")
     t = block_table

@@ -141,18 +141,22 @@ def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: tor
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"value {v.dtype} {tuple(v.shape)} must be like key {k.dtype} {tuple(k.shape)}")
     _ints(slots, "slots", (q.shape[0],), (torch.int64,))
-    shape, kc, vc = _caches(k_cache, v_cache, E4M3 if k_cache.dtype == E4M3 else q.dtype, k.shape[1], k.shape[2])
-    scaled = _scales(k_scale, v_scale, k_cache.dtype, k.shape[1])
-    _inference_only("rope_cache", v, k_cache, v_cache, *((k_scale, v_scale) if scaled else ()))
+    dt = k_cache.dtype
+    shape, kc, vc = _caches(k_cache, v_cache, dt if dt is E4M3 else q.dtype, k.shape[1], k.shape[2])
+    scales = ()
+    if dt is E4M3 or k_scale is not None or v_scale is not None:
+        _scales(k_scale, v_scale, dt, k.shape[1])
+        scales = k_scale, v_scale
+    _inference_only("rope_cache", v, k_cache, v_cache, *scales)
     q_out, os_ = _out(q_out, "q_out", q)
-    dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out, k_scale, v_scale)
+    dev = _lib.same_device(q, k, v, positions, slots, k_cache, v_cache, inv_freq, q_out, *scales)
     if q.shape[0]:
         a = _args(q, qs, k, ks, q_out, os_, positions, inv_freq, attention_factor, interleaved)
         a.v, a.v_st, a.v_sh, a.slots = v.data_ptr(), vs[0], vs[1], slots.data_ptr()
         a.k_cache, a.kc_sp, a.kc_ss, a.kc_sh = k_cache.data_ptr(), kc[0], kc[1], kc[2]
         a.v_cache, a.vc_sp, a.vc_ss, a.vc_sh = v_cache.data_ptr(), vc[0], vc[1], vc[2]
         a.num_pages, a.page_size = shape[0], shape[1]
-        if scaled:
+        if scales:
             a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
         _lib.call("fs_rope", a, dev)
     return q_out
