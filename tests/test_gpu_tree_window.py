@@ -11,7 +11,7 @@ import torch
 
 import fftsparse_amd as fa
 from oracle import paged, tree as ref
-from tests.test_gpu_tree import BF, DEV, F16, I32, SMALL, WIDE, Batch, _cu, _i32, _tree, _words
+from tests.test_gpu_tree import BF, DEV, F16, I32, SMALL, WIDE, Batch, Model, _cu, _i32, _tree, _words
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +124,61 @@ def test_a_captured_plan_under_a_window_replays():
         pos, mask = ref.plan(tree, cu.tolist(), lens.tolist(), 3, 9, 4)
         assert out.positions.tolist() == eager.positions.tolist() == pos
         assert torch.equal(out.mask, eager.mask) and torch.equal(out.mask.cpu(), _words(mask))
+
+
+@pytest.mark.parametrize("window,sinks", [(4, 0), (5, 2)])
+def test_drafts_under_a_short_window_equal_token_by_token(window, sinks):
+    """A serving loop whose trees are deeper than the window: the kept tokens and their outputs are those of decoding one token
+    after the other.  |v| is up to 5; both outputs are within the tolerance above."""
+    B, N, Hq, Hk, D, ps, steps = 3, 12, 4, 2, 64, 16, 6
+    m, inv = Model(97, Hq, Hk, D, 3), fa.rope_frequencies(D, device=DEV)[0]
+
+    def fresh():
+        kc, vc = (torch.zeros(32, ps, Hk, D, dtype=BF, device=DEV) for _ in range(2))
+        return dict(kc=kc, vc=vc, table=torch.zeros(B, 8, dtype=I32, device=DEV), lens=torch.zeros(B, dtype=I32, device=DEV),
+                    free=torch.arange(32, dtype=I32, device=DEV), count=_i32([32]))
+
+    first, a = torch.tensor([3, 50, 11], device=DEV), fresh()
+    tokens, line, outs = first, [[] for _ in range(B)], [[] for _ in range(B)]
+    for _ in range(N * steps):
+        plan = fa.plan_step(a["table"], a["lens"], _i32([1] * B), a["free"], a["count"], page_size=ps, num_tokens=B)
+        q = fa.rope_cache(m.q[tokens], m.k[tokens], m.v[tokens], plan.positions, plan.slots, a["kc"], a["vc"], inv)
+        o = fa.paged_attention(q, a["kc"], a["vc"], a["table"], plan.cu_lens, plan.seq_lens, max_new=1, window=window, sinks=sinks)
+        for b, t in enumerate(tokens.tolist()):
+            line[b].append(t)
+            outs[b].append(o[b])
+        tokens = m.next(tokens, plan.positions)
+        a["lens"], a["count"] = plan.seq_lens, plan.free_count
+    s, at, deepest = fresh(), [0] * B, 0
+    g = torch.Generator().manual_seed(9)
+    for _ in range(steps):
+        parents, toks = [], []
+        for b in range(B):                                 # the right line as far as a chance goes, wrong tokens beside it
+            p, right = [-1], [0]
+            for t in range(1, N):
+                p.append(right[-1] if torch.rand((), generator=g) < 0.85 else int(torch.randint(0, t, (), generator=g)))
+                good = p[t] == right[-1] and torch.rand((), generator=g) < 0.95
+                right += [t] if good else []
+            depth = [len(x) - 1 for x in ref.lines(p)]
+            toks += [line[b][at[b] + depth[t]] if t in right else 96 - line[b][at[b] + depth[t]] for t in range(N)]
+            parents += p
+        par, tokens = _i32(parents), torch.tensor(toks, device=DEV)
+        plan = fa.plan_step(s["table"], s["lens"], _i32([N] * B), s["free"], s["count"], page_size=ps, num_tokens=B * N)
+        tree = fa.plan_tree(par, plan.cu_lens, plan.seq_lens, max_new=N, window=window, sinks=sinks)
+        q = fa.rope_cache(m.q[tokens], m.k[tokens], m.v[tokens], tree.positions, plan.slots, s["kc"], s["vc"], inv)
+        o = fa.tree_attention(q, s["kc"], s["vc"], s["table"], plan.cu_lens, plan.seq_lens, tree.mask, positions=tree.positions,
+                              max_new=N, window=window, sinks=sinks)
+        acc = fa.accept_tree(par, tokens, m.next(tokens, tree.positions), plan.cu_lens, max_new=N)
+        fa.move_kept(s["kc"], s["vc"], s["table"], plan.cu_lens, plan.seq_lens, acc.kept)
+        back = fa.plan_step(s["table"], plan.seq_lens, acc.dropped, s["free"], plan.free_count, page_size=ps, num_tokens=0)
+        s["lens"], s["count"] = back.seq_lens, back.free_count
+        kept, lens = acc.kept.tolist(), acc.kept_lens.tolist()
+        for b in range(B):
+            for i, t in enumerate(kept[b * N:b * N + lens[b]]):
+                assert toks[b * N + t] == line[b][at[b] + i]
+                err = (o[b * N + t].double() - outs[b][at[b] + i].double()).abs().max().item()
+                assert err <= 2 * (3 * torch.finfo(BF).eps / 2 + 2e-4) * 5.0, (b, i, err)
+            at[b] += lens[b]
+            deepest = max(deepest, lens[b])
+            assert int(acc.next_tokens[b]) == line[b][at[b]]
+    assert s["lens"].tolist() == at and deepest > window
