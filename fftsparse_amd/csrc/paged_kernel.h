@@ -968,21 +968,22 @@ __global__ __launch_bounds__(kJoinThreads) void combine_kernel(PagedKArgs a) {
       const int64_t s = slot_of(j0);
       turn(a.part_ml[s * 64 + r], a.part_ml[s * 64 + 32 + r], sums(s));
     }
-  }
-  for (; j0 < np; j0 += AHEAD * J) {
-    float mj[AHEAD], lj[AHEAD];
-    float4 xj[AHEAD];
+  } else {
+    for (; j0 < np; j0 += AHEAD * J) {
+      float mj[AHEAD], lj[AHEAD];
+      float4 xj[AHEAD];
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      const int64_t s = slot_of(min(j0 + k * J, np - 1));
-      mj[k] = a.part_ml[s * 64 + r];
-      lj[k] = a.part_ml[s * 64 + 32 + r];
-      xj[k] = sums(s);
-    }
+      for (int k = 0; k < AHEAD; ++k) {
+        const int64_t s = slot_of(min(j0 + k * J, np - 1));
+        mj[k] = a.part_ml[s * 64 + r];
+        lj[k] = a.part_ml[s * 64 + 32 + r];
+        xj[k] = sums(s);
+      }
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (j0 + k * J >= np) break;
-      turn(mj[k], lj[k], xj[k]);
+      for (int k = 0; k < AHEAD; ++k) {
+        if (j0 + k * J >= np) break;
+        turn(mj[k], lj[k], xj[k]);
+      }
     }
   }
   if (J > 1) {
@@ -1200,9 +1201,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       } else {
         // From e4m3 an operand takes four conversions (128 of the step's 296 VALU instructions at D = 128), so as many go
         // before the first MFMA, and after each the next operand's and one more (of S) or two (of P V) of the softmax's; a read of
-        // keys serves two MFMAs.  In the order above, which has no place for them, 2048 tokens over 30000 took 1047 us and not 929 (D =
-        // 64, 28 / 4 heads: 673 and 602); with 4 or 6 in place of 5 1020 to 1054, with 5, 7, 9 in place of the second 6 1 to 3%
-        // more, with 3 or 8 before the first 13% and 4%.  Trees at D = 64 stay with it: 16 of 64 over 8192 112 us and not 123.
+        // keys serves two MFMAs.  The order above has no place for them.  Whole calls in a graph, its and this one's: 2048 of 30000
+        // tokens 1034 and 912 us (D = 128, 32 / 8 heads; f16 1057, 943), 669 and 602 (D = 64, 28 / 4, f16; bf16 636, 632); 16
+        // requests of 8192 with 64 new tokens 189 and 163, 114 and 107 (bf16 111, 109); trees at D = 128 the same or 2% less.
+        // With 4 and 4 or 6 and 6 in place of 5 and 6 6 and 7% more, with 5, 7, 9 for the second 1 to 3%, with 3 or 8 before the
+        // first 16% and 6%.  Trees at D = 64 stay with the order above: in this one the compiler puts 20 s_nop into their step,
+        // between conversions and the MFMAs that read them, where chains have 5 (16 trees of 64 over 8192 113 us and not 124, 4 of 250
+        // over 4000 76 and 81, 40 under a window 38 and 40; bf16 117 and 124, 78 and 81, 38 and 40).
         __builtin_amdgcn_sched_group_barrier(0x100, LA / 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
 #pragma unroll
