@@ -36,7 +36,7 @@
 // Rounding: scores, maxima, sums and O are in 32 bits; P is rounded to the input type for the
 // second product (its relative error, at most half a step of the type, averages out over the keys as the
 // values' own does), and the row sum adds the rounded P, so that weights add up to one.  Against 64 bits (2-norm)
-// bf16 is off by 1.8e-3 to 2.0e-3 (1.6e-3 to 1.7e-3 with P in 32 bits: the result's own rounding), f16 by 2.2e-4 to 2.8e-4
+// bf16 is off by 1.6e-3 to 2.1e-3 (1.5e-3 to 1.7e-3 with P in 32 bits: the result's own rounding), f16 by 2.2e-4 to 2.8e-4
 // (2.1e-4).  Sums stay below 2^34 of the largest |v| (P up to 2^8, 2^26 keys), so |v| up to 2^93 is safe.
 //
 // Groups of 16 keys are never split by a page (its size is a multiple of 16): a
@@ -48,9 +48,10 @@
 // 8-bit pages (k8): tiles stay e4m3 in LDS, half as large, and operands are widened to the input type, which holds every e4m3
 // number, as they are read (the transposing read of V by bytes).  A key's scale goes into the scores' factor, a value's
 // into the sums at the end.  Two workgroups of few_kernel share a CU, so that as many bytes are on their way as in 16 bits.  Measured
-// (bf16, D = 128, 32 / 8 heads): 64 requests of 64 - 8192 tokens 62 us (103 in 16 bits), 64 of 4096 119 to 124 us, 4.3 to 4.5 TB/s
-// (112 us, 4.8 TB/s, from pages that keep a head's rows together: pieces of 128 bytes of a token's 1024 cost the rest); a
-// chunk of 2048 tokens over 30000 980 us, 1.06 PFLOP/s, as over 16-bit pages.  Widening each group once into 16-bit tiles, a
+// (bf16, D = 128, 32 / 8 heads): 64 requests of 64 - 8192 tokens 69 us (104 to 113 in 16 bits), 3.4 TB/s, where several caches are
+// read in turn (61 from one cache read again and again, most of which the last-level cache holds); 64 of 4096 119 to 129 us, 3.9 to 4.5
+// TB/s (112 to 118 from pages that keep a head's rows together: pieces of 128 bytes of a token's 1024 cost the rest); a
+// chunk of 2048 tokens over 30000 970 to 1000 us, 1.04 to 1.07 PFLOP/s, as over 16-bit pages.  Widening each group once into 16-bit tiles, a
 // quarter of the conversions, took 1072 us (trees at D = 64 5% slower).
 //
 // Trees (kTree): rows of a request see its context and the new tokens that their masks name, so all row tiles of a request
