@@ -23,6 +23,12 @@ def _views(form, dtype):
     if form == "pages hold all layers":
         x = x.view(PAGES, LAYERS, 2, PS, HK, D)
         return raw, [x[:, i, 0] for i in range(LAYERS)], [x[:, i, 1] for i in range(LAYERS)]
+    if form == "tokens hold all layers":
+        x = x.view(PAGES, PS, LAYERS, 2, HK, D)
+        return raw, [x[:, :, i, 0] for i in range(LAYERS)], [x[:, :, i, 1] for i in range(LAYERS)]
+    if form == "pages hold all layers, tokens keys and values":
+        x = x.view(PAGES, LAYERS, PS, 2, HK, D)
+        return raw, [x[:, i, :, 0] for i in range(LAYERS)], [x[:, i, :, 1] for i in range(LAYERS)]
     if form == "tokens hold keys and values":
         x = x.view(LAYERS, PAGES, PS, 2, HK, D)
         return raw, x[:, :, :, 0], x[:, :, :, 1]
@@ -39,7 +45,8 @@ def _views(form, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, E4M3])
 @pytest.mark.parametrize("form", ["pages hold all layers", "tokens hold keys and values", "heads hold keys and values",
-                                  "values by heads", "in turn"])
+                                  "values by heads", "in turn", "tokens hold all layers",
+                                  "pages hold all layers, tokens keys and values"])
 def test_move_kept_in_caches_of_one_storage(form, dtype):
     """Caches that lie between each other's rows are apart: each is moved as if it were alone."""
     raw, k, v = _views(form, dtype)

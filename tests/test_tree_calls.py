@@ -41,6 +41,14 @@ def _move(k, v, **kw):
     ([AT], [AT + 256], {}),
     ([AT], [AT + SIZE - 256], dict(v_ss=128, v_sh=16 * 128)),                          # of different layouts
     ([AT + i * 100 * SIZE for i in range(70)] + [AT], [AT + (i * 100 + 1) * SIZE for i in range(71)], {}),   # two launches
+    # 40 layers side by side in each page, or in each token, one of them twice, or values a head too early
+    ([AT + i % 39 * 2 * PAGE for i in range(40)], [AT + (2 * i + 1) * PAGE for i in range(40)], dict(k_sp=40 * PAGE, v_sp=40 * PAGE)),
+    ([AT + 2 * i * PAGE for i in range(40)], [AT + (2 * i + 1) * PAGE - 256 for i in range(40)], dict(k_sp=40 * PAGE, v_sp=40 * PAGE)),
+    ([AT + 1024 * i for i in range(40)], [AT + 1024 * (i % 39) + 512 for i in range(40)],
+     dict(k_sp=40 * PAGE, v_sp=40 * PAGE, k_ss=20480, v_ss=20480)),
+    ([AT + 1024 * i for i in range(40)], [AT + 1024 * i + 256 for i in range(40)],
+     dict(k_sp=40 * PAGE, v_sp=40 * PAGE, k_ss=20480, v_ss=20480)),
+    ([AT, AT + 256], [AT + SIZE, AT + 2 * SIZE], dict(k_sp=-4096)),                    # backwards
     (AT, AT, {}),
     (AT, AT + SIZE, {}),                                                               # the values are the second layer's keys
     (AT, AT + 2 * SIZE, dict(k_sl=0)),                                                 # layers by a stride that is none,
